@@ -56,6 +56,13 @@ class OutputParam(C.Structure):
                 ("to_tensor", vp), ("stream", vp)]
 
 
+class GatedNormParam(C.Structure):
+    _fields_ = [(n, vp) for n in (
+        "x", "bias", "residual", "gate", "batch_idx", "post_gamma", "post_beta", "pre_gamma", "pre_beta", "h_out",
+        "y_out", "y_mx", "m_ptr", "stream")] + [(n, i32) for n in (
+            "max_m", "n", "gate_rows", "post_norm", "pre_norm")] + [("residual_scale", C.c_float), ("eps", C.c_float)]
+
+
 # name -> (restype, argtypes); every symbol declared in include/et_b200.h
 SIGNATURES = {
     "et_create": (i32, [C.POINTER(Config), C.POINTER(vp)]),
@@ -116,6 +123,13 @@ SIGNATURES = {
     "et_gemm": (i32, [i32, vp, vp, vp, vp, vp, vp, i32, i32, i32, i32, i32, vp, vp]),
     "et_pack_weight": (i32, [i32, vp, vp, i32, i32, vp]),
     "et_split_tf32": (i32, [vp, vp, vp, vp, i32, i32, vp]),
+    "et_mxfp4_bytes": (C.c_size_t, [i32, i32]),
+    "et_mxfp4_quantize": (i32, [i32, vp, i64, vp, i32, i32, vp, vp]),
+    "et_mxfp4_dequantize": (i32, [i32, vp, vp, i32, i32, vp, vp]),
+    "et_mxfp4_pack_weight": (i32, [i32, vp, vp, i32, i32, vp]),
+    "et_mxfp4_gemm": (i32, [i32, vp, vp, vp, vp, vp, vp, vp, i32, i32, i32, i32, vp, vp]),
+    "et_mxfp4_linear": (i32, [i32, vp, i64, vp, vp, vp, vp, vp, vp, vp, i32, i32, i32, i32, vp, vp]),
+    "et_gated_residual_norm": (i32, [i32, C.POINTER(GatedNormParam)]),
     "et_gemm_fp32_tensor": (i32, [vp, vp, vp, vp, vp, vp, vp, i32, i32, i32, i32, vp, vp]),
 }
 

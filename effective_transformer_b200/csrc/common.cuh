@@ -116,7 +116,7 @@ inline cudaError_t launch_pdl(void (*kernel)(KArgs...), dim3 grid, dim3 block, s
 
 // ---- device status word ---------------------------------------------------
 // A kernel whose bounded wait expires records (kernel id << 8 | site) once.
-enum KernelId : int { kKernelGemmTc = 1, kKernelAttnTc = 2, kKernelSelfTest = 15 };
+enum KernelId : int { kKernelGemmTc = 1, kKernelAttnTc = 2, kKernelGemmMx = 3, kKernelSelfTest = 15 };
 
 __device__ __forceinline__ void report_timeout(int* status_word, int kernel_id, int site) {
   if (status_word != nullptr) atomicCAS(status_word, 0, (kernel_id << 8) | site);
@@ -512,6 +512,41 @@ struct SplitPlan {
 SplitPlan gemm_route(bool tf32, int rows, int n, int k, int epilogue);
 cudaError_t launch_gemm_split(const SplitGemm& g, int epilogue, const SplitPlan& plan, TensorMapCache* maps,
                               cudaStream_t stream);
+// MXFP4 (mxfp4.cuh): rows to 4 bits and back, weights [k, n] to the rows of their transpose, and the projection on
+// two such operands.  m_ptr null: max_m rows.  row_stride in elements.
+template <typename T>
+cudaError_t launch_mx_quantize(const T* x, long long row_stride, const int* m_ptr, int max_m, int k, void* mx,
+                               cudaStream_t stream);
+template <typename T>
+cudaError_t launch_mx_dequantize(const void* mx, const int* m_ptr, int max_m, int k, T* out, cudaStream_t stream);
+template <typename T>
+cudaError_t launch_mx_pack_weight(const T* w, void* mx, int k, int n, cudaStream_t stream);
+struct MxGemm {
+  const void* a = nullptr;
+  const void* w = nullptr;
+  void* c_mx = nullptr;  // MXFP4 output instead of c
+  const int* m_ptr = nullptr;
+  int max_m = 0, n = 0, k = 0;
+  int* status_word = nullptr;
+};
+// epilogue: kEpiNone to kEpiBiasTanh; residual (may be c) added behind the activation.
+template <typename T>
+cudaError_t launch_gemm_mxfp4(const MxGemm& p, const T* bias, const T* residual, T* c, int epilogue,
+                              cudaStream_t stream);
+// p = post(x + bias), h = residual_scale * residual + gate * p, y = pre(h): see norm_kernels.cu.
+struct GatedNorm {
+  const void *x = nullptr, *bias = nullptr, *residual = nullptr, *gate = nullptr;
+  const int* batch_idx = nullptr;
+  int gate_rows = 0;
+  float residual_scale = 1.f, eps = 1e-6f;
+  int post_kind = 0, pre_kind = 0;
+  const void *post_gamma = nullptr, *post_beta = nullptr, *pre_gamma = nullptr, *pre_beta = nullptr;
+  void *h = nullptr, *y = nullptr, *y_mx = nullptr;
+  const int* m_ptr = nullptr;
+  int max_m = 0, n = 0;
+};
+template <typename T>
+cudaError_t launch_gated_norm(const GatedNorm& p, cudaStream_t stream);
 // Whether the fused LayerNorm epilogues can serve a projection of n output columns.
 inline bool gemm_layernorm_supported(int n) { return n > 0 && n % 256 == 0 && n <= 1024; }
 

@@ -1,0 +1,200 @@
+// C ABI of the 4-bit projections and of the norms around a block (include/et_b200.h): argument checks and dispatch.
+#include "../../include/et_b200.h"
+
+#include "common.cuh"
+#include "mxfp4.cuh"
+
+using namespace etb;
+
+namespace {
+
+int refuse(const char* msg) {
+  set_global_error(msg);
+  return ET_INVALID_ARGUMENT;
+}
+
+int status_of(cudaError_t e, const char* what) {
+  if (e == cudaSuccess) return ET_OK;
+  set_global_error(std::string(what) + ": " + cudaGetErrorString(e));
+  return e == cudaErrorInvalidValue || e == cudaErrorMisalignedAddress ? ET_INVALID_ARGUMENT : ET_CUDA_ERROR;
+}
+
+// No C++ exception crosses the boundary (the error texts allocate).
+template <typename F>
+int guarded(F f) {
+  try {
+    return f();
+  } catch (...) {
+    return ET_CUDA_ERROR;
+  }
+}
+
+bool misaligned(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) != 0; }
+bool known_dtype(int dtype) { return dtype == ET_FP16 || dtype == ET_FP32; }
+size_t size_of(int dtype) { return dtype == ET_FP16 ? 2 : 4; }
+
+int check_width(int k) {
+  if (k <= 0 || k % kMxBlock != 0) return refuse("the width of an MXFP4 row must be a positive multiple of 32");
+  return ET_OK;
+}
+
+int check_gemm(int dtype, const void* a, const void* w_mx, const void* bias, const void* residual, const void* c,
+               const void* c_mx, int max_m, int n, int k, int epilogue) {
+  if (!known_dtype(dtype)) return refuse("dtype must be ET_FP16 or ET_FP32");
+  if (int rc = check_width(k)) return rc;
+  if (max_m < 0 || n <= 0 || n % 32 != 0) return refuse("max_m must not be negative, n a positive multiple of 32");
+  if (epilogue < kEpiNone || epilogue > kEpiBiasTanh) return refuse("epilogue must be 0 to 3");
+  if ((c == nullptr) == (c_mx == nullptr)) return refuse("exactly one of c and c_mx must be given");
+  if (c_mx != nullptr && (n % 64 != 0 || residual != nullptr))
+    return refuse("MXFP4 output needs n a multiple of 64 and takes no residual");
+  if (a == nullptr || w_mx == nullptr || (epilogue != kEpiNone && bias == nullptr)) return refuse("null pointer");
+  if (misaligned(a) || misaligned(w_mx) || misaligned(bias) || misaligned(residual) || misaligned(c) || misaligned(c_mx))
+    return refuse("pointers must be 16-byte aligned");
+  return ET_OK;
+}
+
+int run_gemm(int dtype, const void* a_mx, const void* w_mx, const void* bias, const void* residual, void* c, void* c_mx,
+             const int* m_ptr, int max_m, int n, int k, int epilogue, int* status_word, cudaStream_t s) {
+  MxGemm g;
+  g.a = a_mx, g.w = w_mx, g.c_mx = c_mx;
+  g.m_ptr = m_ptr, g.max_m = max_m, g.n = n, g.k = k;
+  g.status_word = status_word;
+  if (dtype == ET_FP16)
+    return status_of(launch_gemm_mxfp4<__half>(g, static_cast<const __half*>(bias), static_cast<const __half*>(residual),
+                                               static_cast<__half*>(c), epilogue, s),
+                     "et_mxfp4_gemm");
+  return status_of(launch_gemm_mxfp4<float>(g, static_cast<const float*>(bias), static_cast<const float*>(residual),
+                                            static_cast<float*>(c), epilogue, s),
+                   "et_mxfp4_gemm");
+}
+
+int run_quantize(int dtype, const void* x, long long row_stride, const int* m_ptr, int max_m, int k, void* mx,
+                 cudaStream_t s) {
+  if (dtype == ET_FP16)
+    return status_of(launch_mx_quantize<__half>(static_cast<const __half*>(x), row_stride, m_ptr, max_m, k, mx, s),
+                     "et_mxfp4_quantize");
+  return status_of(launch_mx_quantize<float>(static_cast<const float*>(x), row_stride, m_ptr, max_m, k, mx, s),
+                   "et_mxfp4_quantize");
+}
+
+}  // namespace
+
+extern "C" {
+
+size_t et_mxfp4_bytes(int rows, int k) {
+  if (rows < 0 || k <= 0 || k % kMxBlock != 0) return 0;
+  return mx_bytes(rows, k);
+}
+
+int et_mxfp4_quantize(int dtype, const void* x, long long row_stride, const int* m_ptr, int max_m, int k, void* mx,
+                      void* stream) {
+  return guarded([&] {
+    if (!known_dtype(dtype)) return refuse("dtype must be ET_FP16 or ET_FP32");
+    if (int rc = check_width(k)) return rc;
+    if (max_m < 0 || row_stride < k || row_stride * size_of(dtype) % 16 != 0)
+      return refuse("max_m must not be negative, row_stride at least k and a multiple of 16 bytes");
+    if (max_m == 0) return static_cast<int>(ET_OK);
+    if (x == nullptr || mx == nullptr) return refuse("null pointer");
+    if (misaligned(x) || misaligned(mx)) return refuse("pointers must be 16-byte aligned");
+    return run_quantize(dtype, x, row_stride, m_ptr, max_m, k, mx, static_cast<cudaStream_t>(stream));
+  });
+}
+
+int et_mxfp4_dequantize(int dtype, const void* mx, const int* m_ptr, int max_m, int k, void* out, void* stream) {
+  return guarded([&] {
+    if (!known_dtype(dtype)) return refuse("dtype must be ET_FP16 or ET_FP32");
+    if (int rc = check_width(k)) return rc;
+    if (max_m < 0) return refuse("max_m must not be negative");
+    if (max_m == 0) return static_cast<int>(ET_OK);
+    if (mx == nullptr || out == nullptr) return refuse("null pointer");
+    if (misaligned(mx) || misaligned(out)) return refuse("pointers must be 16-byte aligned");
+    cudaStream_t s = static_cast<cudaStream_t>(stream);
+    if (dtype == ET_FP16)
+      return status_of(launch_mx_dequantize<__half>(mx, m_ptr, max_m, k, static_cast<__half*>(out), s),
+                       "et_mxfp4_dequantize");
+    return status_of(launch_mx_dequantize<float>(mx, m_ptr, max_m, k, static_cast<float*>(out), s),
+                     "et_mxfp4_dequantize");
+  });
+}
+
+int et_mxfp4_pack_weight(int dtype, const void* w, void* w_mx, int k, int n, void* stream) {
+  return guarded([&] {
+    if (!known_dtype(dtype)) return refuse("dtype must be ET_FP16 or ET_FP32");
+    if (int rc = check_width(k)) return rc;
+    if (n <= 0 || n % 32 != 0) return refuse("n must be a positive multiple of 32");
+    if (w == nullptr || w_mx == nullptr) return refuse("null pointer");
+    if (misaligned(w_mx)) return refuse("pointers must be 16-byte aligned");
+    cudaStream_t s = static_cast<cudaStream_t>(stream);
+    if (dtype == ET_FP16)
+      return status_of(launch_mx_pack_weight<__half>(static_cast<const __half*>(w), w_mx, k, n, s),
+                       "et_mxfp4_pack_weight");
+    return status_of(launch_mx_pack_weight<float>(static_cast<const float*>(w), w_mx, k, n, s), "et_mxfp4_pack_weight");
+  });
+}
+
+int et_mxfp4_gemm(int dtype, const void* a_mx, const void* w_mx, const void* bias, const void* residual, void* c,
+                  void* c_mx, const int* m_ptr, int max_m, int n, int k, int epilogue, int* status_word, void* stream) {
+  return guarded([&] {
+    if (int rc = check_gemm(dtype, a_mx, w_mx, bias, residual, c, c_mx, max_m, n, k, epilogue)) return rc;
+    if (max_m == 0) return static_cast<int>(ET_OK);
+    return run_gemm(dtype, a_mx, w_mx, bias, residual, c, c_mx, m_ptr, max_m, n, k, epilogue, status_word,
+                    static_cast<cudaStream_t>(stream));
+  });
+}
+
+int et_mxfp4_linear(int dtype, const void* x, long long row_stride, void* x_mx, const void* w_mx, const void* bias,
+                    const void* residual, void* c, void* c_mx, const int* m_ptr, int max_m, int n, int k, int epilogue,
+                    int* status_word, void* stream) {
+  return guarded([&] {
+    if (int rc = check_gemm(dtype, x, w_mx, bias, residual, c, c_mx, max_m, n, k, epilogue)) return rc;
+    if (row_stride < k || row_stride * size_of(dtype) % 16 != 0)
+      return refuse("row_stride must be at least k and a multiple of 16 bytes");
+    if (max_m == 0) return static_cast<int>(ET_OK);
+    if (x_mx == nullptr || misaligned(x_mx)) return refuse("x_mx must be 16-byte aligned device memory");
+    cudaStream_t s = static_cast<cudaStream_t>(stream);
+    if (int rc = run_quantize(dtype, x, row_stride, m_ptr, max_m, k, x_mx, s)) return rc;
+    return run_gemm(dtype, x_mx, w_mx, bias, residual, c, c_mx, m_ptr, max_m, n, k, epilogue, status_word, s);
+  });
+}
+
+int et_gated_residual_norm(int dtype, const et_gated_norm_param_t* p) {
+  return guarded([&] {
+    if (!known_dtype(dtype)) return refuse("dtype must be ET_FP16 or ET_FP32");
+    if (p == nullptr) return refuse("null pointer");
+    const int elems = dtype == ET_FP16 ? 8 : 4;
+    if (p->max_m < 0 || p->n <= 0 || p->n % elems != 0)
+      return refuse("max_m must not be negative, n a positive multiple of 16 bytes");
+    if (p->n > 32 * 8 * 4 * elems) return refuse("n is limited to 8192 (ET_FP16) and 4096 (ET_FP32)");
+    if (p->post_norm < ET_NORM_NONE || p->post_norm > ET_NORM_RMS || p->pre_norm < ET_NORM_NONE ||
+        p->pre_norm > ET_NORM_RMS)
+      return refuse("post_norm and pre_norm must be ET_NORM_NONE, ET_NORM_LAYER or ET_NORM_RMS");
+    if ((p->post_norm != ET_NORM_NONE && !p->post_gamma) || (p->post_norm == ET_NORM_LAYER && !p->post_beta) ||
+        (p->pre_norm != ET_NORM_NONE && !p->pre_gamma) || (p->pre_norm == ET_NORM_LAYER && !p->pre_beta))
+      return refuse("a norm needs its gamma, a LayerNorm its beta too");
+    if (!p->h_out && !p->y_out && !p->y_mx) return refuse("at least one of h_out, y_out and y_mx must be given");
+    if (p->y_mx != nullptr && p->n % kMxBlock != 0) return refuse("y_mx needs n a multiple of 32");
+    if (p->gate != nullptr && (p->gate_rows < 1 || (p->gate_rows > 1 && !p->batch_idx)))
+      return refuse("gate needs gate_rows >= 1, and batch_idx with more than one row");
+    if (p->max_m == 0) return static_cast<int>(ET_OK);
+    if (p->x == nullptr) return refuse("null pointer");
+    for (const void* q : {p->x, p->bias, p->residual, p->gate, p->post_gamma, p->post_beta, p->pre_gamma, p->pre_beta,
+                          static_cast<const void*>(p->h_out), static_cast<const void*>(p->y_out),
+                          static_cast<const void*>(p->y_mx)})
+      if (misaligned(q)) return refuse("pointers must be 16-byte aligned");
+    GatedNorm g;
+    g.x = p->x, g.bias = p->bias, g.residual = p->residual, g.gate = p->gate;
+    g.batch_idx = p->gate_rows > 1 ? p->batch_idx : nullptr;
+    g.gate_rows = p->gate_rows;
+    g.residual_scale = p->residual_scale;
+    g.eps = p->eps > 0.f ? p->eps : 1e-6f;
+    g.post_kind = p->post_norm, g.pre_kind = p->pre_norm;
+    g.post_gamma = p->post_gamma, g.post_beta = p->post_beta, g.pre_gamma = p->pre_gamma, g.pre_beta = p->pre_beta;
+    g.h = p->h_out, g.y = p->y_out, g.y_mx = p->y_mx;
+    g.m_ptr = p->m_ptr, g.max_m = p->max_m, g.n = p->n;
+    cudaStream_t s = static_cast<cudaStream_t>(p->stream);
+    return dtype == ET_FP16 ? status_of(launch_gated_norm<__half>(g, s), "et_gated_residual_norm")
+                            : status_of(launch_gated_norm<float>(g, s), "et_gated_residual_norm");
+  });
+}
+
+}  // extern "C"

@@ -119,6 +119,14 @@ __device__ __forceinline__ void tma_load_3d(uint32_t smem_dst, const CUtensorMap
       : "memory");
 }
 
+// Untiled copy of `bytes` (a multiple of 16, both addresses 16-byte aligned), completion on an mbarrier of this CTA.
+__device__ __forceinline__ void bulk_load(uint32_t smem_dst, const void* src, uint32_t bytes, uint32_t bar) {
+  asm volatile(
+      "cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
+      ::"r"(smem_dst), "l"(src), "r"(bytes), "r"(bar)
+      : "memory");
+}
+
 // ---- tcgen05 / TMEM ----------------------------------------------------------
 __device__ __forceinline__ void tmem_alloc(uint32_t smem_slot, uint32_t ncols) {
   asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_slot),
@@ -241,6 +249,34 @@ __device__ __forceinline__ void umma_commit_pair(uint32_t bar_cluster_addr) {
   asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(
                    bar_cluster_addr)
                : "memory");
+}
+
+// ---- block-scaled MMA (kind::mxf4: e2m1 operands, one e8m0 scale per 32 values of K) ----
+// 512 bytes of scales (32 rows of 16 bytes, one 4-byte word per 32 operand rows) from shared memory into columns
+// [taddr, taddr + 4) of all four lane quadrants.  Ordered in front of the MMAs that the same thread issues after it.
+__device__ __forceinline__ void tmem_cp_scales(uint32_t taddr, uint64_t sdesc) {
+  asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(sdesc) : "memory");
+}
+// D[tmem] (+)= (A * scales of A)(B * scales of B), K = 64; which two of a word's four scales apply is in idesc.
+__device__ __forceinline__ void umma_mxf4_ss(uint32_t tmem_d, uint64_t adesc, uint64_t bdesc, uint32_t idesc,
+                                             uint32_t tmem_sfa, uint32_t tmem_sfb, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %6, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%4], [%5], p;\n\t}"
+      ::"r"(tmem_d), "l"(adesc), "l"(bdesc), "r"(idesc), "r"(tmem_sfa), "r"(tmem_sfb), "r"(accumulate)
+      : "memory");
+}
+// Descriptor of such a 512-byte piece: no swizzle, 8-row groups of 128 bytes one behind the other.
+__device__ __forceinline__ uint64_t make_scale_desc(uint32_t smem_addr) {
+  return static_cast<uint64_t>((smem_addr & 0x3FFFFu) >> 4) | (1ull << 16) | (8ull << 32) | (1ull << 46);
+}
+// Instruction descriptor for kind::mxf4, dense: bits [4,6) / [29,31) first byte of the scale words of B / A that
+// applies (0 or 2), [7,10) / [10,12) A / B format (1 = e2m1), [17,23) N >> 3, bit 23 scale format (1 = e8m0),
+// [24,29) M >> 4.
+__host__ __device__ constexpr uint32_t make_idesc_mxf4(int m, int n, int scale_byte) {
+  return (static_cast<uint32_t>(scale_byte) << 4) | (1u << 7) | (1u << 10) | (static_cast<uint32_t>(n >> 3) << 17) |
+         (1u << 23) | (static_cast<uint32_t>(m >> 4) << 24) | (static_cast<uint32_t>(scale_byte) << 29);
 }
 
 // Shared-memory matrix descriptor for a K-major operand tile laid out by TMA

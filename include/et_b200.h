@@ -577,6 +577,83 @@ int et_gemm_fp32_tensor(const float* a_hi, const float* a_lo, const float* w_hi,
                         const float* bias, float* c, const int* m_ptr, int max_m, int n, int k, int epilogue,
                         int* status_word, void* stream);
 
+/* ---- projections in 4-bit microscaled floating point (MXFP4) ---------------
+ * 32 consecutive values of a row share a power-of-two scale, each is a 4-bit
+ * float: 17 bytes per 32 values instead of 64 or 128, and a tensor-core rate
+ * four times that of fp16.  The scale of a block is
+ * 2^(floor(log2 max|x|) - 2), at least 2^-127; a value is rounded to the nearest
+ * of 0, 0.5, 1, 1.5, 2, 3, 4, 6 times the scale (ties to the even code) and
+ * saturates at 6; a block with an infinity or a NaN reads as NaN throughout.
+ * No reference counterpart.
+ *
+ * An MXFP4 tensor of `rows` rows of k values (k a multiple of 32) is an opaque
+ * buffer of et_mxfp4_bytes(rows, k) bytes of device memory, 16-byte aligned
+ * (0 for shapes that are not served).  It holds rows in the form the tensor
+ * core reads: tiles of 128 rows x 256 values with their scales.
+ *
+ * dtype is the element type of what is not MXFP4 (x, w, bias, residual, c, out);
+ * m_ptr is a DEVICE pointer to the number of valid rows, NULL = all max_m; rows
+ * past it are neither read nor written.  All pointers 16-byte aligned.  The text
+ * of a refusal is et_last_error(NULL).  Calls that overlap on the GPU may share
+ * what they only read. */
+size_t et_mxfp4_bytes(int rows, int k);
+/* x [max_m, k] with row_stride elements between rows (a multiple of 16 bytes) -> MXFP4. */
+int et_mxfp4_quantize(int dtype, const void* x, long long row_stride, const int* m_ptr, int max_m, int k, void* mx,
+                      void* stream);
+/* The values an MXFP4 tensor stands for, rounded to dtype: out [max_m, k]. */
+int et_mxfp4_dequantize(int dtype, const void* mx, const int* m_ptr, int max_m, int k, void* out, void* stream);
+/* w [k, n] ([in, out], as et_pack_weight; n a multiple of 32) -> the MXFP4 tensor of n rows of
+ * et_mxfp4_bytes(n, k) bytes that the products take; scales run along k. */
+int et_mxfp4_pack_weight(int dtype, const void* w, void* w_mx, int k, int n, void* stream);
+/* C[m, n] = act(A W + bias) (+ residual): A of max_m rows of k values, W^T as et_mxfp4_pack_weight
+ * made it, fp32 accumulation, one rounding at the end.  epilogue as for et_gemm (0 none, 1 +bias,
+ * 2 gelu(+bias), 3 tanh(+bias)); residual [max_m, n] or NULL, may be c.  Exactly one of c [max_m, n]
+ * and c_mx (the result as MXFP4, the operand of the next product: n a multiple of 64, no residual)
+ * is given. */
+int et_mxfp4_gemm(int dtype, const void* a_mx, const void* w_mx, const void* bias, const void* residual, void* c,
+                  void* c_mx, const int* m_ptr, int max_m, int n, int k, int epilogue, int* status_word, void* stream);
+/* et_mxfp4_quantize into x_mx (workspace of et_mxfp4_bytes(max_m, k) bytes) and et_mxfp4_gemm in one call. */
+int et_mxfp4_linear(int dtype, const void* x, long long row_stride, void* x_mx, const void* w_mx, const void* bias,
+                    const void* residual, void* c, void* c_mx, const int* m_ptr, int max_m, int n, int k, int epilogue,
+                    int* status_word, void* stream);
+
+/* ---- norms before and after a block, fused with its gate and residual scale --
+ *   p = post(x + bias)
+ *   h = residual_scale * residual + gate * p
+ *   y = pre(h)
+ * per row, in fp32, each output rounded once.  post and pre: ET_NORM_NONE,
+ * ET_NORM_LAYER ((v - mean) * rsqrt(var + eps) * gamma + beta) or ET_NORM_RMS
+ * (v * rsqrt(mean(v^2) + eps) * gamma).  With post none, no gate and scale 1 it
+ * is the post-norm encoder's add_bias_input_layernorm
+ * (cuda/cuda_kernels.cu:157-271), out of place.  y_mx takes y as MXFP4, straight
+ * into the projection behind it.  Rows past *m_ptr are left as they are. */
+enum { ET_NORM_NONE = 0, ET_NORM_LAYER = 1, ET_NORM_RMS = 2 };
+typedef struct {
+  const void* x;          /* [max_m, n] block output */
+  const void* bias;       /* [n] or NULL */
+  const void* residual;   /* [max_m, n] or NULL (then h = gate * p) */
+  const void* gate;       /* [gate_rows, n] or NULL */
+  const int* batch_idx;   /* [max_m] gate row of every row (et_padding_offsets); unused with gate_rows <= 1.
+                           * A row whose entry is outside [0, gate_rows) has gate 0. */
+  const void* post_gamma; /* [n] each */
+  const void* post_beta;
+  const void* pre_gamma;
+  const void* pre_beta;
+  void* h_out;            /* [max_m, n] or NULL; may be x or residual */
+  void* y_out;            /* [max_m, n] or NULL; may be x or residual, not h_out */
+  void* y_mx;             /* MXFP4 tensor of max_m rows or NULL (n a multiple of 32) */
+  const int* m_ptr;       /* device row count, NULL = max_m */
+  void* stream;
+  int max_m;
+  int n;                  /* a multiple of 16 bytes, at most 8192 (ET_FP16) or 4096 (ET_FP32) */
+  int gate_rows;
+  int post_norm;
+  int pre_norm;
+  float residual_scale;
+  float eps;              /* <= 0 selects 1e-6 */
+} et_gated_norm_param_t;
+int et_gated_residual_norm(int dtype, const et_gated_norm_param_t* param);
+
 #ifdef __cplusplus
 }
 #endif

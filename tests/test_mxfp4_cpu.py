@@ -1,0 +1,149 @@
+"""The 4-bit operators without a GPU: the oracle against a search over all codes, sizes, and every refusal."""
+import ctypes as C
+
+import numpy as np
+import pytest
+import torch
+
+import mx_oracle as X
+from effective_transformer_b200 import _capi, mxfp4, norms
+
+LIB = _capi.load()
+BAD = _capi.ET_INVALID_ARGUMENT
+P = 1 << 20  # an aligned address that no refused call reads
+
+
+def nearest(x, scale):
+    """Code of |x| by search: the nearest grid value, of two equally near ones the even code."""
+    d = np.abs(abs(x) / scale - X.GRID)
+    best = np.flatnonzero(d == d.min())
+    return int(best[0] if len(best) == 1 else best[best % 2 == 0][0])
+
+
+def test_oracle_rounds_to_the_nearest_code():
+    rng = np.random.RandomState(0)
+    x = rng.randn(3, 64).astype(np.float32)
+    x[1, :32] = np.arange(32) / 4            # 0.25 steps up to 7.75: every tie, and saturation
+    x[2] = 0.0
+    codes, scales = X.mx_parts(x)
+    for r in range(3):
+        for b in range(2):
+            block = x[r, b * 32:b * 32 + 32]
+            top = np.abs(block).max()
+            e = np.floor(np.log2(top)) - 2 if top > 0 else -127
+            assert scales[r, b] == e + 127
+            assert [c & 7 for c in codes[r, b * 32:b * 32 + 32]] == [nearest(v, 2.0 ** e) for v in block]
+
+
+def test_bytes():
+    for rows, k in ((0, 32), (1, 32), (128, 256), (129, 256), (128, 288), (40000, 4096), (2 ** 31 - 1, 65536)):
+        assert LIB.et_mxfp4_bytes(rows, k) == X.mx_bytes(rows, k)
+    for rows, k in ((-1, 32), (1, 0), (1, 16), (1, -32), (1, 33)):
+        assert LIB.et_mxfp4_bytes(rows, k) == 0
+
+
+def refused(rc, text):
+    assert rc == BAD
+    assert text in LIB.et_last_error(None).decode()
+
+
+@pytest.mark.parametrize("change,text", [
+    (dict(dtype=2), "dtype"), (dict(k=0), "multiple of 32"), (dict(k=48), "multiple of 32"), (dict(m=-1), "negative"),
+    (dict(stride=32), "row_stride"), (dict(stride=68), "row_stride"), (dict(x=None), "null"), (dict(mx=None), "null"),
+    (dict(x=P + 8), "aligned"), (dict(mx=P + 4), "aligned")])
+def test_quantize_refusals(change, text):
+    a = dict(dtype=1, x=P, stride=64, m=5, k=64, mx=P)
+    a.update(change)
+    refused(LIB.et_mxfp4_quantize(a["dtype"], a["x"], a["stride"], None, a["m"], a["k"], a["mx"], None), text)
+
+
+@pytest.mark.parametrize("change,text", [
+    (dict(dtype=-1), "dtype"), (dict(k=31), "multiple of 32"), (dict(m=-1), "negative"), (dict(out=None), "null"),
+    (dict(mx=None), "null"), (dict(out=P + 2), "aligned")])
+def test_dequantize_refusals(change, text):
+    a = dict(dtype=0, mx=P, m=5, k=64, out=P)
+    a.update(change)
+    refused(LIB.et_mxfp4_dequantize(a["dtype"], a["mx"], None, a["m"], a["k"], a["out"], None), text)
+
+
+@pytest.mark.parametrize("change,text", [
+    (dict(dtype=3), "dtype"), (dict(k=40), "multiple of 32"), (dict(n=0), "n must"), (dict(n=40), "n must"),
+    (dict(w=None), "null"), (dict(mx=None), "null"), (dict(mx=P + 1), "aligned")])
+def test_pack_weight_refusals(change, text):
+    a = dict(dtype=1, w=P, mx=P, k=64, n=64)
+    a.update(change)
+    refused(LIB.et_mxfp4_pack_weight(a["dtype"], a["w"], a["mx"], a["k"], a["n"], None), text)
+
+
+GEMM_BAD = [
+    (dict(dtype=5), "dtype"), (dict(k=0), "multiple of 32"), (dict(k=72), "multiple of 32"), (dict(n=48), "n a"),
+    (dict(n=0), "n a"), (dict(m=-3), "negative"), (dict(epi=4), "epilogue"), (dict(epi=-1), "epilogue"),
+    (dict(c=None), "exactly one"), (dict(c_mx=P), "exactly one"), (dict(c=None, c_mx=P, n=96), "multiple of 64"),
+    (dict(c=None, c_mx=P, residual=P), "no residual"), (dict(a=None), "null"), (dict(w=None), "null"),
+    (dict(epi=2, bias=None), "null"), (dict(a=P + 8), "aligned"), (dict(w=P + 8), "aligned"), (dict(c=P + 2), "aligned"),
+    (dict(bias=P + 2, epi=1), "aligned"), (dict(residual=P + 2), "aligned")]
+
+
+@pytest.mark.parametrize("change,text", GEMM_BAD)
+def test_gemm_refusals(change, text):
+    a = dict(dtype=1, a=P, w=P, bias=None, residual=None, c=P, c_mx=None, m=3, n=64, k=64, epi=0)
+    a.update(change)
+    refused(LIB.et_mxfp4_gemm(a["dtype"], a["a"], a["w"], a["bias"], a["residual"], a["c"], a["c_mx"], None, a["m"],
+                              a["n"], a["k"], a["epi"], None, None), text)
+
+
+@pytest.mark.parametrize("change,text", GEMM_BAD + [
+    (dict(stride=32), "row_stride"), (dict(stride=67), "row_stride"), (dict(x_mx=None), "x_mx"), (dict(x_mx=P + 8), "x_mx")])
+def test_linear_refusals(change, text):
+    a = dict(dtype=1, a=P, stride=64, x_mx=P, w=P, bias=None, residual=None, c=P, c_mx=None, m=3, n=64, k=64, epi=0)
+    a.update(change)
+    refused(LIB.et_mxfp4_linear(a["dtype"], a["a"], a["stride"], a["x_mx"], a["w"], a["bias"], a["residual"], a["c"],
+                                a["c_mx"], None, a["m"], a["n"], a["k"], a["epi"], None, None), text)
+
+
+NORM_BAD = [
+    (dict(max_m=-1), "negative"), (dict(n=0), "16 bytes"), (dict(n=12), "16 bytes"), (dict(n=8200), "limited"),
+    (dict(post_norm=3), "post_norm"), (dict(pre_norm=-1), "pre_norm"), (dict(post_norm=1), "gamma"),
+    (dict(post_norm=1, post_gamma=P), "gamma"), (dict(post_norm=2), "gamma"), (dict(pre_norm=1), "gamma"),
+    (dict(h_out=None), "at least one"), (dict(y_mx=P, n=48), "multiple of 32"), (dict(gate=P, gate_rows=0), "gate"),
+    (dict(gate=P, gate_rows=2), "gate"), (dict(x=None), "null"), (dict(x=P + 8), "aligned"),
+    (dict(residual=P + 4), "aligned"), (dict(gate=P + 2, gate_rows=1), "aligned"), (dict(y_out=P + 2), "aligned")]
+
+
+@pytest.mark.parametrize("change,text", NORM_BAD)
+def test_norm_refusals(change, text):
+    p = _capi.GatedNormParam()
+    p.x, p.h_out, p.max_m, p.n, p.residual_scale = P, P, 4, 64, 1.0
+    for k, v in change.items():
+        setattr(p, k, v)
+    refused(LIB.et_gated_residual_norm(1, C.byref(p)), text)
+
+
+def test_norm_refuses_types_and_null():
+    p = _capi.GatedNormParam()
+    refused(LIB.et_gated_residual_norm(9, C.byref(p)), "dtype")
+    refused(LIB.et_gated_residual_norm(1, None), "null")
+    p.x, p.h_out, p.max_m, p.n = P, P, 4, 4100
+    refused(LIB.et_gated_residual_norm(0, C.byref(p)), "limited")
+
+
+def test_empty_batches_are_fine():
+    assert LIB.et_mxfp4_quantize(1, None, 64, None, 0, 64, None, None) == 0
+    assert LIB.et_mxfp4_dequantize(1, None, None, 0, 64, None, None) == 0
+    assert LIB.et_mxfp4_gemm(1, P, P, None, None, P, None, None, 0, 64, 64, 0, None, None) == 0
+    p = _capi.GatedNormParam()
+    p.h_out, p.n = P, 64
+    assert LIB.et_gated_residual_norm(1, C.byref(p)) == 0
+
+
+def test_python_refuses_before_any_launch():
+    x = torch.zeros(4, 64, dtype=torch.float16)
+    w = mxfp4.MxTensor(torch.zeros(17408, dtype=torch.uint8), 64, 64)
+    for call in (lambda: mxfp4.quantize(x), lambda: mxfp4.linear(x, w), lambda: mxfp4.pack_weight(x),
+                 lambda: norms.gated_residual_norm(x), lambda: mxfp4.dequantize(w, torch.bfloat16),
+                 lambda: mxfp4.dequantize(x, torch.float16), lambda: mxfp4.gemm(x, w), lambda: mxfp4.gemm(w, x),
+                 lambda: mxfp4.empty(-1, 64, "cpu"), lambda: mxfp4.empty(1, 40, "cpu"),
+                 lambda: mxfp4.gemm(w, mxfp4.MxTensor(w.data, 64, 96))):
+        with pytest.raises(ValueError):
+            call()
+    assert mxfp4.empty(129, 288, "cpu").data.numel() == X.mx_bytes(129, 288)

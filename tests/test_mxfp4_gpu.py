@@ -1,0 +1,310 @@
+"""The 4-bit operators on the GPU against float64.
+
+Quantisation is exact: codes and scales are compared bit by bit.  In a product every term is exact; the fp32 sum of K
+terms is off by at most K steps of 2^-23 of sum |a w| (a step each if the adder truncates), the result is rounded once
+(half a step: 2^-11 of it in fp16, 2^-24 in fp32), and the activations pass an error on with a slope of at most 1.13.
+Their own errors: GELU in fp32 1e-5 of the value; its tanh in fp16 results is the hardware's, documented as 2^-11
+relative, so 0.5 |x| 2^-11; tanhf 2^-22.
+"""
+import numpy as np
+import pytest
+import torch
+
+import mx_oracle as X
+from effective_transformer_b200 import _capi, mxfp4
+
+pytestmark = pytest.mark.gpu
+NP = {torch.float16: np.float16, torch.float32: np.float32}
+DTYPES = [torch.float16, torch.float32]
+
+
+def rows_of(rng, rows, k, dtype, spread=True):
+    x = rng.randn(rows, k)
+    if spread:
+        x *= np.exp2(rng.randint(-6, 7, size=(rows, max(1, k // 32)))).repeat(32, axis=1)[:, :k]
+    return x.astype(NP[dtype])
+
+
+def cuda(a):
+    return torch.from_numpy(np.ascontiguousarray(a)).cuda()
+
+
+def count(n):
+    return torch.full((1,), n, dtype=torch.int32, device="cuda")
+
+
+def same_parts(mx, x):
+    codes, scales = X.mx_parts(x)
+    got_codes, got_scales = X.mx_unpack(mx.data.cpu().numpy(), x.shape[0], x.shape[1])
+    assert np.array_equal(got_scales, scales)
+    assert np.array_equal(got_codes, codes)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rows,k", [(1, 32), (1, 1024), (7, 96), (33, 256), (128, 288), (129, 768), (300, 2080),
+                                    (1000, 1024)])
+def test_quantize(dtype, rows, k):
+    x = rows_of(np.random.RandomState(rows + k), rows, k, dtype)
+    mx = mxfp4.quantize(cuda(x))
+    same_parts(mx, x)
+    back = mxfp4.dequantize(mx, torch.float32).cpu().numpy()
+    assert np.array_equal(back, X.mx_values(x).astype(np.float32))
+    assert np.array_equal(mxfp4.dequantize(mx, torch.float16).cpu().numpy(), X.mx_values(x).astype(np.float16))
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_quantize_ties_ranges_and_specials(dtype):
+    t = NP[dtype]
+    x = np.zeros((12, 64), t)
+    x[0] = np.arange(64) / 8                                  # ties and saturation, scale 1 and 1
+    x[1] = -x[0]
+    x[2] = np.finfo(t).max
+    x[3] = np.finfo(t).smallest_subnormal
+    x[4, ::2] = np.finfo(t).tiny
+    x[5, 5] = np.inf
+    x[6, 40] = -np.inf
+    x[7, 63] = np.nan
+    x[8, :32] = np.linspace(-7.9, 7.9, 32)
+    x[9] = -0.0
+    x[10, 0], x[10, 1:32] = 4096, np.linspace(1, 600, 31)     # a value that dwarfs its block
+    x[11] = np.float64(np.finfo(t).smallest_subnormal) * np.arange(64)
+    mx = mxfp4.quantize(cuda(x))
+    same_parts(mx, x)
+    want = X.mx_values(x)
+    got = mxfp4.dequantize(mx, torch.float32).cpu().numpy()
+    assert np.array_equal(got, want.astype(np.float32), equal_nan=True)
+    assert np.isnan(got[5, :32]).all() and not np.isnan(got[5, 32:]).any()
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_quantize_strided_rows_and_rows_past_the_count(dtype):
+    rng = np.random.RandomState(3)
+    wide = cuda(rows_of(rng, 200, 3 * 96, dtype))
+    x = wide[:, 96:192]                                        # a head group of a fused projection's rows
+    mx = mxfp4.empty(200, 96)
+    mx.data.fill_(0xAB)
+    mxfp4.quantize(x, valid_rows=count(133), out=mx)
+    codes, scales = X.mx_unpack(mx.data.cpu().numpy(), 200, 96)
+    want_codes, want_scales = X.mx_parts(x[:133].cpu().numpy())
+    assert np.array_equal(codes[:133], want_codes) and np.array_equal(scales[:133], want_scales)
+    assert (scales[133:] == 0xAB).all() and (codes[133:, 0::2] == 0xB).all() and (codes[133:, 1::2] == 0xA).all()
+    out = torch.full((200, 96), 7.0, dtype=dtype, device="cuda")
+    mxfp4.dequantize(mx, dtype, valid_rows=count(100), out=out)
+    assert torch.equal(out[:100].cpu().double(), torch.from_numpy(X.mx_values(x[:100].cpu().numpy())))
+    assert (out[100:] == 7.0).all()
+    for n in (0, -5):
+        mx.data.fill_(0xAB)
+        mxfp4.quantize(x, valid_rows=count(n), out=mx)
+        assert (mx.data == 0xAB).all()
+    mxfp4.quantize(x, valid_rows=count(10 ** 6), out=mx)       # a count past the capacity is the capacity
+    same_parts(mx, x.cpu().numpy())
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("k,n", [(32, 32), (96, 160), (768, 128), (800, 2304)])
+def test_pack_weight(dtype, k, n):
+    w = rows_of(np.random.RandomState(k + n), n, k, dtype).T.copy()
+    mx = mxfp4.pack_weight(cuda(w))
+    assert (mx.rows, mx.cols) == (n, k)
+    same_parts(mx, np.ascontiguousarray(w.T))
+
+
+def reference(x, kernel, bias, act, residual, dtype):
+    """(result, bound on |error|) in float64, on the GPU."""
+    a, w = cuda(X.mx_values(x)), cuda(X.mx_values(np.ascontiguousarray(kernel.T)))
+    k = x.shape[1]
+    y = a @ w.t()
+    err = (k + 8) * 2.0 ** -23 * (a.abs() @ w.abs().t())
+    if bias is not None:
+        y = y + bias.double()
+        err = err + 2.0 ** -24 * y.abs()
+    if act == "gelu":
+        u = y
+        y = X.gelu(u)
+        err = 1.13 * err + 1e-5 * y.abs() + (0.5 * u.abs() * 2.0 ** -11 if dtype == torch.float16 else 0)
+    elif act == "tanh":
+        y = y.tanh()
+        err = err + 2.0 ** -22
+    if residual is not None:
+        y = y + residual.double()
+        err = err + 2.0 ** -24 * y.abs()
+    half_step = 2.0 ** -11 if dtype == torch.float16 else 2.0 ** -24
+    return y, err + half_step * (y.abs() + err) + 2.0 ** -25  # (half a step of fp16 subnormals)
+
+
+def product_case(seed, m, k, n, dtype, act, with_bias, with_residual, spread=False):
+    rng = np.random.RandomState(seed)
+    x = rows_of(rng, m, k, dtype, spread)
+    kernel = (rng.randn(k, n) * 0.05).astype(NP[dtype])
+    bias = cuda((rng.randn(n) * 0.3).astype(NP[dtype])) if with_bias else None
+    residual = cuda(rng.randn(m, n).astype(NP[dtype])) if with_residual else None
+    return x, kernel, bias, residual, reference(x, kernel, bias, act, residual, dtype)
+
+
+SHAPES = [(1, 32, 32), (1, 1024, 1024), (3, 64, 64), (37, 96, 160), (64, 768, 2304), (128, 256, 128), (129, 800, 96),
+          (200, 1056, 288), (513, 128, 4096), (1000, 2048, 512)]
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("m,k,n", SHAPES)
+def test_product(dtype, m, k, n):
+    x, kernel, bias, _, (want, bound) = product_case(m + k + n, m, k, n, dtype, None, True, False)
+    a, w = mxfp4.quantize(cuda(x)), mxfp4.pack_weight(cuda(kernel))
+    got = mxfp4.gemm(a, w, bias=bias)
+    assert got.dtype == dtype and got.shape == (m, n)
+    assert ((got.double() - want).abs() <= bound).all()
+    assert mxfp4.device_status() == 0
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("act", [None, "gelu", "tanh"])
+@pytest.mark.parametrize("with_residual", [False, True])
+@pytest.mark.parametrize("m,k,n", [(5, 128, 96), (300, 512, 640)])
+def test_epilogues(dtype, act, with_residual, m, k, n):
+    x, kernel, bias, residual, (want, bound) = product_case(17, m, k, n, dtype, act, True, with_residual, True)
+    w = mxfp4.pack_weight(cuda(kernel))
+    got = mxfp4.linear(cuda(x), w, bias=bias, activation=act, residual=residual)
+    assert ((got.double() - want).abs() <= bound).all()
+    if residual is not None:                                    # in place on the residual
+        same = mxfp4.linear(cuda(x), w, bias=bias, activation=act, residual=residual, out=residual)
+        assert same is residual and torch.equal(residual, got)
+
+
+@pytest.mark.parametrize("m,k,n", [(1, 512, 256), (130, 1024, 512), (700, 320, 1024)])
+def test_products_of_small_numbers_are_exact(m, k, n):
+    """Operands of one scale: sums of multiples of 2^-2 below 2^16 fit 24 bits, whatever the order."""
+    rng = np.random.RandomState(m)
+    x = rng.choice(np.concatenate([X.GRID, -X.GRID]), size=(m, k)).astype(np.float32)
+    kernel = rng.choice(np.concatenate([X.GRID, -X.GRID]), size=(k, n)).astype(np.float32)
+    x[:, ::32], kernel[::32] = 6.0, -6.0                        # every block has scale 1
+    got = mxfp4.gemm(mxfp4.quantize(cuda(x)), mxfp4.pack_weight(cuda(kernel)), dtype=torch.float32)
+    assert torch.equal(got.double(), cuda(x).double() @ cuda(kernel).double())
+
+
+@pytest.mark.parametrize("m,k,n", [(1, 256, 64), (77, 768, 320), (300, 512, 1024)])
+@pytest.mark.parametrize("act", [None, "gelu"])
+def test_product_in_4_bits(m, k, n, act):
+    """c_mx is the quantised form of the fp32 result: scales and codes agree except where the fp32 result lies within
+    its bound of a border, and there they are off by one code."""
+    x, kernel, bias, _, _ = product_case(5, m, k, n, torch.float16, None, True, False)
+    a, w = mxfp4.quantize(cuda(x)), mxfp4.pack_weight(cuda(kernel))
+    out = mxfp4.gemm(a, w, bias=bias, activation=act, out=mxfp4.empty(m, n))
+    want, bound = reference(x, kernel, bias, act, None, torch.float32)
+    got = mxfp4.dequantize(out, torch.float32).cpu().numpy()
+    lo, hi = (want - bound).cpu().numpy(), (want + bound).cpu().numpy()
+    top_lo = np.abs(want.cpu().numpy()).reshape(m, -1, 32).max(-1) - bound.cpu().numpy().reshape(m, -1, 32).max(-1)
+    top_hi = np.abs(want.cpu().numpy()).reshape(m, -1, 32).max(-1) + bound.cpu().numpy().reshape(m, -1, 32).max(-1)
+    _, scales = X.mx_unpack(out.data.cpu().numpy(), m, n)
+    e = scales.astype(np.float64) - 127 + 2
+    assert (np.floor(np.log2(np.maximum(top_lo, 1e-30))) <= e).all() and (e <= np.floor(np.log2(top_hi))).all()
+
+    def code_values(v):                                         # rounded on the scales that came back
+        s = np.exp2(scales.astype(np.float64) - 127).repeat(32, axis=1)
+        q = np.abs(v) / s
+        c = np.zeros(q.shape, int)
+        for i in range(7):
+            mid = (X.GRID[i] + X.GRID[i + 1]) / 2
+            c += (q > mid) if i % 2 == 0 else (q >= mid)
+        return np.copysign(X.GRID[c], v) * s
+
+    assert (got >= code_values(lo)).all() and (got <= code_values(hi)).all()
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_rows_past_the_count_are_left_alone(dtype):
+    x, kernel, bias, _, (want, bound) = product_case(23, 400, 288, 224, dtype, None, True, False)
+    w = mxfp4.pack_weight(cuda(kernel))
+    for valid in (0, 1, 127, 128, 129, 399, 400, 1000):
+        xt = cuda(x)
+        xt[valid:] = float("nan")
+        out = torch.full((400, 224), 3.0, dtype=dtype, device="cuda")
+        mxfp4.linear(xt, w, bias=bias, valid_rows=count(valid), out=out)
+        t = min(valid, 400)
+        assert ((out[:t].double() - want[:t]).abs() <= bound[:t]).all()
+        assert (out[t:] == 3.0).all()
+    small = mxfp4.empty(400, 64)
+    small.data.fill_(0xCD)
+    w64 = mxfp4.pack_weight(cuda(kernel[:, :64].copy()))
+    mxfp4.linear(cuda(x), w64, valid_rows=count(250), out=small)
+    codes, scales = X.mx_unpack(small.data.cpu().numpy(), 400, 64)
+    assert (scales[250:] == 0xCD).all() and (codes[250:, 0::2] == 0xD).all() and (codes[250:, 1::2] == 0xC).all()
+
+
+def test_non_finite_rows_stay_in_their_rows():
+    x, kernel, bias, _, (want, bound) = product_case(29, 140, 512, 160, torch.float16, None, True, False)
+    x[3, 100], x[130, 0] = np.inf, np.nan
+    got = mxfp4.linear(cuda(x), mxfp4.pack_weight(cuda(kernel)), bias=bias)
+    bad = torch.zeros(140, dtype=torch.bool, device="cuda")
+    bad[[3, 130]] = True
+    assert got[bad].isnan().all()
+    assert ((got[~bad].double() - want[~bad]).abs() <= bound[~bad]).all()
+    kernel[7, 5] = np.nan                                       # and in the column of a weight
+    got = mxfp4.linear(cuda(x), mxfp4.pack_weight(cuda(kernel)), bias=bias)
+    assert got[:, 5].isnan().all() and not got[~bad][:, [4, 6]].isnan().any()
+
+
+def test_results_repeat_bit_by_bit():
+    x, kernel, bias, _, _ = product_case(31, 300, 1024, 256, torch.float16, None, True, False)
+    w = mxfp4.pack_weight(cuda(kernel))
+    first = mxfp4.linear(cuda(x), w, bias=bias)
+    for _ in range(3):
+        assert torch.equal(mxfp4.linear(cuda(x), w, bias=bias), first)
+
+
+def test_other_streams_and_capture():
+    x, kernel, bias, _, (want, bound) = product_case(37, 90, 768, 256, torch.float16, "gelu", True, False)
+    w, xt = mxfp4.pack_weight(cuda(kernel)), cuda(x)
+    mxfp4.device_status()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        got = mxfp4.linear(xt, w, bias=bias, activation="gelu")
+    torch.cuda.current_stream().wait_stream(side)
+    assert ((got.double() - want).abs() <= bound).all()
+    ws, out, valid = mxfp4.empty(90, 768), torch.zeros(90, 256, dtype=torch.float16, device="cuda"), count(90)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        mxfp4.linear(xt, w, bias=bias, activation="gelu", valid_rows=valid, workspace=ws, out=out)
+    for rows in (90, 11, 64):
+        out.zero_()
+        valid.fill_(rows)
+        graph.replay()
+        assert ((out[:rows].double() - want[:rows]).abs() <= bound[:rows]).all() and (out[rows:] == 0).all()
+
+
+def test_capture_needs_a_status_word_first():
+    word = mxfp4._status.pop(torch.cuda.current_device(), None)
+    try:
+        a = mxfp4.empty(4, 64)
+        w = mxfp4.empty(64, 64)
+        out = torch.zeros(4, 64, dtype=torch.float16, device="cuda")
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            torch.zeros(1, device="cuda")
+            with pytest.raises(ValueError, match="captured"):
+                mxfp4.gemm(a, w, out=out)
+    finally:
+        if word is not None:
+            mxfp4._status[torch.cuda.current_device()] = word
+
+
+def test_python_refusals_on_the_gpu():
+    x = torch.zeros(4, 64, dtype=torch.float16, device="cuda")
+    w = mxfp4.pack_weight(torch.zeros(64, 96, dtype=torch.float16, device="cuda"))
+    b = torch.zeros(96, dtype=torch.float16, device="cuda")
+    a = mxfp4.quantize(x)
+    for call in (lambda: mxfp4.quantize(x[:, :33]), lambda: mxfp4.quantize(x.t()), lambda: mxfp4.quantize(x.double()),
+                 lambda: mxfp4.quantize(x, out=mxfp4.empty(3, 64)), lambda: mxfp4.quantize(x, out=mxfp4.empty(4, 96)),
+                 lambda: mxfp4.quantize(x, valid_rows=torch.ones(1, device="cuda")),
+                 lambda: mxfp4.quantize(x, valid_rows=torch.ones(1, dtype=torch.int32)),
+                 lambda: mxfp4.linear(x, w, activation="gelu"), lambda: mxfp4.linear(x, w, bias=b, activation="relu"),
+                 lambda: mxfp4.linear(x, w, bias=b.float()), lambda: mxfp4.linear(x, w, bias=b[:64]),
+                 lambda: mxfp4.linear(x, w, residual=x), lambda: mxfp4.linear(x, w, out=mxfp4.empty(4, 96)),
+                 lambda: mxfp4.linear(x, w, out=torch.zeros(4, 96, device="cuda")),
+                 lambda: mxfp4.gemm(a, w, out=torch.zeros(5, 96, dtype=torch.float16, device="cuda")),
+                 lambda: mxfp4.gemm(a, mxfp4.pack_weight(torch.zeros(96, 64, dtype=torch.float16, device="cuda"))),
+                 lambda: mxfp4.dequantize(a, torch.float16, out=torch.zeros(5, 64, dtype=torch.float16, device="cuda"))):
+        with pytest.raises(ValueError):
+            call()
+    with pytest.raises(_capi.EtError):                          # rows that start between two 16-byte boundaries
+        mxfp4.quantize(torch.zeros(4 * 64 + 4, dtype=torch.float16, device="cuda")[4:].view(4, 64))

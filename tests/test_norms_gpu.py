@@ -1,0 +1,197 @@
+"""norms.gated_residual_norm against float64.
+
+One rounding per output: 2^-11 (fp16) or 2^-24 (fp32) of the value.  In front of it the fp32 arithmetic: a mean of n
+terms and a mean of squares summed in groups of at most 32 * 4 * 8 / 32 terms per lane and 8 more levels carry less than
+64 steps of 2^-24, a row with |mean| = 60 sigma loses 60 of them to the difference, rsqrtf 2 steps, and the two norms
+follow one another: 1e-5 relative to the row's largest |h| (gamma and the gate are of order one) bounds all of it.
+"""
+import numpy as np
+import pytest
+import torch
+
+import mx_oracle as X
+from effective_transformer_b200 import mxfp4, norms
+
+pytestmark = pytest.mark.gpu
+HALF = {torch.float16: 2.0 ** -11, torch.float32: 2.0 ** -24}
+DTYPES = [torch.float16, torch.float32]
+
+
+def make(seed, rows, n, dtype, seqs=0, mean=0.0):
+    gen = torch.Generator(device="cuda").manual_seed(seed)
+
+    def normal(*shape, scale=1.0, centre=0.0):
+        return (torch.randn(*shape, generator=gen, device="cuda") * scale + centre).to(dtype)
+
+    a = dict(x=normal(rows, n, centre=mean), bias=normal(n, scale=0.1), residual=normal(rows, n),
+             post_gamma=normal(n, scale=0.1, centre=1.0), post_beta=normal(n, scale=0.1),
+             pre_gamma=normal(n, scale=0.1, centre=1.0), pre_beta=normal(n, scale=0.1))
+    if seqs:
+        a["gate"] = normal(seqs, n, scale=0.5)
+        a["batch_idx"] = torch.sort(torch.randint(0, seqs, (rows,), generator=gen, device="cuda", dtype=torch.int32))[0]
+    return a
+
+
+def want_of(a, post, pre, scale=1.0, eps=1e-6):
+    return X.gated_norm(a["x"], a.get("bias"), a.get("residual"), scale, a.get("gate"), a.get("batch_idx"), post,
+                        a["post_gamma"], a["post_beta"], pre, a["pre_gamma"], a["pre_beta"], eps)
+
+
+def close(got, want, h, dtype):
+    """h: the row whose size scales the fp32 error."""
+    size = torch.maximum(want.abs(), h.abs()).amax(-1, keepdim=True) + 1.0
+    assert ((got.double() - want).abs() <= HALF[dtype] * want.abs() + 1e-5 * size + 2.0 ** -25).all()
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rows,n", [(1, 8), (1, 768), (5, 136), (33, 1024), (9, 2080), (300, 256), (17, 4096)])
+@pytest.mark.parametrize("post,pre", [("none", "layer"), ("layer", "rms"), ("rms", "layer"), ("rms", "none"), ("layer", "layer")])
+def test_norms(dtype, rows, n, post, pre):
+    a = make(rows + n, rows, n, dtype, seqs=3)
+    h, y = norms.gated_residual_norm(**a, post_norm=post, pre_norm=pre, residual_scale=0.75)
+    wh, wy = want_of(a, post, pre, 0.75)
+    close(h, wh, wh, dtype)
+    close(y, wy, wh, dtype)
+
+
+@pytest.mark.parametrize("n", [8192, 5000, 8184])
+def test_widest_fp16_rows(n):
+    a = make(n, 6, n, torch.float16)
+    h, y = norms.gated_residual_norm(**a, post_norm="layer", pre_norm="rms")
+    wh, wy = want_of(a, "layer", "rms")
+    close(h, wh, wh, torch.float16)
+    close(y, wy, wh, torch.float16)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("drop", ["bias", "residual", "gate", "all"])
+def test_absent_terms(dtype, drop):
+    a = make(3, 40, 384, dtype, seqs=4)
+    for k in ("bias", "residual", "gate", "batch_idx"):
+        if drop in (k, "all") or (drop == "gate" and k == "batch_idx"):
+            a[k] = None
+    h, y = norms.gated_residual_norm(**a, post_norm="rms", pre_norm="layer", residual_scale=2.0)
+    wh, wy = want_of(a, "rms", "layer", 2.0)
+    close(h, wh, wh, dtype)
+    close(y, wy, wh, dtype)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_gates(dtype):
+    a = make(4, 64, 256, dtype)
+    for gate in (torch.randn(256, device="cuda").to(dtype), torch.randn(1, 256, device="cuda").to(dtype)):
+        a["gate"] = gate
+        h, _ = norms.gated_residual_norm(**a, post_norm="layer")
+        wh, _ = want_of(a, "layer", "layer")
+        close(h, wh, wh, dtype)
+    a = make(5, 64, 256, dtype, seqs=7)
+    a["batch_idx"] = torch.randint(0, 7, (64,), device="cuda", dtype=torch.int32)
+    a["batch_idx"][[3, 9, 63]] = torch.tensor([-1, 7, 2 ** 31 - 1], dtype=torch.int32, device="cuda")
+    a["x"][9] = float("inf")                                    # a closed gate lets nothing through
+    h, y = norms.gated_residual_norm(**a, pre_norm="rms", residual_scale=0.5)
+    assert torch.equal(h[[3, 9, 63]].double(), (a["residual"][[3, 9, 63]].double() * 0.5).to(dtype).double())
+    wh, wy = want_of(a, "none", "rms", 0.5)
+    close(h, wh, wh, dtype)
+    close(y, wy, wh, dtype)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_constant_rows_and_large_means(dtype):
+    """A constant row has no spread: LayerNorm gives beta.  |mean| = 60 sigma loses no more than the bound says."""
+    a = make(6, 8, 1024, dtype, mean=60.0)
+    a["x"][2], a["bias"], a["residual"] = 5.0, None, None
+    h, y = norms.gated_residual_norm(**a, post_norm="none", pre_norm="layer")
+    wh, wy = want_of(a, "none", "layer")
+    assert torch.equal(y[2], a["pre_beta"])
+    close(h, wh, wh, dtype)
+    close(y, wy, wh, dtype)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_non_finite_rows_stay_in_their_rows(dtype):
+    a = make(7, 12, 512, dtype)
+    a["x"][4, 7], a["x"][5, 0] = float("nan"), float("inf")
+    h, y = norms.gated_residual_norm(**a, post_norm="layer", pre_norm="layer")
+    keep = [i for i in range(12) if i not in (4, 5)]
+    wh, wy = want_of(a, "layer", "layer")
+    assert y[4].isnan().all() and y[5].isnan().all()
+    close(h[keep], wh[keep], wh[keep], dtype)
+    close(y[keep], wy[keep], wh[keep], dtype)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_in_place_and_rows_past_the_count(dtype):
+    a = make(8, 100, 640, dtype, seqs=5)
+    wh, wy = want_of(a, "layer", "rms")
+    for valid in (0, 1, 57, 100, 1000):
+        b = {k: (v.clone() if v is not None else None) for k, v in a.items()}
+        t = min(valid, 100)
+        n = torch.full((1,), valid, dtype=torch.int32, device="cuda")
+        h, y = norms.gated_residual_norm(**b, post_norm="layer", pre_norm="rms", valid_rows=n, h_out=b["residual"],
+                                         y_out=b["x"])
+        assert h is b["residual"] and y is b["x"]
+        close(h[:t], wh[:t], wh[:t], dtype)
+        close(y[:t], wy[:t], wh[:t], dtype)
+        assert torch.equal(h[t:], a["residual"][t:]) and torch.equal(y[t:], a["x"][t:])
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rows,n", [(1, 32), (70, 96), (131, 1024), (40, 2080), (3, 4096), (5, 416)])
+def test_quantized_output_is_the_quantised_y(dtype, rows, n):
+    """y in 4 bits next to y itself: what fp32 y rounds to, up to the rounding of y as it is returned (a code's border
+    may lie between); with fp32 rows they are equal bit by bit."""
+    a = make(rows + n, rows, n, dtype)
+    mx = mxfp4.empty(rows, n)
+    mx.data.fill_(0xEE)
+    y_out = torch.empty_like(a["x"])
+    h, y = norms.gated_residual_norm(**a, post_norm="none", pre_norm="layer", y_out=y_out, mx_out=mx)
+    got = X.mx_unpack(mx.data.cpu().numpy(), rows, n)
+    if dtype == torch.float32:
+        codes, scales = X.mx_parts(y.cpu().numpy())
+        assert np.array_equal(got[0], codes) and np.array_equal(got[1], scales)
+    else:
+        yv = y.double().cpu().numpy()
+        back = mxfp4.dequantize(mx, torch.float32).cpu().numpy()
+        step = np.exp2(got[1].astype(np.float64) - 127).repeat(32, axis=1) * np.where(
+            np.abs(back) >= 4 * np.exp2(got[1].astype(np.float64) - 127).repeat(32, axis=1), 2.0, 1.0)
+        assert (np.abs(back - yv) <= step * (1 + 2.0 ** -10)).all()
+    # the block between an odd width / 32 and a multiple of 64 is zero: the product reads it
+    kernel = torch.randn(n, 64, device="cuda").to(dtype)
+    c = mxfp4.gemm(mx, mxfp4.pack_weight(kernel), dtype=torch.float32)
+    v = mxfp4.dequantize(mx, torch.float32).double() @ mxfp4.dequantize(mxfp4.pack_weight(kernel), torch.float32).double().t()
+    assert ((c.double() - v).abs() <= 1e-4 * v.abs().max() + 1e-6).all()
+    only, none = norms.gated_residual_norm(**a, post_norm="none", pre_norm="layer", mx_out=mxfp4.empty(rows, n))
+    assert none is None and torch.equal(only, h)
+
+
+def test_refusals():
+    x = torch.zeros(4, 64, dtype=torch.float16, device="cuda")
+    g = torch.ones(64, dtype=torch.float16, device="cuda")
+    ok = dict(pre_gamma=g, pre_beta=g)
+    for kw in (dict(), dict(pre_gamma=g), dict(ok, post_norm="layer"), dict(ok, post_norm="batch"),
+               dict(ok, gate=torch.zeros(3, 64, dtype=torch.float16, device="cuda")), dict(ok, gate=g[:32]),
+               dict(ok, residual=x[:2]), dict(ok, bias=g.float()), dict(ok, h_out=x, y_out=x),
+               dict(ok, mx_out=mxfp4.empty(3, 64)), dict(pre_gamma=g, pre_beta=g.cpu()),
+               dict(ok, gate=torch.zeros(3, 64, dtype=torch.float16, device="cuda"),
+                    batch_idx=torch.zeros(3, dtype=torch.int32, device="cuda"))):
+        with pytest.raises(ValueError):
+            norms.gated_residual_norm(x, **kw)
+    with pytest.raises(ValueError):
+        norms.gated_residual_norm(x.t(), **ok)
+
+
+def test_streams_and_capture():
+    a = make(9, 50, 768, torch.float16)
+    wh, wy = want_of(a, "layer", "layer")
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        h, y = norms.gated_residual_norm(**a, post_norm="layer")
+    torch.cuda.current_stream().wait_stream(side)
+    close(y, wy, wh, torch.float16)
+    h2, y2 = torch.zeros_like(a["x"]), torch.zeros_like(a["x"])
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        norms.gated_residual_norm(**a, post_norm="layer", h_out=h2, y_out=y2)
+    graph.replay()
+    assert torch.equal(h2, h) and torch.equal(y2, y)
