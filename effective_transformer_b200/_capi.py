@@ -59,7 +59,7 @@ class OutputParam(C.Structure):
 class GatedNormParam(C.Structure):
     _fields_ = [(n, vp) for n in (
         "x", "bias", "residual", "gate", "batch_idx", "post_gamma", "post_beta", "pre_gamma", "pre_beta", "h_out",
-        "y_out", "y_mx", "m_ptr", "stream")] + [(n, i32) for n in (
+        "y_out", "y_mx", "m_ptr")] + [(n, i32) for n in (
             "max_m", "n", "gate_rows", "post_norm", "pre_norm")] + [("residual_scale", C.c_float), ("eps", C.c_float)]
 
 
@@ -129,7 +129,7 @@ SIGNATURES = {
     "et_mxfp4_pack_weight": (i32, [i32, vp, vp, i32, i32, vp]),
     "et_mxfp4_gemm": (i32, [i32, vp, vp, vp, vp, vp, vp, vp, i32, i32, i32, i32, vp, vp]),
     "et_mxfp4_linear": (i32, [i32, vp, i64, vp, vp, vp, vp, vp, vp, vp, i32, i32, i32, i32, vp, vp]),
-    "et_gated_residual_norm": (i32, [i32, C.POINTER(GatedNormParam)]),
+    "et_gated_residual_norm": (i32, [i32, C.POINTER(GatedNormParam), vp]),
     "et_gemm_fp32_tensor": (i32, [vp, vp, vp, vp, vp, vp, vp, i32, i32, i32, i32, vp, vp]),
 }
 

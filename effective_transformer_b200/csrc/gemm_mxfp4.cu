@@ -5,12 +5,12 @@
 // A product of two e2m1 values and two power-of-two scales is exact, so the only roundings are those of the fp32
 // sum and the one at the end.
 //
-// Structure (one persistent CTA per SM, 320 threads), tiles of 128 x 128:
-//   warp 0    producer: one untiled bulk copy per operand and k-tile of 256 values (codes and scales, 17 KB) into a
-//             ring of kStages stages
-//   warp 1    MMA issuer: the stage's scales go to tensor memory (tcgen05.cp), then four tcgen05.mma kind::mxf4 of
-//             K = 64, accumulating in one of two TMEM buffers
-//   warps 2-9 epilogue: one TMEM lane quadrant and one half of the columns each
+// Two persistent kernels, one CTA per SM:
+//   warp 0    producer: operand tiles of 256 values of K, codes and scales, into a ring of kStages stages
+//   warp 1    MMA issuer: the stage's scales go to tensor memory (tcgen05.cp), then tcgen05.mma kind::mxf4 of K = 64,
+//             accumulating in one of two TMEM buffers
+//   the rest  epilogue: one TMEM lane quadrant and 64 of a buffer's columns each
+// gemm_mxfp4_kernel works on tiles of 128 x 128, gemm_mxfp4_pair_kernel on tiles of 256 x 192 by CTA pairs.
 // Scales have a TMEM region per stage, so a stage's are replaced only after the MMAs that read them have retired.
 #include "common.cuh"
 #include "mxfp4.cuh"
@@ -25,8 +25,8 @@ using namespace ptx;
 constexpr int BM = 128;
 constexpr int kEpilogueWarps = 8;
 constexpr int kNumThreads = 64 + kEpilogueWarps * 32;
-constexpr int kStagingPerWarp = 32 * 128;
 constexpr int kUmmaK = 64;
+constexpr int kPairTiles = 512;  // from so many 128 x 128 tiles on, CTA pairs
 
 enum Site : int {
   kSiteProducerEmpty = 1,
@@ -48,150 +48,283 @@ struct MxArgs {
   int* status_word;
 };
 
-__device__ __forceinline__ void st_shared_v4(uint32_t addr, const Vec16& v) {
-  asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(addr), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w)
-               : "memory");
-}
-__device__ __forceinline__ Vec16 ld_shared_v4(uint32_t addr) {
-  Vec16 v;
-  asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];"
-               : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
-               : "r"(addr)
-               : "memory");
-  return v;
-}
-
 // Rows as MXFP4 instead of T.
 struct MxOut {};
+
+// Two fp32 values in one 64-bit register: the packed fp32 instructions do two elements an issue slot.
+__device__ __forceinline__ uint64_t pack2(float a, float b) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ void unpack2(uint64_t v, float& a, float& b) {
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v));
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+
+// tanh-form GELU of a pair whose result is rounded to fp16 or to 4 bits: 0.5 x (1 + tanh u) with the hardware's
+// tanh (relative error 2^-11, so at most 0.5 |x| 2^-11 here, the size of the fp16 rounding behind it; in 4 bits a
+// sixteenth of half a step at the least).  One special-function operation an element where exp and a reciprocal
+// would be two: those alone take 36 us of a 39778 x 4096 result.
+__device__ __forceinline__ void gelu_pair(float& a, float& b) {
+  const uint64_t x = pack2(a, b);
+  const uint64_t c1 = pack2(0.7978845608028654f, 0.7978845608028654f);
+  const uint64_t c2 = pack2(0.7978845608028654f * 0.044715f, 0.7978845608028654f * 0.044715f);
+  float ua, ub;
+  unpack2(mul2(x, fma2(mul2(x, x), c2, c1)), ua, ub);
+  asm("tanh.approx.f32 %0, %0;" : "+f"(ua));
+  asm("tanh.approx.f32 %0, %0;" : "+f"(ub));
+  const uint64_t h = mul2(x, pack2(0.5f, 0.5f));
+  unpack2(fma2(h, pack2(ua, ub), h), a, b);
+}
+
+// Activation of kCount values.
+template <int kCount, int ACT, bool kRough>
+__device__ __forceinline__ void activate(float* f) {
+  if (ACT == kEpiBiasGelu) {
+#pragma unroll
+    for (int i = 0; i < kCount; i += 2) {
+      if (kRough) {
+        gelu_pair(f[i], f[i + 1]);
+      } else {
+        f[i] = gelu_tanh(f[i]);
+        f[i + 1] = gelu_tanh(f[i + 1]);
+      }
+    }
+  }
+  if (ACT == kEpiBiasTanh) {
+#pragma unroll
+    for (int i = 0; i < kCount; ++i) f[i] = tanhf(f[i]);
+  }
+}
+
+// Eight neighbouring values of a row of T.
 template <typename T>
-struct BiasOf {
-  typedef T type;
+struct Oct {
+  Vec16 v[sizeof(T) / 2];
+  __device__ __forceinline__ void zero() {
+#pragma unroll
+    for (int i = 0; i < static_cast<int>(sizeof(T)) / 2; ++i) v[i] = Vec16{0u, 0u, 0u, 0u};
+  }
+  __device__ __forceinline__ void load_activation(const T* p) {
+#pragma unroll
+    for (int i = 0; i < static_cast<int>(sizeof(T)) / 2; ++i) v[i] = ld_activation_v4(p + i * VecTraits<T>::kElems);
+  }
+  __device__ __forceinline__ void load(const T* p) {
+#pragma unroll
+    for (int i = 0; i < static_cast<int>(sizeof(T)) / 2; ++i) v[i] = ld_global_v4(p + i * VecTraits<T>::kElems);
+  }
+  __device__ __forceinline__ void add_to(float* f) const {
+#pragma unroll
+    for (int i = 0; i < static_cast<int>(sizeof(T)) / 2; ++i) {
+      float x[VecTraits<T>::kElems];
+      VecTraits<T>::unpack(v[i], x);
+#pragma unroll
+      for (int e = 0; e < VecTraits<T>::kElems; e += 2) {
+        float* d = f + i * VecTraits<T>::kElems + e;
+        unpack2(add2(pack2(d[0], d[1]), pack2(x[e], x[e + 1])), d[0], d[1]);
+      }
+    }
+  }
+};
+template <typename T>
+__device__ __forceinline__ void store_oct(T* p, const float* f) {
+#pragma unroll
+  for (int i = 0; i < 8; i += VecTraits<T>::kElems) st_global_v4(p + i, VecTraits<T>::pack(f + i));
+}
+
+// The epilogue of one warp for a piece of 32 rows x 64 columns of a finished accumulator: row0, col0 its first row and
+// column, (TMEM lanes at the lane field of t_row).  prepare() runs before the accumulator is waited for, finish()
+// behind; release() in it once the warp's values are in registers.
+//
+// fp16 and fp32 results: a thread has, for each of 2 column groups of 32 and 4 row groups of 8, eight neighbouring
+// columns of one row (see mxfp4.cuh): bias and residual come in, and the result goes out, as 16 or 32 bytes a thread
+// and 64 or 128 contiguous bytes a row.
+template <typename T, typename OUT, int ACT>
+struct Piece {
+  static constexpr int kParts = 2 / (sizeof(T) / 2);  // column groups whose residual is fetched ahead
+  Oct<T> bias[2];
+  Oct<T> res[kParts][4];
+
+  // Row of row group i (rows are lanes in the order of mx_row).
+  static __device__ __forceinline__ int row_of(int i, int lane) { return mx_row(8 * i + (lane >> 2)); }
+
+  __device__ __forceinline__ void fetch(const MxArgs& g, int part, int slot, int row0, int col0, int M, int lane) {
+    const int col = col0 + part * 32 + (lane & 3) * 8;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int row = row0 + row_of(i, lane);
+      res[slot][i].zero();
+      if (row < M && col < g.n)
+        res[slot][i].load_activation(static_cast<const T*>(g.residual) + static_cast<size_t>(row) * g.n + col);
+    }
+  }
+  __device__ __forceinline__ void prepare(const MxArgs& g, const T* __restrict__ bias_ptr, int row0, int col0, int M,
+                                          int lane) {
+#pragma unroll
+    for (int c = 0; c < 2; ++c) {
+      const int col = col0 + c * 32 + (lane & 3) * 8;
+      bias[c].zero();
+      if (bias_ptr != nullptr && col < g.n) bias[c].load(bias_ptr + col);
+    }
+    if (g.residual != nullptr) {
+#pragma unroll
+      for (int c = 0; c < kParts; ++c) fetch(g, c, c, row0, col0, M, lane);
+    }
+  }
+  template <typename Release>
+  __device__ __forceinline__ void finish(const MxArgs& g, uint32_t t_row, int row0, int col0, int M, int lane,
+                                         Release release) {
+    uint32_t r[2][2][16];  // column group, upper or lower 16 lanes
+#pragma unroll
+    for (int c = 0; c < 2; ++c)
+#pragma unroll
+      for (int h = 0; h < 2; ++h) tmem_ld_16x256b_x4(t_row + (static_cast<uint32_t>(16 * h) << 16) + 32 * c, r[c][h]);
+    tmem_ld_wait();
+    tc_fence_before();
+    __syncwarp();
+    release();
+    T* base = static_cast<T*>(g.c) + static_cast<size_t>(row0) * g.n + col0 + (lane & 3) * 8;
+#pragma unroll
+    for (int c = 0; c < 2; ++c) {
+      if (c >= kParts && g.residual != nullptr) fetch(g, c, 0, row0, col0, M, lane);
+      const bool in = col0 + c * 32 < g.n;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        float f[8];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          f[2 * j] = __uint_as_float(r[c][i >> 1][4 * j + 2 * (i & 1)]);
+          f[2 * j + 1] = __uint_as_float(r[c][i >> 1][4 * j + 2 * (i & 1) + 1]);
+        }
+        bias[c].add_to(f);
+        activate<8, ACT, sizeof(T) == 2>(f);
+        if (g.residual != nullptr) res[c < kParts ? c : 0][i].add_to(f);
+        const int row = row_of(i, lane);
+        if (in && row0 + row < M) store_oct<T>(base + static_cast<size_t>(row) * g.n + c * 32, f);
+      }
+    }
+  }
 };
 
-template <int ACT>
-__device__ __forceinline__ float activate(float x) {
-  if (ACT == kEpiBiasGelu) return gelu_tanh(x);
-  if (ACT == kEpiBiasTanh) return tanhf(x);
-  return x;
-}
-
-// 64 columns of 32 rows, a row per thread in r: bias and activation in fp32.
+// MXFP4 results: a thread has the 64 columns of one row, two scale blocks, and needs no other's.
 template <typename T, int ACT>
-__device__ __forceinline__ void bias_act(float* f, const T* bias_s) {
-  if (bias_s != nullptr) {
-#pragma unroll
-    for (int i = 0; i < 64; i += VecTraits<T>::kElems) {
-      float b[VecTraits<T>::kElems];
-      VecTraits<T>::unpack(*reinterpret_cast<const Vec16*>(bias_s + i), b);
-#pragma unroll
-      for (int e = 0; e < VecTraits<T>::kElems; ++e) f[i + e] += b[e];
-    }
-  }
-#pragma unroll
-  for (int i = 0; i < 64; ++i) f[i] = activate<ACT>(f[i]);
-}
+struct Piece<T, MxOut, ACT> {
+  Oct<T> bias[8];  // of all 64 columns
 
-// Stores them to C, rows [0, rows_valid) and columns [0, cols_valid) of the piece; ctile / rtile: its first element.
-// The warp's staging bytes turn one row per thread into whole row segments per instruction.  With a residual the
-// sum is formed in fp32 and rounded once.
-template <typename T>
-__device__ __forceinline__ void store_rows(const float* f, T* ctile, const T* rtile, int n, int rows_valid,
-                                           int cols_valid, uint32_t buf, int lane) {
-  const int piece = lane & 7;
-  if (sizeof(T) == 2 && rtile == nullptr) {
-#pragma unroll
-    for (int p = 0; p < 8; ++p)
-      st_shared_v4(buf + lane * 128 + ((p ^ (lane & 7)) << 4), VecTraits<__half>::pack(f + 8 * p));
-    __syncwarp();
+  __device__ __forceinline__ void prepare(const MxArgs& g, const T* __restrict__ bias_ptr, int, int col0, int, int) {
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      const int rr = 4 * i + (lane >> 3);
-      const Vec16 v = ld_shared_v4(buf + rr * 128 + ((piece ^ (rr & 7)) << 4));
-      if (rr < rows_valid && piece * 8 < cols_valid) st_global_v4(ctile + static_cast<size_t>(rr) * n + piece * 8, v);
+      bias[i].zero();
+      if (bias_ptr != nullptr && col0 + 8 * i < g.n) bias[i].load(bias_ptr + col0 + 8 * i);
     }
-    __syncwarp();
-    return;
   }
-#pragma unroll
-  for (int h = 0; h < 2; ++h) {
-#pragma unroll
-    for (int p = 0; p < 8; ++p)
-      st_shared_v4(buf + lane * 128 + ((p ^ (lane & 7)) << 4), VecTraits<float>::pack(f + h * 32 + 4 * p));
+  template <typename Release>
+  __device__ __forceinline__ void finish(const MxArgs& g, uint32_t t_row, int row0, int col0, int M, int lane,
+                                         Release release) {
+    uint32_t r[64];
+    tmem_ld_32x32b_x32(t_row, r);
+    tmem_ld_32x32b_x32(t_row + 32, r + 32);
+    tmem_ld_wait();
+    tc_fence_before();
     __syncwarp();
-    const int col = h * 32 + piece * 4;
-    float res[8][4];
+    release();
+    const int row = row0 + mx_row(lane);
+    if (row >= M || col0 >= g.n) return;  // (n is a multiple of 64)
+    uint8_t* tile = static_cast<uint8_t*>(g.c) + mx_tile_offset(row, col0 >> 8, mx_k_tiles(g.n));
+    const int rt = row & (kMxTileRows - 1), b0 = (col0 & 255) >> 5;
+    uint32_t scales = 0u;
+    Vec16 out[2];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const int rr = 4 * i + (lane >> 3);
-      const bool in = rtile != nullptr && rr < rows_valid && col < cols_valid;
-      if (sizeof(T) == 2) {
-        uint2 u = make_uint2(0u, 0u);
-        if (in) u = *reinterpret_cast<const uint2*>(rtile + static_cast<size_t>(rr) * n + col);
-        const float2 a = __half22float2(*reinterpret_cast<const __half2*>(&u.x));
-        const float2 b = __half22float2(*reinterpret_cast<const __half2*>(&u.y));
-        res[i][0] = a.x, res[i][1] = a.y, res[i][2] = b.x, res[i][3] = b.y;
-      } else {
-        Vec16 v = {0u, 0u, 0u, 0u};
-        if (in) v = ld_activation_v4(rtile + static_cast<size_t>(rr) * n + col);
-        VecTraits<float>::unpack(v, res[i]);
+    for (int h = 0; h < 2; ++h) {
+      float f[32];
+#pragma unroll
+      for (int i = 0; i < 32; ++i) f[i] = __uint_as_float(r[h * 32 + mx_row(i)]);  // columns in their order
+      float top = 0.f;
+#pragma unroll
+      for (int i = 0; i < 32; i += 8) {
+        bias[h * 4 + i / 8].add_to(f + i);
+        activate<8, ACT, true>(f + i);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) asm("max.NaN.f32 %0, %0, %1;" : "+f"(top) : "f"(fabsf(f[i + e])));
       }
+      const MxScale s = mx_scale(abs_bits(top));
+      out[h].x = mx_codes8(f, s);
+      out[h].y = mx_codes8(f + 8, s);
+      out[h].z = mx_codes8(f + 16, s);
+      out[h].w = mx_codes8(f + 24, s);
+      scales |= s.byte << (8 * h);
     }
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const int rr = 4 * i + (lane >> 3);
-      float v[4];
-      VecTraits<float>::unpack(ld_shared_v4(buf + rr * 128 + ((piece ^ (rr & 7)) << 4)), v);
-      if (rtile != nullptr) {
-#pragma unroll
-        for (int e = 0; e < 4; ++e) v[e] += res[i][e];
-      }
-      if (rr < rows_valid && col < cols_valid) {
-        T* dst = ctile + static_cast<size_t>(rr) * n + col;
-        if (sizeof(T) == 2) {
-          const __half2 a = __floats2half2_rn(v[0], v[1]), b = __floats2half2_rn(v[2], v[3]);
-          *reinterpret_cast<uint2*>(dst) =
-              make_uint2(*reinterpret_cast<const uint32_t*>(&a), *reinterpret_cast<const uint32_t*>(&b));
-        } else {
-          st_global_v4(dst, VecTraits<float>::pack(v));
-        }
-      }
-    }
-    __syncwarp();
+    // the two blocks are neighbours under the swizzle too, in either order: one 32-byte sector
+    const bool swap = (mx_row(rt) & 1) != 0;
+    const Vec16 lo = swap ? out[1] : out[0], hi = swap ? out[0] : out[1];
+    asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(tile + (mx_code_offset(rt, b0) & ~16)),
+                 "r"(lo.x), "r"(lo.y), "r"(lo.z), "r"(lo.w), "r"(hi.x), "r"(hi.y), "r"(hi.z), "r"(hi.w)
+                 : "memory");
+    *reinterpret_cast<uint16_t*>(tile + mx_scale_offset(rt, b0)) = static_cast<uint16_t>(scales);
   }
-}
+};
 
-// The same 64 columns as two scale blocks of a row of MXFP4; a thread has whole blocks in its registers.
-__device__ __forceinline__ void store_mx(const float* f, uint8_t* mx, int row, int col, int n, bool row_valid) {
-  if (!row_valid || col >= n) return;  // (n is a multiple of 64)
-  uint8_t* tile = mx + mx_tile_offset(row, col >> 8, mx_k_tiles(n));
-  const int r = row & (kMxTileRows - 1), b0 = (col & 255) >> 5;
-  uint32_t scales = 0u;
+// What one thread issues for a stage: the scales' copies and the MMAs of kSteps x 64 values of K.  The instruction
+// stream of that thread is what the tensor core waits for when it is longer than an MMA (64 cycles at N = 128), so it is
+// unrolled, with descriptors that differ by constants.
+// kBlocks: W row blocks, each with its own 1 KB of scales, side by side; b_shift: columns to the scales of the tile's
+// first W row; idesc0: the descriptor that reads the first two scales of a word.
+template <bool kPair, int kBlocks>
+__device__ __forceinline__ void issue_stage(int steps, uint32_t d_tmem, uint32_t a_addr, uint32_t b_addr,
+                                            uint32_t bs_addr, uint32_t sfa, uint32_t sfb, uint32_t b_shift,
+                                            uint32_t idesc0, bool first) {
+  const uint64_t adesc = make_kmajor_sw128_desc(a_addr), bdesc = make_kmajor_sw128_desc(b_addr);
+  const uint64_t as_desc = make_scale_desc(a_addr + kMxCodeBytes), bs_desc = make_scale_desc(bs_addr);
+  auto cp = [&](uint32_t dst, uint64_t desc) {
+    if (kPair) tmem_cp_scales_pair(dst, desc);
+    else tmem_cp_scales(dst, desc);
+  };
+  auto copy = [&](int p) {
+    cp(sfa + 4 * p, as_desc + 32u * p);
 #pragma unroll
-  for (int h = 0; h < 2; ++h) {
-    uint32_t top = 0u;
+    for (int i = 0; i < kBlocks; ++i) cp(sfb + 4 * (kBlocks * p + i), bs_desc + 32u * p + 64u * i);
+  };
+  auto mma = [&](int j) {
+    const uint32_t idesc = idesc0 | ((j & 1) ? make_idesc_mxf4(0, 0, 2) : 0u), acc = first && j == 0 ? 0u : 1u;
+    const uint32_t sa = sfa + 4 * (j >> 1), sb = sfb + 4 * kBlocks * (j >> 1) + b_shift;
+    if (kPair) umma_mxf4_ss_pair(d_tmem, adesc + 2u * j, bdesc + 2u * j, idesc, sa, sb, acc);
+    else umma_mxf4_ss(d_tmem, adesc + 2u * j, bdesc + 2u * j, idesc, sa, sb, acc);
+  };
+  if (steps == 4) {
+    copy(0);
+    copy(1);
 #pragma unroll
-    for (int i = 0; i < 32; ++i) top = max(top, abs_bits(f[h * 32 + i]));
-    const MxScale s = mx_scale(top);
-    Vec16 v;
-    v.x = mx_codes8(f + h * 32, s);
-    v.y = mx_codes8(f + h * 32 + 8, s);
-    v.z = mx_codes8(f + h * 32 + 16, s);
-    v.w = mx_codes8(f + h * 32 + 24, s);
-    st_global_v4(tile + mx_code_offset(r, b0 + h), v);
-    scales |= s.byte << (8 * h);
+    for (int j = 0; j < 4; ++j) mma(j);
+  } else {  // the rest of a width that is no multiple of 256
+    copy(0);
+    if (steps > 2) copy(1);
+#pragma unroll
+    for (int j = 0; j < 3; ++j)
+      if (j < steps) mma(j);
   }
-  *reinterpret_cast<uint16_t*>(tile + mx_scale_offset(r, b0)) = static_cast<uint16_t>(scales);
 }
 
 template <int BN>
 struct Cfg {
-  static constexpr int kStages = 5;
+  static constexpr int kStages = 6;
   static constexpr int kStageBytes = 2 * kMxTileBytes;
-  static constexpr int kStagingBytes = kEpilogueWarps * kStagingPerWarp;
-  static constexpr int kColsPerWarp = BN / 2;
-  static constexpr int kBiasBytes = kEpilogueWarps * kColsPerWarp * 4;
   static constexpr int kNumBars = 2 * kStages + 5;
-  static constexpr int kSmemBytes = kStages * kStageBytes + kStagingBytes + kBiasBytes + 256;
+  static constexpr int kSmemBytes = kStages * kStageBytes + 256;
   static constexpr int kScaleCols = 16;  // per stage: 2 pieces of A, 2 of B, 4 columns each
   static constexpr int kTmemCols = 512;
   static_assert(2 * BN + kStages * kScaleCols <= kTmemCols, "tensor memory");
@@ -205,7 +338,6 @@ gemm_mxfp4_kernel(const MxArgs g, const T* __restrict__ bias) {
   constexpr int BN = 128;
   using cfg = Cfg<BN>;
   constexpr int S = cfg::kStages;
-  constexpr bool kMxOut = sizeof(OUT) != sizeof(T);
   pdl_trigger();
 
   extern __shared__ __align__(1024) uint8_t smem_raw[];
@@ -215,10 +347,7 @@ gemm_mxfp4_kernel(const MxArgs g, const T* __restrict__ bias) {
     if (threadIdx.x == 0) report_timeout(g.status_word, kKernelGemmMx, kSiteSmemAlign);
     return;
   }
-  const uint32_t staging_addr = tiles_addr + S * cfg::kStageBytes;
-  T* bias_all = reinterpret_cast<T*>(smem_raw + S * cfg::kStageBytes + cfg::kStagingBytes);
-  uint64_t* bars =
-      reinterpret_cast<uint64_t*>(smem_raw + S * cfg::kStageBytes + cfg::kStagingBytes + cfg::kBiasBytes);
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem_raw + S * cfg::kStageBytes);
   const uint32_t bar0 = smem_u32(bars);
   auto full_bar = [&](int s) { return bar0 + 8u * s; };
   auto free_bar = [&](int s) { return bar0 + 8u * (S + s); };
@@ -227,7 +356,7 @@ gemm_mxfp4_kernel(const MxArgs g, const T* __restrict__ bias) {
   const uint32_t drain_bar = bar0 + 8u * (2 * S + 4);
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + cfg::kNumBars);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = __shfl_sync(0xffffffffu, static_cast<int>(threadIdx.x) >> 5, 0), lane = threadIdx.x & 31;
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < S; ++s) {
@@ -250,7 +379,7 @@ gemm_mxfp4_kernel(const MxArgs g, const T* __restrict__ bias) {
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  const uint32_t tmem_base = *tmem_slot;
+  const uint32_t tmem_base = __shfl_sync(0xffffffffu, *tmem_slot, 0);
 
   int M = g.max_m;
   if (g.m_ptr != nullptr) M = pdl_wait_row_count(g.m_ptr, g.max_m, 0);
@@ -266,31 +395,38 @@ gemm_mxfp4_kernel(const MxArgs g, const T* __restrict__ bias) {
   };
 
   if (warp == 0) {
-    if (lane == 0) {
-      uint32_t stage = 0, phase = 0;
-      long long issued = 0;
-      bool ok = true;
-      for (int tile = blockIdx.x; tile < num_tiles && ok; tile += gridDim.x) {
-        const int m_tile = tile / n_tiles, n_tile = tile - m_tile * n_tiles;
-        const uint8_t* a_src = g.a + static_cast<size_t>(m_tile) * k_tiles * kMxTileBytes;
-        const uint8_t* w_src = g.w + static_cast<size_t>(n_tile) * k_tiles * kMxTileBytes;
-        for (int kt = 0; kt < k_tiles; ++kt) {
-          if (!mbar_wait(free_bar(stage), phase ^ 1u, abort_flag)) {
-            fail(kSiteProducerEmpty);
-            ok = false;
-            break;
-          }
-          const uint32_t dst = tiles_addr + stage * cfg::kStageBytes;
-          mbar_arrive_expect_tx(full_bar(stage), cfg::kStageBytes);
-          bulk_load(dst, a_src + static_cast<size_t>(kt) * kMxTileBytes, kMxTileBytes, full_bar(stage));
-          bulk_load(dst + kMxTileBytes, w_src + static_cast<size_t>(kt) * kMxTileBytes, kMxTileBytes, full_bar(stage));
-          ++issued;
-          if (++stage == S) {
-            stage = 0;
-            phase ^= 1u;
-          }
+    // all lanes walk through the loop, one issues (see elect_one)
+    const bool issuer = elect_one();
+    uint32_t stage = 0, phase = 0;
+    long long issued = 0;
+    bool ok = true;
+    for (int tile = blockIdx.x; tile < num_tiles && ok; tile += gridDim.x) {
+      const int m_tile = tile / n_tiles, n_tile = tile - m_tile * n_tiles;
+      const uint8_t* a_src = g.a + static_cast<size_t>(m_tile) * k_tiles * kMxTileBytes;
+      const uint8_t* w_src = g.w + static_cast<size_t>(n_tile) * k_tiles * kMxTileBytes;
+      for (int kt = 0; kt < k_tiles; ++kt) {
+        if (!__all_sync(0xffffffffu, mbar_wait(free_bar(stage), phase ^ 1u, abort_flag))) {
+          if (lane == 0) fail(kSiteProducerEmpty);
+          ok = false;
+          break;
+        }
+        const uint32_t dst = tiles_addr + stage * cfg::kStageBytes, bar = full_bar(stage);
+        if (issuer) {
+          mbar_arrive_expect_tx(bar, cfg::kStageBytes);
+          bulk_load(dst, a_src, kMxTileBytes, bar);
+          bulk_load(dst + kMxTileBytes, w_src, kMxTileBytes, bar);
+        }
+        __syncwarp();
+        a_src += kMxTileBytes;
+        w_src += kMxTileBytes;
+        ++issued;
+        if (++stage == S) {
+          stage = 0;
+          phase ^= 1u;
         }
       }
+    }
+    if (issuer) {
       // the issuer's commits on the ring are asynchronous arrivals: the last of them land before the barriers go away
       const long long pending = issued < S ? issued : S;
       for (long long i = 0; i < pending; ++i) {
@@ -307,92 +443,67 @@ gemm_mxfp4_kernel(const MxArgs g, const T* __restrict__ bias) {
       }
     }
   } else if (warp == 1) {
-    if (lane == 0) {
-      uint32_t stage = 0, phase = 0;
-      int it = 0;
-      bool ok = true;
-      for (int tile = blockIdx.x; tile < num_tiles && ok; tile += gridDim.x, ++it) {
-        const int acc = it & 1;
-        if (!mbar_wait(tmem_empty_bar(acc), ((it >> 1) & 1) ^ 1u, abort_flag)) {
-          fail(kSiteMmaTmemEmpty);
+    // all lanes walk through the loop, one issues (see elect_one)
+    const bool issuer = elect_one();
+    uint32_t stage = 0, phase = 0;
+    int it = 0;
+    bool ok = true;
+    for (int tile = blockIdx.x; tile < num_tiles && ok; tile += gridDim.x, ++it) {
+      const int acc = it & 1;
+      if (!__all_sync(0xffffffffu, mbar_wait(tmem_empty_bar(acc), ((it >> 1) & 1) ^ 1u, abort_flag))) {
+        if (lane == 0) fail(kSiteMmaTmemEmpty);
+        break;
+      }
+      tc_fence_after();
+      const uint32_t d_tmem = tmem_base + acc * BN;
+      for (int kt = 0; kt < k_tiles; ++kt) {
+        if (!__all_sync(0xffffffffu, mbar_wait(full_bar(stage), phase, abort_flag))) {
+          if (lane == 0) fail(kSiteMmaFull);
+          ok = false;
           break;
         }
         tc_fence_after();
-        const uint32_t d_tmem = tmem_base + acc * BN;
-        for (int kt = 0; kt < k_tiles; ++kt) {
-          if (!mbar_wait(full_bar(stage), phase, abort_flag)) {
-            fail(kSiteMmaFull);
-            ok = false;
-            break;
-          }
-          tc_fence_after();
-          const uint32_t a_addr = tiles_addr + stage * cfg::kStageBytes, b_addr = a_addr + kMxTileBytes;
-          const uint32_t sf = tmem_base + 2 * BN + stage * cfg::kScaleCols;
-          const int left = g.k - kt * kMxTileK;
-          const int steps = left >= kMxTileK ? 4 : (left + kUmmaK - 1) / kUmmaK;
-          for (int p = 0; 2 * p < steps; ++p) {
-            tmem_cp_scales(sf + 4 * p, make_scale_desc(a_addr + kMxCodeBytes + 512 * p));
-            tmem_cp_scales(sf + 8 + 4 * p, make_scale_desc(b_addr + kMxCodeBytes + 512 * p));
-          }
-          const uint64_t adesc = make_kmajor_sw128_desc(a_addr), bdesc = make_kmajor_sw128_desc(b_addr);
-          for (int j = 0; j < steps; ++j)
-            umma_mxf4_ss(d_tmem, adesc + 2u * j, bdesc + 2u * j,
-                         (j & 1) ? make_idesc_mxf4(BM, BN, 2) : make_idesc_mxf4(BM, BN, 0), sf + 4 * (j >> 1),
-                         sf + 8 + 4 * (j >> 1), (kt | j) != 0 ? 1u : 0u);
+        const uint32_t a_addr = tiles_addr + stage * cfg::kStageBytes, b_addr = a_addr + kMxTileBytes;
+        const uint32_t sf = tmem_base + 2 * BN + stage * cfg::kScaleCols;
+        const int left = g.k - kt * kMxTileK;
+        const int steps = left >= kMxTileK ? 4 : (left + kUmmaK - 1) / kUmmaK;
+        if (issuer) {
+          issue_stage<false, 1>(steps, d_tmem, a_addr, b_addr, b_addr + kMxCodeBytes, sf, sf + 8, 0, make_idesc_mxf4(BM, BN, 0),
+                                kt == 0);
           umma_commit(free_bar(stage));
-          if (++stage == S) {
-            stage = 0;
-            phase ^= 1u;
-          }
+          if (kt == k_tiles - 1) umma_commit(tmem_full_bar(acc));
         }
-        if (ok) umma_commit(tmem_full_bar(acc));
+        __syncwarp();
+        if (++stage == S) {
+          stage = 0;
+          phase ^= 1u;
+        }
       }
-      // all MMAs must have retired before TMEM is freed
+    }
+    // all MMAs must have retired before TMEM is freed
+    if (issuer) {
       umma_commit(drain_bar);
       if (!mbar_drain(drain_bar, 0u) && *abort_flag == 0) fail(kSiteMmaDrain);
     }
+    __syncwarp();
   } else {
-    const int quad = warp & 3, ew = warp - 2, half = ew >> 2;
-    constexpr int kCols = cfg::kColsPerWarp;
-    const uint32_t buf = staging_addr + ew * kStagingPerWarp;
-    T* bias_s = bias_all + ew * kCols;
+    const int quad = warp & 3, half = (warp - 2) >> 2;
     int it = 0;
     for (int tile = blockIdx.x; tile < num_tiles; tile += gridDim.x, ++it) {
       const int m_tile = tile / n_tiles, n_tile = tile - m_tile * n_tiles;
-      const int acc = it & 1;
-      const int col0 = n_tile * BN + half * kCols;
-      if (bias != nullptr) {
-        for (int i = lane; i < kCols; i += 32) bias_s[i] = col0 + i < N ? bias[col0 + i] : T(0.f);
-        __syncwarp();
-      }
+      const int acc = it & 1, row0 = m_tile * BM + quad * 32, col0 = n_tile * BN + half * 64;
+      Piece<T, OUT, ACT> piece;
+      piece.prepare(g, bias, row0, col0, M, lane);
       const bool got = mbar_wait(tmem_full_bar(acc), (it >> 1) & 1, abort_flag);
       if (!__all_sync(0xffffffffu, got)) {
         if (lane == 0) fail(kSiteEpilogueFull);
         break;
       }
       tc_fence_after();
-      const int row0 = m_tile * BM + quad * 32;
-      const uint32_t t_row = tmem_base + (static_cast<uint32_t>(quad * 32) << 16) + acc * BN + half * kCols;
-      uint32_t r[64];
-      tmem_ld_32x32b_x32(t_row, r);
-      tmem_ld_32x32b_x32(t_row + 32, r + 32);
-      tmem_ld_wait();
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(tmem_empty_bar(acc));
-      float f[64];
-#pragma unroll
-      for (int i = 0; i < 64; ++i) f[i] = __uint_as_float(r[i]);
-      bias_act<T, ACT>(f, bias != nullptr ? bias_s : nullptr);
-      if (kMxOut) {
-        store_mx(f, static_cast<uint8_t*>(g.c), row0 + lane, col0, N, row0 + lane < M);
-      } else {
-        const size_t off = static_cast<size_t>(row0) * N + col0;
-        const T* res = static_cast<const T*>(g.residual);
-        store_rows<T>(f, static_cast<T*>(g.c) + off, res != nullptr ? res + off : nullptr, N, M - row0, N - col0, buf,
-                      lane);
-      }
-      __syncwarp();  // bias_s is rewritten for the next tile
+      piece.finish(g, tmem_base + (static_cast<uint32_t>(quad * 32) << 16) + acc * BN + half * 64, row0, col0, M, lane,
+                   [&] {
+                     if (lane == 0) mbar_arrive(tmem_empty_bar(acc));
+                   });
     }
   }
 
@@ -405,6 +516,288 @@ gemm_mxfp4_kernel(const MxArgs g, const T* __restrict__ bias) {
   }
 }
 
+// Tiles of 256 x 192 by a cluster of two CTAs.  Per 256 values of K a CTA loads its own 128 rows of A, half of the
+// tile's W rows, and the scales of both: 31 KB for 128 x 192 of output, against 34 KB for 128 x 128 of the tile above.
+// CTA 0 issues the MMAs (M = 256) of both.
+//
+// The width follows from three things.  The issuing thread needs 45 cycles for an MMA and, per stage, about 170 more
+// for its waits, copies and commits: MMAs of N = 128 (64 cycles) do not cover that, of N = 192 (96 cycles) nearly do.
+// A single accumulator buffer leaves the tensor core idle for 1000 to 1800 cycles a tile, the way from the last MMA
+// to the epilogue and back.  And two buffers have to fit 512 columns beside the scales (24 columns a stage).
+// 39778 x 1024 by 1024 x 4096, plain fp16 result / 39778 x 4096 by 4096 x 1024: 256 x 256 in two column halves with
+// three half-width buffers 120 / 82 us, 256 x 256 with one buffer 118 / 71 us, tiles of 128 x 128 105 / 87 us.
+//
+// A tile's 192 W rows begin at the start or in the middle of a row block of 128: it takes the scales of two blocks, and
+// in the second case the MMAs read them from two columns (64 rows) further on.
+struct PairCfg {
+  static constexpr int BN = 192;
+  static constexpr int kEpiWarps = 12;  // three per TMEM lane quadrant, 64 columns each
+  static constexpr int kThreads = 64 + kEpiWarps * 32;
+  static constexpr int kStages = 5;
+  static constexpr int kBCodes = BN / 2 * 128;
+  static constexpr int kStageBytes = kMxTileBytes + kBCodes + 2 * kMxScaleBytes;
+  static constexpr int kScaleCols = 24;  // per stage: 2 pieces of A, 2 of each block of W, 4 columns each
+  static constexpr int kTmemCols = 512;
+  static constexpr int kNumBars = 2 * kStages + 5;
+  static constexpr int kSmemBytes = kStages * kStageBytes + 256;
+  static_assert(2 * BN + kStages * kScaleCols <= kTmemCols, "tensor memory");
+  static_assert(kStageBytes % 1024 == 0 && kSmemBytes <= 232448 && kNumBars * 8 + 8 <= 256, "shared memory");
+};
+
+template <typename T, typename OUT, int ACT>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PairCfg::kThreads, 1)
+gemm_mxfp4_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant__ CUtensorMap tmap_w,
+                       const __grid_constant__ CUtensorMap tmap_ws, const MxArgs g, const T* __restrict__ bias) {
+  using cfg = PairCfg;
+  constexpr int S = cfg::kStages;
+  pdl_trigger();
+  const uint32_t rank = cluster_ctarank();  // 0 issues the MMAs
+  const int pair_id = blockIdx.x >> 1, num_pairs = gridDim.x >> 1;
+
+  extern __shared__ __align__(1024) uint8_t smem_raw[];
+  const uint32_t tiles_addr = smem_u32(smem_raw);
+  if ((tiles_addr & 1023u) != 0u) {  // same layout in both CTAs: uniform for the pair
+    pdl_wait();
+    if (threadIdx.x == 0) report_timeout(g.status_word, kKernelGemmMx, kSiteSmemAlign);
+    return;
+  }
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem_raw + S * cfg::kStageBytes);
+  const uint32_t bar0 = smem_u32(bars);
+  auto full_bar = [&](int s) { return bar0 + 8u * s; };
+  auto free_bar = [&](int s) { return bar0 + 8u * (S + s); };
+  auto tmem_full_bar = [&](int a) { return bar0 + 8u * (2 * S + a); };
+  auto tmem_empty_bar = [&](int a) { return bar0 + 8u * (2 * S + 2 + a); };
+  const uint32_t drain_bar = bar0 + 8u * (2 * S + 4);
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + cfg::kNumBars);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  const int warp = __shfl_sync(0xffffffffu, static_cast<int>(threadIdx.x) >> 5, 0), lane = threadIdx.x & 31;
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < S; ++s) {
+      mbar_init(full_bar(s), 1);
+      mbar_init(free_bar(s), 1);
+    }
+    for (int a = 0; a < 2; ++a) {
+      mbar_init(tmem_full_bar(a), 1);
+      mbar_init(tmem_empty_bar(a), 2 * cfg::kEpiWarps);
+    }
+    mbar_init(drain_bar, 1);
+    *abort_flag = 0;
+    fence_mbar_init();
+    fence_proxy_async_smem();
+  }
+  if (warp == 1) {
+    tmem_alloc_pair(smem_u32(tmem_slot), cfg::kTmemCols);
+    tmem_relinquish_pair();
+  }
+  tc_fence_before();
+  __syncthreads();
+  cluster_sync_all();  // the peer's barriers are initialised before anything signals them
+  tc_fence_after();
+  const uint32_t tmem_base = __shfl_sync(0xffffffffu, *tmem_slot, 0);
+
+  int M = g.max_m;
+  if (g.m_ptr != nullptr) M = pdl_wait_row_count(g.m_ptr, g.max_m, 0);
+  else pdl_wait();
+  const int N = g.n;
+  const int n_tiles = (N + cfg::BN - 1) / cfg::BN;
+  const int num_tiles = (M + 255) / 256 * n_tiles;
+  const int k_tiles = mx_k_tiles(g.k);
+  // columns of a tile: the last one of a row of tiles has what is left of N, in steps of 64
+  auto columns = [&](int n_tile) { return min(cfg::BN, (N - n_tile * cfg::BN + 63) / 64 * 64); };
+
+  auto fail = [&](int site) {
+    *abort_flag = 1;
+    report_timeout(g.status_word, kKernelGemmMx, site);
+  };
+
+  if (warp == 0) {
+    // ------------------------- producer (both CTAs) -------------------------
+    // all lanes walk through the loop, one issues (see elect_one)
+    const bool issuer = elect_one();
+    if (issuer) {
+      prefetch_tensormap(&tmap_a);
+      prefetch_tensormap(&tmap_w);
+      prefetch_tensormap(&tmap_ws);
+    }
+    {
+      constexpr int kTileLines = kMxTileBytes / 1024;  // 16 of codes (8 rows each), 1 of scales
+      uint32_t stage = 0, phase = 0;
+      long long issued = 0;
+      bool ok = true;
+      for (int tile = pair_id; tile < num_tiles && ok; tile += num_pairs) {
+        const int m_tile = tile / n_tiles, n_tile = tile - m_tile * n_tiles;
+        const int cols = columns(n_tile), n0 = n_tile * cfg::BN;
+        // (row blocks behind the last one are filled with zeros)
+        int a_line = (m_tile * 2 + static_cast<int>(rank)) * k_tiles * kTileLines;
+        const int w_row = n0 + static_cast<int>(rank) * (cols / 2);  // this CTA's first W row, of cols / 2
+        int ws_line = n0 / kMxTileRows * k_tiles * kTileLines + kMxCodeBytes / 1024;
+        int w_line[3];  // 32 W rows each, which never cross a row block
+#pragma unroll
+        for (int j = 0; j < 3; ++j)
+          w_line[j] = (w_row + 32 * j) / kMxTileRows * k_tiles * kTileLines + (w_row + 32 * j) % kMxTileRows / 8;
+        const uint32_t stage_tx = 2u * (kMxTileBytes + cols / 2 * 128 + 2 * kMxScaleBytes);
+        for (int kt = 0; kt < k_tiles; ++kt) {
+          if (!__all_sync(0xffffffffu, mbar_wait(free_bar(stage), phase ^ 1u, abort_flag))) {
+            if (lane == 0) fail(kSiteProducerEmpty);
+            ok = false;
+            break;
+          }
+          const uint32_t dst = tiles_addr + stage * cfg::kStageBytes, w_dst = dst + kMxTileBytes;
+          const uint32_t s_dst = w_dst + cfg::kBCodes, full0 = mapa_shared(full_bar(stage), 0);
+          if (issuer) {
+            if (rank == 0) mbar_arrive_expect_tx(full_bar(stage), stage_tx);
+            tma_load_2d_pair(dst, &tmap_a, 0, a_line, full0);
+            tma_load_2d_pair(w_dst, &tmap_w, 0, w_line[0], full0);
+            if (cols > 64) tma_load_2d_pair(w_dst + 4096, &tmap_w, 0, w_line[1], full0);
+            if (cols > 128) tma_load_2d_pair(w_dst + 8192, &tmap_w, 0, w_line[2], full0);
+            tma_load_2d_pair(s_dst, &tmap_ws, 0, ws_line, full0);
+            tma_load_2d_pair(s_dst + kMxScaleBytes, &tmap_ws, 0, ws_line + k_tiles * kTileLines, full0);
+          }
+          __syncwarp();
+          a_line += kTileLines;
+          ws_line += kTileLines;
+#pragma unroll
+          for (int j = 0; j < 3; ++j) w_line[j] += kTileLines;
+          ++issued;
+          if (++stage == S) {
+            stage = 0;
+            phase ^= 1u;
+          }
+        }
+      }
+      // the issuer's commits on the ring are asynchronous arrivals, in the peer from the other SM: the last of them
+      // land before the barriers go away
+      const long long pending = !issuer ? 0 : issued < S ? issued : S;
+      for (long long i = 0; i < pending; ++i) {
+        const long long f = issued - 1 - i;
+        if (!mbar_wait(free_bar(static_cast<int>(f % S)), static_cast<uint32_t>((f / S) & 1), abort_flag) &&
+            *abort_flag == 0)
+          fail(kSiteProducerDrain);
+      }
+      if (rank == 0) {
+        // full counts both CTAs' bytes: behind these phases no copy of the pair is in flight; the peer learns it at
+        // the closing cluster barrier
+        for (long long i = 0; i < pending; ++i) {
+          const long long f = issued - 1 - i;
+          if (!mbar_drain(full_bar(static_cast<int>(f % S)), static_cast<uint32_t>((f / S) & 1)) && *abort_flag == 0)
+            fail(kSiteProducerDrain);
+        }
+      }
+    }
+  } else if (warp == 1) {
+    // ------------------------- MMA issuer (CTA 0 only) -------------------------
+    // all lanes walk through the loop, one issues (see elect_one)
+    if (rank == 0) {
+      const bool issuer = elect_one();
+      uint32_t stage = 0, phase = 0;
+      int it = 0;
+      bool ok = true;
+      for (int tile = pair_id; tile < num_tiles && ok; tile += num_pairs, ++it) {
+        const int n_tile = tile % n_tiles, cols = columns(n_tile), acc = it & 1;
+        if (!__all_sync(0xffffffffu, mbar_wait(tmem_empty_bar(acc), ((it >> 1) & 1) ^ 1u, abort_flag))) {
+          if (lane == 0) fail(kSiteMmaTmemEmpty);
+          break;
+        }
+        tc_fence_after();
+        const uint32_t d_tmem = tmem_base + acc * cfg::BN;
+        const uint32_t shift = (n_tile & 1) * 2;  // the tile's W rows begin in the middle of a row block
+        const uint32_t idesc0 = make_idesc_mxf4(2 * BM, cols, 0);
+        for (int kt = 0; kt < k_tiles; ++kt) {
+          if (!__all_sync(0xffffffffu, mbar_wait(full_bar(stage), phase, abort_flag))) {
+            if (lane == 0) fail(kSiteMmaFull);
+            ok = false;
+            break;
+          }
+          tc_fence_after();
+          const uint32_t a_addr = tiles_addr + stage * cfg::kStageBytes, b_addr = a_addr + kMxTileBytes;
+          const uint32_t sf = tmem_base + 2 * cfg::BN + stage * cfg::kScaleCols;
+          const int left = g.k - kt * kMxTileK;
+          const int steps = left >= kMxTileK ? 4 : (left + kUmmaK - 1) / kUmmaK;
+          if (issuer) {
+            issue_stage<true, 2>(steps, d_tmem, a_addr, b_addr, b_addr + cfg::kBCodes, sf, sf + 8, shift, idesc0, kt == 0);
+            umma_commit_both(free_bar(stage));
+            if (kt == k_tiles - 1) umma_commit_both(tmem_full_bar(acc));
+          }
+          __syncwarp();
+          if (++stage == S) {
+            stage = 0;
+            phase ^= 1u;
+          }
+        }
+      }
+      // all MMAs must have retired before TMEM is freed
+      if (issuer) {
+        umma_commit_pair(drain_bar);
+        if (!mbar_drain(drain_bar, 0u) && *abort_flag == 0) fail(kSiteMmaDrain);
+      }
+      __syncwarp();
+    }
+  } else {
+    // ------------------------- epilogue (both CTAs) -------------------------
+    const int quad = warp & 3, third = (warp - 2) >> 2;
+    int it = 0;
+    for (int tile = pair_id; tile < num_tiles; tile += num_pairs, ++it) {
+      const int m_tile = tile / n_tiles, n_tile = tile - m_tile * n_tiles, acc = it & 1;
+      const int col0 = n_tile * cfg::BN + third * 64, row0 = m_tile * 256 + static_cast<int>(rank) * BM + quad * 32;
+      Piece<T, OUT, ACT> piece;
+      piece.prepare(g, bias, row0, col0, M, lane);
+      const bool got = mbar_wait(tmem_full_bar(acc), (it >> 1) & 1, abort_flag);
+      if (!__all_sync(0xffffffffu, got)) {
+        if (lane == 0) fail(kSiteEpilogueFull);
+        break;
+      }
+      tc_fence_after();
+      piece.finish(g, tmem_base + (static_cast<uint32_t>(quad * 32) << 16) + acc * cfg::BN + third * 64, row0, col0, M,
+                   lane, [&] {
+                     if (lane == 0) mbar_arrive_cluster(mapa_shared(tmem_empty_bar(acc), 0));
+                   });
+    }
+  }
+
+  tc_fence_before();
+  __syncthreads();
+  cluster_sync_all();  // neither CTA leaves while the other may still touch its barriers or TMEM
+  if (warp == 1) {
+    __syncwarp();
+    tc_fence_after();
+    tmem_dealloc_pair(tmem_base, cfg::kTmemCols);
+  }
+}
+
+// An MXFP4 tensor as lines of 1024 bytes, for boxes of `box` lines.  (Lines of 128 bytes move the same bytes at half
+// the rate.)
+bool encode_lines(CUtensorMap* map, const void* base, int rows, int k, uint32_t box) {
+  EncodeTiledFn fn = get_encode_tiled();
+  if (fn == nullptr) return false;
+  const cuuint64_t dims[2] = {128, mx_bytes(rows, k) / 1024};
+  const cuuint64_t strides[1] = {1024};
+  const cuuint32_t boxes[2] = {128, box};
+  const cuuint32_t elem_strides[2] = {1, 1};
+  return fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT64, 2, const_cast<void*>(base), dims, strides, boxes, elem_strides,
+            CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+            CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+template <typename T, typename OUT, int ACT>
+cudaError_t launch_pair(const MxArgs& g, const T* bias, cudaStream_t stream) {
+  using cfg = PairCfg;
+  static PerDeviceOnce once;
+  const cudaError_t err = once.run([] {
+    return cudaFuncSetAttribute(gemm_mxfp4_pair_kernel<T, OUT, ACT>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                cfg::kSmemBytes);
+  });
+  if (err != cudaSuccess) return err;
+  CUtensorMap ta, tw, tws;
+  if (!encode_lines(&ta, g.a, g.max_m, g.k, kMxTileBytes / 1024) || !encode_lines(&tw, g.w, g.n, g.k, 4) ||
+      !encode_lines(&tws, g.w, g.n, g.k, 1))
+    return cudaErrorInvalidValue;
+  const long long tiles = static_cast<long long>((g.max_m + 255) / 256) * ((g.n + cfg::BN - 1) / cfg::BN);
+  const int pairs = static_cast<int>(tiles < sm_count() / 2 ? tiles : sm_count() / 2);
+  return launch_pdl(gemm_mxfp4_pair_kernel<T, OUT, ACT>, dim3(2 * pairs), dim3(cfg::kThreads), cfg::kSmemBytes, stream,
+                    ta, tw, tws, g, bias);
+}
+
 template <typename T, typename OUT, int ACT>
 cudaError_t launch_act(const MxArgs& g, const T* bias, cudaStream_t stream) {
   using cfg = Cfg<128>;
@@ -415,7 +808,7 @@ cudaError_t launch_act(const MxArgs& g, const T* bias, cudaStream_t stream) {
   });
   if (err != cudaSuccess) return err;
   const long long tiles = static_cast<long long>((g.max_m + BM - 1) / BM) * ((g.n + 127) / 128);
-  if (tiles > 0x7fffffffll) return cudaErrorInvalidValue;
+  if (tiles >= kPairTiles) return launch_pair<T, OUT, ACT>(g, bias, stream);
   const int grid = static_cast<int>(tiles < sm_count() ? tiles : sm_count());
   return launch_pdl(gemm_mxfp4_kernel<T, OUT, ACT>, dim3(grid), dim3(kNumThreads), cfg::kSmemBytes, stream, g, bias);
 }
@@ -446,9 +839,10 @@ cudaError_t launch_gemm_mxfp4(const MxGemm& p, const T* bias, const T* residual,
   if ((c == nullptr) == (p.c_mx == nullptr)) return cudaErrorInvalidValue;
   if (p.c_mx != nullptr && (p.n % 64 != 0 || residual != nullptr)) return cudaErrorInvalidValue;
   if (epilogue != kEpiNone && bias == nullptr) return cudaErrorInvalidValue;
-  for (const void* q : {p.a, p.w, static_cast<const void*>(c), static_cast<const void*>(p.c_mx),
-                        static_cast<const void*>(bias), static_cast<const void*>(residual)})
+  for (const void* q : {static_cast<const void*>(c), static_cast<const void*>(bias), static_cast<const void*>(residual)})
     if (reinterpret_cast<uintptr_t>(q) & 15u) return cudaErrorMisalignedAddress;
+  for (const void* q : {p.a, p.w, static_cast<const void*>(p.c_mx)})
+    if (reinterpret_cast<uintptr_t>(q) & 127u) return cudaErrorMisalignedAddress;
   MxArgs g;
   g.a = static_cast<const uint8_t*>(p.a);
   g.w = static_cast<const uint8_t*>(p.w);

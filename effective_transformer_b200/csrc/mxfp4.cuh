@@ -6,8 +6,12 @@
 // scales for each of 128 rows.  Rows are kept in exactly that form, so that one untiled bulk copy moves an operand
 // tile and its scales and no tensor map is needed: tiles of 128 rows x 256 values, 17408 bytes each, all k-tiles of
 // a row block side by side.
-//   value k of row r in a tile:  byte r * 128 + (((k / 32) ^ (r & 7)) * 16) + (k % 32) / 2, even k in the low nibble
-//   scale of block b = k / 32:   byte 16384 + (b / 4) * 512 + (r % 32) * 16 + (r / 32) * 4 + b % 4
+//   value k of row r in a tile:  byte p * 128 + (((k / 32) ^ (p & 7)) * 16) + (k % 32) / 2, even k in the low nibble
+//   scale of block b = k / 32:   byte 16384 + (b / 4) * 512 + (p % 32) * 16 + (p / 32) * 4 + b % 4
+// with p = r but for its bits 1-2 and 3-4, which change places.  In the accumulator a tensor's rows are lanes (A) or
+// columns (W), and with columns in this order a thread that reads four 8-column groups of a row in the layout of
+// tcgen05.ld 16x256b, two columns of each, has eight neighbouring columns of the result: they go to memory from
+// registers in whole 32-byte sectors, without a turn through shared memory, whose bandwidth the product is short of.
 // A 16-byte piece of a row is one scale block.  Rows past the row count and, in a valid row, blocks past the width
 // rounded up to 64 hold anything; the one block between an odd width / 32 and that multiple of 64 is zero.
 #pragma once
@@ -33,10 +37,16 @@ inline size_t mx_bytes(long long rows, int k) {
 __device__ __forceinline__ size_t mx_tile_offset(int row, int kt, int k_tiles) {
   return (static_cast<size_t>(row >> 7) * k_tiles + kt) * kMxTileBytes;
 }
+// Where row r stands in its group of 32 (and which row stands at r: the exchange is its own inverse).
+__host__ __device__ constexpr int mx_row(int r) { return (r & ~0x1e) | ((r & 0x18) >> 2) | ((r & 0x06) << 2); }
 // Within a tile: the 16-byte piece of block b (0..7) of row r (0..127), and its scale byte.
-__device__ __forceinline__ int mx_code_offset(int r, int b) { return r * 128 + ((b ^ (r & 7)) << 4); }
+__device__ __forceinline__ int mx_code_offset(int r, int b) {
+  const int p = mx_row(r);
+  return p * 128 + ((b ^ (p & 7)) << 4);
+}
 __device__ __forceinline__ int mx_scale_offset(int r, int b) {
-  return kMxCodeBytes + (b >> 2) * 512 + (r & 31) * 16 + (r >> 5) * 4 + (b & 3);
+  const int p = mx_row(r);
+  return kMxCodeBytes + (b >> 2) * 512 + (p & 31) * 16 + (p >> 5) * 4 + (b & 3);
 }
 
 // Scale of a block from the bits of its largest magnitude (fp32): 2^(floor(log2 amax) - 2), since the largest code

@@ -180,7 +180,7 @@ cudaError_t launch_mx_quantize(const T* x, long long row_stride, const int* m_pt
   if (max_m <= 0) return cudaSuccess;
   if (k <= 0 || k % kMxBlock != 0 || row_stride < k) return cudaErrorInvalidValue;
   if ((reinterpret_cast<uintptr_t>(x) & 15u) || (row_stride * sizeof(T)) % 16 != 0 ||
-      (reinterpret_cast<uintptr_t>(mx) & 15u))
+      (reinterpret_cast<uintptr_t>(mx) & 127u))
     return cudaErrorMisalignedAddress;
   return launch_pdl(mx_quantize_kernel<T>, dim3(mx_grid(max_m, k)), dim3(kThreads), 0, stream, x, row_stride, m_ptr,
                     max_m, k, static_cast<uint8_t*>(mx));
@@ -190,7 +190,7 @@ template <typename T>
 cudaError_t launch_mx_dequantize(const void* mx, const int* m_ptr, int max_m, int k, T* out, cudaStream_t stream) {
   if (max_m <= 0) return cudaSuccess;
   if (k <= 0 || k % kMxBlock != 0) return cudaErrorInvalidValue;
-  if ((reinterpret_cast<uintptr_t>(out) & 15u) || (reinterpret_cast<uintptr_t>(mx) & 15u))
+  if ((reinterpret_cast<uintptr_t>(out) & 15u) || (reinterpret_cast<uintptr_t>(mx) & 127u))
     return cudaErrorMisalignedAddress;
   return launch_pdl(mx_dequantize_kernel<T>, dim3(mx_grid(max_m, k)), dim3(kThreads), 0, stream,
                     static_cast<const uint8_t*>(mx), m_ptr, max_m, k, out);
@@ -199,7 +199,7 @@ cudaError_t launch_mx_dequantize(const void* mx, const int* m_ptr, int max_m, in
 template <typename T>
 cudaError_t launch_mx_pack_weight(const T* w, void* mx, int k, int n, cudaStream_t stream) {
   if (k <= 0 || n <= 0 || k % kMxBlock != 0 || (k + 63) / 64 * 2 > 65535) return cudaErrorInvalidValue;
-  if (reinterpret_cast<uintptr_t>(mx) & 15u) return cudaErrorMisalignedAddress;
+  if (reinterpret_cast<uintptr_t>(mx) & 127u) return cudaErrorMisalignedAddress;
   const dim3 grid((n + kThreads - 1) / kThreads, (k + 63) / 64 * 2);
   mx_pack_weight_kernel<T><<<grid, kThreads, 0, stream>>>(w, static_cast<uint8_t*>(mx), k, n);
   return cudaGetLastError();

@@ -238,9 +238,9 @@ cudaError_t launch_gated_norm(const GatedNorm& p, cudaStream_t stream) {
   if (p.x == nullptr || (p.h == nullptr && p.y == nullptr && p.y_mx == nullptr)) return cudaErrorInvalidValue;
   if (p.gate != nullptr && p.gate_rows < 1) return cudaErrorInvalidValue;
   for (const void* q : {p.x, p.bias, p.residual, p.gate, p.post_gamma, p.post_beta, p.pre_gamma, p.pre_beta,
-                        static_cast<const void*>(p.h), static_cast<const void*>(p.y),
-                        static_cast<const void*>(p.y_mx)})
+                        static_cast<const void*>(p.h), static_cast<const void*>(p.y)})
     if (reinterpret_cast<uintptr_t>(q) & 15u) return cudaErrorMisalignedAddress;
+  if (reinterpret_cast<uintptr_t>(p.y_mx) & 127u) return cudaErrorMisalignedAddress;
   const int vecs = p.n / E;
   for (int wpr = 1; wpr <= kWarps; wpr *= 2) {
     const int v = (vecs + 32 * wpr - 1) / (32 * wpr);

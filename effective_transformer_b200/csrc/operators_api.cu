@@ -8,6 +8,8 @@ using namespace etb;
 
 namespace {
 
+constexpr char kAlignment[] = "pointers must be 16-byte aligned, those of MXFP4 tensors 128-byte aligned";
+
 int refuse(const char* msg) {
   set_global_error(msg);
   return ET_INVALID_ARGUMENT;
@@ -30,6 +32,7 @@ int guarded(F f) {
 }
 
 bool misaligned(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) != 0; }
+bool misaligned_mx(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 127u) != 0; }
 bool known_dtype(int dtype) { return dtype == ET_FP16 || dtype == ET_FP32; }
 size_t size_of(int dtype) { return dtype == ET_FP16 ? 2 : 4; }
 
@@ -48,8 +51,8 @@ int check_gemm(int dtype, const void* a, const void* w_mx, const void* bias, con
   if (c_mx != nullptr && (n % 64 != 0 || residual != nullptr))
     return refuse("MXFP4 output needs n a multiple of 64 and takes no residual");
   if (a == nullptr || w_mx == nullptr || (epilogue != kEpiNone && bias == nullptr)) return refuse("null pointer");
-  if (misaligned(a) || misaligned(w_mx) || misaligned(bias) || misaligned(residual) || misaligned(c) || misaligned(c_mx))
-    return refuse("pointers must be 16-byte aligned");
+  if (misaligned(a) || misaligned(bias) || misaligned(residual) || misaligned(c) || misaligned_mx(w_mx) || misaligned_mx(c_mx))
+    return refuse(kAlignment);
   return ET_OK;
 }
 
@@ -95,7 +98,7 @@ int et_mxfp4_quantize(int dtype, const void* x, long long row_stride, const int*
       return refuse("max_m must not be negative, row_stride at least k and a multiple of 16 bytes");
     if (max_m == 0) return static_cast<int>(ET_OK);
     if (x == nullptr || mx == nullptr) return refuse("null pointer");
-    if (misaligned(x) || misaligned(mx)) return refuse("pointers must be 16-byte aligned");
+    if (misaligned(x) || misaligned_mx(mx)) return refuse(kAlignment);
     return run_quantize(dtype, x, row_stride, m_ptr, max_m, k, mx, static_cast<cudaStream_t>(stream));
   });
 }
@@ -107,7 +110,7 @@ int et_mxfp4_dequantize(int dtype, const void* mx, const int* m_ptr, int max_m, 
     if (max_m < 0) return refuse("max_m must not be negative");
     if (max_m == 0) return static_cast<int>(ET_OK);
     if (mx == nullptr || out == nullptr) return refuse("null pointer");
-    if (misaligned(mx) || misaligned(out)) return refuse("pointers must be 16-byte aligned");
+    if (misaligned_mx(mx) || misaligned(out)) return refuse(kAlignment);
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     if (dtype == ET_FP16)
       return status_of(launch_mx_dequantize<__half>(mx, m_ptr, max_m, k, static_cast<__half*>(out), s),
@@ -123,7 +126,7 @@ int et_mxfp4_pack_weight(int dtype, const void* w, void* w_mx, int k, int n, voi
     if (int rc = check_width(k)) return rc;
     if (n <= 0 || n % 32 != 0) return refuse("n must be a positive multiple of 32");
     if (w == nullptr || w_mx == nullptr) return refuse("null pointer");
-    if (misaligned(w_mx)) return refuse("pointers must be 16-byte aligned");
+    if (misaligned_mx(w_mx)) return refuse(kAlignment);
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     if (dtype == ET_FP16)
       return status_of(launch_mx_pack_weight<__half>(static_cast<const __half*>(w), w_mx, k, n, s),
@@ -136,6 +139,7 @@ int et_mxfp4_gemm(int dtype, const void* a_mx, const void* w_mx, const void* bia
                   void* c_mx, const int* m_ptr, int max_m, int n, int k, int epilogue, int* status_word, void* stream) {
   return guarded([&] {
     if (int rc = check_gemm(dtype, a_mx, w_mx, bias, residual, c, c_mx, max_m, n, k, epilogue)) return rc;
+    if (misaligned_mx(a_mx)) return refuse(kAlignment);
     if (max_m == 0) return static_cast<int>(ET_OK);
     return run_gemm(dtype, a_mx, w_mx, bias, residual, c, c_mx, m_ptr, max_m, n, k, epilogue, status_word,
                     static_cast<cudaStream_t>(stream));
@@ -150,14 +154,14 @@ int et_mxfp4_linear(int dtype, const void* x, long long row_stride, void* x_mx, 
     if (row_stride < k || row_stride * size_of(dtype) % 16 != 0)
       return refuse("row_stride must be at least k and a multiple of 16 bytes");
     if (max_m == 0) return static_cast<int>(ET_OK);
-    if (x_mx == nullptr || misaligned(x_mx)) return refuse("x_mx must be 16-byte aligned device memory");
+    if (x_mx == nullptr || misaligned_mx(x_mx)) return refuse("x_mx must be 128-byte aligned device memory");
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     if (int rc = run_quantize(dtype, x, row_stride, m_ptr, max_m, k, x_mx, s)) return rc;
     return run_gemm(dtype, x_mx, w_mx, bias, residual, c, c_mx, m_ptr, max_m, n, k, epilogue, status_word, s);
   });
 }
 
-int et_gated_residual_norm(int dtype, const et_gated_norm_param_t* p) {
+int et_gated_residual_norm(int dtype, const et_gated_norm_param_t* p, void* stream) {
   return guarded([&] {
     if (!known_dtype(dtype)) return refuse("dtype must be ET_FP16 or ET_FP32");
     if (p == nullptr) return refuse("null pointer");
@@ -178,9 +182,9 @@ int et_gated_residual_norm(int dtype, const et_gated_norm_param_t* p) {
     if (p->max_m == 0) return static_cast<int>(ET_OK);
     if (p->x == nullptr) return refuse("null pointer");
     for (const void* q : {p->x, p->bias, p->residual, p->gate, p->post_gamma, p->post_beta, p->pre_gamma, p->pre_beta,
-                          static_cast<const void*>(p->h_out), static_cast<const void*>(p->y_out),
-                          static_cast<const void*>(p->y_mx)})
-      if (misaligned(q)) return refuse("pointers must be 16-byte aligned");
+                          static_cast<const void*>(p->h_out), static_cast<const void*>(p->y_out)})
+      if (misaligned(q)) return refuse(kAlignment);
+    if (misaligned_mx(p->y_mx)) return refuse(kAlignment);
     GatedNorm g;
     g.x = p->x, g.bias = p->bias, g.residual = p->residual, g.gate = p->gate;
     g.batch_idx = p->gate_rows > 1 ? p->batch_idx : nullptr;
@@ -191,7 +195,7 @@ int et_gated_residual_norm(int dtype, const et_gated_norm_param_t* p) {
     g.post_gamma = p->post_gamma, g.post_beta = p->post_beta, g.pre_gamma = p->pre_gamma, g.pre_beta = p->pre_beta;
     g.h = p->h_out, g.y = p->y_out, g.y_mx = p->y_mx;
     g.m_ptr = p->m_ptr, g.max_m = p->max_m, g.n = p->n;
-    cudaStream_t s = static_cast<cudaStream_t>(p->stream);
+    cudaStream_t s = static_cast<cudaStream_t>(stream);
     return dtype == ET_FP16 ? status_of(launch_gated_norm<__half>(g, s), "et_gated_residual_norm")
                             : status_of(launch_gated_norm<float>(g, s), "et_gated_residual_norm");
   });

@@ -187,6 +187,18 @@ __device__ __forceinline__ void tmem_ld_32x32b_x16(uint32_t taddr, uint32_t* r) 
       : "r"(taddr)
       : "memory");
 }
+// 16 lanes x 32 columns: thread i of the warp reads lanes i / 4 and i / 4 + 8 behind the lane field of taddr, columns
+// 2 (i % 4) and + 1 of each group of 8: r[4 g + 2 h + e] = lane i / 4 + 8 h, column 8 g + 2 (i % 4) + e.
+__device__ __forceinline__ void tmem_ld_16x256b_x4(uint32_t taddr, uint32_t* r) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.16x256b.x4.b32 "
+      "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]),
+        "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]),
+        "=r"(r[14]), "=r"(r[15])
+      : "r"(taddr)
+      : "memory");
+}
 __device__ __forceinline__ void tmem_ld_wait() {
   asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
 }
@@ -251,6 +263,16 @@ __device__ __forceinline__ void umma_commit_pair(uint32_t bar_cluster_addr) {
                : "memory");
 }
 
+// One lane of a converged warp.  Code that all lanes walk through, with only the issuing instructions under this
+// predicate, keeps descriptors and addresses in uniform registers, where tcgen05.mma and tcgen05.cp take them from.
+__device__ __forceinline__ bool elect_one() {
+  uint32_t e;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(e));
+  return e != 0;
+}
+
 // ---- block-scaled MMA (kind::mxf4: e2m1 operands, one e8m0 scale per 32 values of K) ----
 // 512 bytes of scales (32 rows of 16 bytes, one 4-byte word per 32 operand rows) from shared memory into columns
 // [taddr, taddr + 4) of all four lane quadrants.  Ordered in front of the MMAs that the same thread issues after it.
@@ -267,6 +289,20 @@ __device__ __forceinline__ void umma_mxf4_ss(uint32_t tmem_d, uint64_t adesc, ui
       ::"r"(tmem_d), "l"(adesc), "l"(bdesc), "r"(idesc), "r"(tmem_sfa), "r"(tmem_sfb), "r"(accumulate)
       : "memory");
 }
+// The same for a CTA pair: the scales go from each CTA's own shared memory (same offset) to its own tensor memory, and
+// one MMA covers both CTAs' rows (M = 256).
+__device__ __forceinline__ void tmem_cp_scales_pair(uint32_t taddr, uint64_t sdesc) {
+  asm volatile("tcgen05.cp.cta_group::2.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(sdesc) : "memory");
+}
+__device__ __forceinline__ void umma_mxf4_ss_pair(uint32_t tmem_d, uint64_t adesc, uint64_t bdesc, uint32_t idesc,
+                                                  uint32_t tmem_sfa, uint32_t tmem_sfb, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %6, 0;\n\t"
+      "tcgen05.mma.cta_group::2.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%4], [%5], p;\n\t}"
+      ::"r"(tmem_d), "l"(adesc), "l"(bdesc), "r"(idesc), "r"(tmem_sfa), "r"(tmem_sfb), "r"(accumulate)
+      : "memory");
+}
 // Descriptor of such a 512-byte piece: no swizzle, 8-row groups of 128 bytes one behind the other.
 __device__ __forceinline__ uint64_t make_scale_desc(uint32_t smem_addr) {
   return static_cast<uint64_t>((smem_addr & 0x3FFFFu) >> 4) | (1ull << 16) | (8ull << 32) | (1ull << 46);
@@ -277,6 +313,14 @@ __device__ __forceinline__ uint64_t make_scale_desc(uint32_t smem_addr) {
 __host__ __device__ constexpr uint32_t make_idesc_mxf4(int m, int n, int scale_byte) {
   return (static_cast<uint32_t>(scale_byte) << 4) | (1u << 7) | (1u << 10) | (static_cast<uint32_t>(n >> 3) << 17) |
          (1u << 23) | (static_cast<uint32_t>(m >> 4) << 24) | (static_cast<uint32_t>(scale_byte) << 29);
+}
+
+// Arrives on the mbarrier at this offset in both CTAs of the pair.
+__device__ __forceinline__ void umma_commit_both(uint32_t bar) {
+  asm volatile(
+      "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;"
+      ::"r"(bar), "h"(static_cast<uint16_t>(3))
+      : "memory");
 }
 
 // Shared-memory matrix descriptor for a K-major operand tile laid out by TMA

@@ -14,7 +14,6 @@ them.  Tensors must be contiguous (x of quantize and linear: contiguous rows) an
 """
 from __future__ import annotations
 
-import ctypes as C
 from typing import Dict, Optional, Union
 
 import torch
@@ -26,15 +25,18 @@ __all__ = ["MxTensor", "empty", "quantize", "dequantize", "pack_weight", "gemm",
 _DTYPE = {torch.float16: _capi.ET_FP16, torch.float32: _capi.ET_FP32}
 _EPILOGUE = {None: 1, "gelu": 2, "tanh": 3}
 _status: Dict[int, torch.Tensor] = {}
+_lib = None
 
 
 class MxTensor:
-    """`rows` rows of `cols` values in MXFP4; `data` is the device buffer, in the layout of the tensor core."""
+    """`rows` rows of `cols` values in MXFP4; `data` is the device buffer, in the layout of the tensor core (`ptr` its
+    address, `device` the index of its GPU)."""
 
-    __slots__ = ("data", "rows", "cols")
+    __slots__ = ("data", "rows", "cols", "ptr", "device")
 
     def __init__(self, data: torch.Tensor, rows: int, cols: int):
         self.data, self.rows, self.cols = data, rows, cols
+        self.ptr, self.device = data.data_ptr(), data.get_device()
 
     def __repr__(self) -> str:
         return f"MxTensor({self.rows} x {self.cols}, {self.data.device})"
@@ -45,74 +47,80 @@ def _require(ok: bool, message: str) -> None:
         raise ValueError(message)
 
 
-def _check(t: Optional[torch.Tensor], name: str, shape, dtype: torch.dtype, device: torch.device) -> None:
-    if t is None:
-        return
-    _require(isinstance(t, torch.Tensor) and t.is_contiguous() and t.dtype == dtype and t.device == device
-             and tuple(t.shape) == shape, f"{name} must be a contiguous {list(shape)} tensor of dtype {dtype} on {device}")
+# The checks run in front of every launch, and for few rows they are what a call costs: one comparison per property,
+# and the text of an error is put together only when it is raised.  Devices are compared by index (get_device(), -1 on
+# the CPU).
+
+def _check(t: Optional[torch.Tensor], name: str, shape, dtype: torch.dtype, device: int) -> None:
+    if t is not None and not (isinstance(t, torch.Tensor) and t.dtype is dtype and t.shape == shape
+                              and t.get_device() == device and t.is_contiguous()):
+        raise ValueError(f"{name} must be a contiguous {list(shape)} tensor of dtype {dtype} on cuda:{device}")
 
 
-def _check_rows(t: torch.Tensor, name: str) -> None:
-    _require(isinstance(t, torch.Tensor) and t.is_cuda and t.dtype in _DTYPE and t.dim() == 2,
-             f"{name} must be a [rows, width] CUDA tensor of dtype torch.float16 or torch.float32")
-    _require(t.shape[1] > 0 and t.shape[1] % 32 == 0, f"the width of {name} must be a positive multiple of 32")
+def _check_rows(x: torch.Tensor, name: str):
+    """(rows, width, row stride, device) of a matrix whose rows may be strided."""
+    if not (isinstance(x, torch.Tensor) and x.dtype in _DTYPE and x.dim() == 2 and x.is_cuda):
+        raise ValueError(f"{name} must be a [rows, width] CUDA tensor of dtype torch.float16 or torch.float32")
+    rows, width = x.shape
+    if width <= 0 or width % 32 != 0:
+        raise ValueError(f"the width of {name} must be a positive multiple of 32")
+    stride, step = x.stride()
+    if step != 1:
+        raise ValueError(f"the values of a row of {name} must be contiguous")
+    return rows, width, stride if rows > 1 else width, x.get_device()   # (torch gives a single row any stride)
 
 
-def _check_count(valid_rows: Optional[torch.Tensor], device: torch.device) -> None:
+def _count(valid_rows: Optional[torch.Tensor], device: int) -> Optional[int]:
     if valid_rows is None:
-        return
-    _require(isinstance(valid_rows, torch.Tensor) and valid_rows.dtype == torch.int32 and valid_rows.numel() == 1
-             and valid_rows.device == device, "valid_rows must be one int32 on the rows' device")
+        return None
+    if not (isinstance(valid_rows, torch.Tensor) and valid_rows.dtype is torch.int32 and valid_rows.numel() == 1
+            and valid_rows.get_device() == device):
+        raise ValueError("valid_rows must be one int32 on the rows' device")
+    return valid_rows.data_ptr()
 
 
-def _check_mx(t: MxTensor, name: str, rows: Optional[int], cols: int, device: torch.device) -> None:
-    _require(isinstance(t, MxTensor), f"{name} must be an MxTensor")
-    _require(t.cols == cols and (rows is None or t.rows >= rows) and t.data.device == device,
-             f"{name} must be an MxTensor of {'' if rows is None else f'at least {rows} rows of '}{cols} values on {device}")
+def _check_mx(t: "MxTensor", name: str, rows: int, cols: int, device: int) -> None:
+    if not (isinstance(t, MxTensor) and t.cols == cols and t.rows >= rows and t.device == device):
+        raise ValueError(f"{name} must be an MxTensor of at least {rows} rows of {cols} values on cuda:{device}")
 
 
 def _ptr(t: Optional[torch.Tensor]) -> Optional[int]:
     return None if t is None else t.data_ptr()
 
 
-class _On:
-    """Makes a tensor's device current for a call (the library launches on the current device)."""
-
-    __slots__ = ("device", "previous")
-
-    def __init__(self, device: torch.device):
-        self.device, self.previous = device.index, -1
-
-    def __enter__(self) -> int:
-        if torch.cuda.current_device() != self.device:
-            self.previous = torch.cuda.current_device()
-            torch.cuda.set_device(self.device)
-        return torch.cuda.current_stream().cuda_stream
-
-    def __exit__(self, *exc) -> None:
-        if self.previous >= 0:
-            torch.cuda.set_device(self.previous)
+def _call(device: int, name: str, *args) -> None:
+    """One entry point of the library on the current stream of `device` (it launches on the current device)."""
+    global _lib
+    if _lib is None:
+        _lib = _capi.load()
+    stream = torch._C._cuda_getCurrentRawStream(device)
+    if torch._C._cuda_getDevice() == device:
+        rc = getattr(_lib, name)(*args, stream)
+    else:
+        with torch.cuda.device(device):
+            rc = getattr(_lib, name)(*args, stream)
+    if rc != 0:
+        _capi.check(rc)
 
 
-def _status_word(device: torch.device) -> torch.Tensor:
-    word = _status.get(device.index)
+def _status_word(device: int) -> int:
+    word = _status.get(device)
     if word is None:
         _require(not torch.cuda.is_current_stream_capturing(),
                  "call mxfp4.device_status(device) once before a product is captured on this device")
-        word = _status[device.index] = torch.zeros(1, dtype=torch.int32, device=device)
-    return word
+        word = _status[device] = torch.zeros(1, dtype=torch.int32, device=torch.device("cuda", device))
+    return word.data_ptr()
 
 
 def device_status(device: Union[int, str, torch.device] = "cuda") -> int:
     """0, or the code of a bounded device-side wait that ran out in a product on this device since the last call
     (its results are then incomplete).  Waits for the device's current stream."""
     device = torch.device(device) if not isinstance(device, int) else torch.device("cuda", device)
-    if device.index is None:
-        device = torch.device("cuda", torch.cuda.current_device())
-    word = _status_word(device)
-    code = int(word.item())
+    index = torch.cuda.current_device() if device.index is None else device.index
+    _status_word(index)
+    code = int(_status[index].item())
     if code != 0:
-        word.zero_()
+        _status[index].zero_()
     return code
 
 
@@ -125,22 +133,13 @@ def empty(rows: int, cols: int, device: Union[str, torch.device] = "cuda") -> Mx
 
 def quantize(x: torch.Tensor, valid_rows: Optional[torch.Tensor] = None, out: Optional[MxTensor] = None) -> MxTensor:
     """Rows of x [rows, width] to MXFP4 (rows may be strided, the values of a row are contiguous)."""
-    _check_rows(x, "x")
-    _require(x.stride(1) == 1, "the values of a row of x must be contiguous")
-    _check_count(valid_rows, x.device)
+    rows, k, stride, device = _check_rows(x, "x")
+    count = _count(valid_rows, device)
     if out is None:
-        out = empty(x.shape[0], x.shape[1], x.device)
-    _check_mx(out, "out", x.shape[0], x.shape[1], x.device)
-    with _On(x.device) as stream:
-        _capi.check(_capi.load().et_mxfp4_quantize(
-            _DTYPE[x.dtype], x.data_ptr(), _row_stride(x), _ptr(valid_rows), x.shape[0], x.shape[1],
-            out.data.data_ptr(), stream))
+        out = empty(rows, k, x.device)
+    _check_mx(out, "out", rows, k, device)
+    _call(device, "et_mxfp4_quantize", _DTYPE[x.dtype], x.data_ptr(), stride, count, rows, k, out.ptr)
     return out
-
-
-def _row_stride(x: torch.Tensor) -> int:
-    # (torch gives a single row any stride)
-    return x.shape[1] if x.shape[0] <= 1 else x.stride(0)
 
 
 def dequantize(mx: MxTensor, dtype: torch.dtype, valid_rows: Optional[torch.Tensor] = None,
@@ -148,15 +147,13 @@ def dequantize(mx: MxTensor, dtype: torch.dtype, valid_rows: Optional[torch.Tens
     """The values that an MXFP4 tensor stands for, as [rows, cols] of `dtype`."""
     _require(isinstance(mx, MxTensor), "mx must be an MxTensor")
     _require(dtype in _DTYPE, "dtype must be torch.float16 or torch.float32")
-    rows = mx.rows if out is None else out.shape[0]
     if out is None:
         out = torch.empty(mx.rows, mx.cols, dtype=dtype, device=mx.data.device)
+    rows = out.shape[0]
     _require(rows <= mx.rows, "out has more rows than mx")
-    _check(out, "out", (rows, mx.cols), dtype, mx.data.device)
-    _check_count(valid_rows, mx.data.device)
-    with _On(mx.data.device) as stream:
-        _capi.check(_capi.load().et_mxfp4_dequantize(_DTYPE[dtype], mx.data.data_ptr(), _ptr(valid_rows), rows, mx.cols,
-                                                     out.data_ptr(), stream))
+    _check(out, "out", (rows, mx.cols), dtype, mx.device)
+    _call(mx.device, "et_mxfp4_dequantize", _DTYPE[dtype], mx.ptr, _count(valid_rows, mx.device), rows, mx.cols,
+          out.data_ptr())
     return out
 
 
@@ -167,47 +164,29 @@ def pack_weight(kernel: torch.Tensor) -> MxTensor:
     k, n = kernel.shape
     _require(k > 0 and n > 0 and k % 32 == 0 and n % 32 == 0, "in and out must be positive multiples of 32")
     w = empty(n, k, kernel.device)
-    with _On(kernel.device) as stream:
-        _capi.check(_capi.load().et_mxfp4_pack_weight(_DTYPE[kernel.dtype], kernel.data_ptr(), w.data.data_ptr(), k, n,
-                                                      stream))
+    _call(w.device, "et_mxfp4_pack_weight", _DTYPE[kernel.dtype], kernel.data_ptr(), w.ptr, k, n)
     return w
 
 
-def _product(a, stride: Optional[int], workspace: Optional[MxTensor], rows: int, device: torch.device, weight: MxTensor,
-             bias, activation, residual, valid_rows, out, dtype: Optional[torch.dtype]):
-    _require(isinstance(weight, MxTensor) and weight.data.device == device, "weight must be an MxTensor on the rows' device")
-    k, n = weight.cols, weight.rows
+def _result(rows: int, device: int, weight: MxTensor, bias, activation, residual, valid_rows, out, dtype: torch.dtype):
+    """(out, arguments of the entry points from the bias on) of a product of `rows` rows."""
+    n = weight.rows
     _require(activation in _EPILOGUE, "activation must be None, 'gelu' or 'tanh'")
     _require(activation is None or bias is not None, "an activation needs a bias")
-    to_mx = isinstance(out, MxTensor)
-    if dtype is None:
-        given = next((t for t in (None if to_mx else out, bias, residual) if t is not None), None)
-        dtype = torch.float16 if given is None else given.dtype
-    _require(dtype in _DTYPE, "dtype must be torch.float16 or torch.float32")
-    if out is None:
-        out = torch.empty(rows, n, dtype=dtype, device=device)
-    if to_mx:
+    if isinstance(out, MxTensor):
         _check_mx(out, "out", rows, n, device)
         _require(n % 64 == 0 and residual is None, "MXFP4 output needs a width that is a multiple of 64, and no residual")
+        c, c_mx = None, out.ptr
     else:
-        _check(out, "out", (rows, n), dtype, device)
+        if out is None:
+            out = torch.empty(rows, n, dtype=dtype, device=torch.device("cuda", device))
+        else:
+            _check(out, "out", (rows, n), dtype, device)
+        c, c_mx = out.data_ptr(), None
     _check(bias, "bias", (n,), dtype, device)
     _check(residual, "residual", (rows, n), dtype, device)
-    _check_count(valid_rows, device)
-    epilogue = 0 if bias is None else _EPILOGUE[activation]
-    c, c_mx = (None, out.data.data_ptr()) if to_mx else (out.data_ptr(), None)
-    lib = _capi.load()
-    with _On(device) as stream:
-        word = _status_word(device).data_ptr()
-        if stride is None:
-            rc = lib.et_mxfp4_gemm(_DTYPE[dtype], a, weight.data.data_ptr(), _ptr(bias), _ptr(residual), c, c_mx,
-                                   _ptr(valid_rows), rows, n, k, epilogue, word, stream)
-        else:
-            rc = lib.et_mxfp4_linear(_DTYPE[dtype], a, stride, workspace.data.data_ptr(), weight.data.data_ptr(),
-                                     _ptr(bias), _ptr(residual), c, c_mx, _ptr(valid_rows), rows, n, k, epilogue, word,
-                                     stream)
-    _capi.check(rc)
-    return out
+    return out, (_ptr(bias), _ptr(residual), c, c_mx, _count(valid_rows, device), rows, n, weight.cols,
+                 0 if bias is None else _EPILOGUE[activation], _status_word(device))
 
 
 def gemm(a: MxTensor, weight: MxTensor, bias: Optional[torch.Tensor] = None, activation: Optional[str] = None,
@@ -217,11 +196,17 @@ def gemm(a: MxTensor, weight: MxTensor, bias: Optional[torch.Tensor] = None, act
     """act(A W + bias) (+ residual) on rows that are in MXFP4 already.  The result has the dtype of out, bias or
     residual, or `dtype` (torch.float16 where nothing says); an MxTensor as out keeps it in 4 bits.  out may be residual."""
     _require(isinstance(a, MxTensor) and isinstance(weight, MxTensor), "a and weight must be MxTensors")
-    _require(a.cols == weight.cols, "a and weight must have the same inner width")
-    rows = out.shape[0] if isinstance(out, torch.Tensor) else a.rows
+    _require(a.cols == weight.cols and a.device == weight.device, "a and weight must have one inner width and device")
+    plain = isinstance(out, torch.Tensor)
+    rows = out.shape[0] if plain else a.rows
     _require(rows <= a.rows, "out has more rows than a")
-    return _product(a.data.data_ptr(), None, None, rows, a.data.device, weight, bias, activation, residual, valid_rows,
-                    out, dtype)
+    if dtype is None:
+        given = out if plain else bias if bias is not None else residual
+        dtype = torch.float16 if given is None else given.dtype
+    _require(dtype in _DTYPE, "dtype must be torch.float16 or torch.float32")
+    out, args = _result(rows, a.device, weight, bias, activation, residual, valid_rows, out, dtype)
+    _call(a.device, "et_mxfp4_gemm", _DTYPE[dtype], a.ptr, weight.ptr, *args)
+    return out
 
 
 def linear(x: torch.Tensor, weight: MxTensor, bias: Optional[torch.Tensor] = None, activation: Optional[str] = None,
@@ -230,11 +215,13 @@ def linear(x: torch.Tensor, weight: MxTensor, bias: Optional[torch.Tensor] = Non
            out: Union[torch.Tensor, MxTensor, None] = None) -> Union[torch.Tensor, MxTensor]:
     """gemm(quantize(x), weight, ...) in one call; the result has x's dtype.  `workspace` takes x in MXFP4 (a program
     that calls this in a loop keeps one per stream)."""
-    _check_rows(x, "x")
-    _require(isinstance(weight, MxTensor) and x.shape[1] == weight.cols, "weight must be an MxTensor of x's width")
-    _require(x.stride(1) == 1, "the values of a row of x must be contiguous")
+    rows, k, stride, device = _check_rows(x, "x")
+    _require(isinstance(weight, MxTensor) and weight.cols == k and weight.device == device,
+             "weight must be an MxTensor of x's width and device")
     if workspace is None:
-        workspace = empty(x.shape[0], x.shape[1], x.device)
-    _check_mx(workspace, "workspace", x.shape[0], x.shape[1], x.device)
-    return _product(x.data_ptr(), _row_stride(x), workspace, x.shape[0], x.device, weight, bias, activation, residual,
-                    valid_rows, out, x.dtype)
+        workspace = empty(rows, k, x.device)
+    _check_mx(workspace, "workspace", rows, k, device)
+    dtype = x.dtype
+    out, args = _result(rows, device, weight, bias, activation, residual, valid_rows, out, dtype)
+    _call(device, "et_mxfp4_linear", _DTYPE[dtype], x.data_ptr(), stride, workspace.ptr, weight.ptr, *args)
+    return out

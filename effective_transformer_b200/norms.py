@@ -14,7 +14,7 @@ from typing import Optional, Tuple
 import torch
 
 from . import _capi
-from .mxfp4 import MxTensor, _check, _check_count, _check_mx, _DTYPE, _On, _ptr, _require
+from .mxfp4 import MxTensor, _call, _check, _check_mx, _count, _DTYPE, _ptr, _require
 
 __all__ = ["gated_residual_norm"]
 
@@ -38,44 +38,49 @@ def gated_residual_norm(x: torch.Tensor, bias: Optional[torch.Tensor] = None, re
     they are.  h_out / y_out: buffers for the results, either may be x or residual.  mx_out takes y in MXFP4 for the
     projection behind it; y itself is then written only where y_out is given (None is returned otherwise).  The width
     is a multiple of 16 bytes (of 32 with mx_out), at most 8192 (fp16) or 4096 (fp32)."""
-    _require(isinstance(x, torch.Tensor) and x.is_cuda and x.dtype in _DTYPE and x.dim() == 2 and x.is_contiguous(),
-             "x must be a contiguous [rows, width] CUDA tensor of dtype torch.float16 or torch.float32")
-    rows, n = x.shape
-    dtype, device = x.dtype, x.device
-    _require(post_norm in _KIND and pre_norm in _KIND, "post_norm and pre_norm must be 'none', 'layer' or 'rms'")
+    if not (isinstance(x, torch.Tensor) and x.dtype in _DTYPE and x.dim() == 2 and x.is_cuda and x.is_contiguous()):
+        raise ValueError("x must be a contiguous [rows, width] CUDA tensor of dtype torch.float16 or torch.float32")
+    shape, dtype, device = x.shape, x.dtype, x.get_device()
+    rows, n = shape
+    row = (n,)
+    post, pre = _KIND.get(post_norm), _KIND.get(pre_norm)
+    _require(post is not None and pre is not None, "post_norm and pre_norm must be 'none', 'layer' or 'rms'")
     if h_out is None:
         h_out = torch.empty_like(x)
     if y_out is None and mx_out is None:
         y_out = torch.empty_like(x)
-    for name, t in (("residual", residual), ("h_out", h_out), ("y_out", y_out)):
-        _check(t, name, (rows, n), dtype, device)
-    _require(y_out is None or y_out.data_ptr() != h_out.data_ptr() or rows == 0, "h_out and y_out must be two buffers")
-    for name, t, kinds, kind in (("post_gamma", post_gamma, ("layer", "rms"), post_norm),
-                                 ("post_beta", post_beta, ("layer",), post_norm),
-                                 ("pre_gamma", pre_gamma, ("layer", "rms"), pre_norm),
-                                 ("pre_beta", pre_beta, ("layer",), pre_norm)):
-        if kind in kinds:
-            _require(t is not None, f"{kind} norm needs {name}")
-            _check(t, name, (n,), dtype, device)
-    _check(bias, "bias", (n,), dtype, device)
-    gate_rows = 0
+    h_ptr, y_ptr = h_out.data_ptr(), _ptr(y_out)
+    _require(h_ptr != y_ptr or rows == 0, "h_out and y_out must be two buffers")
+    _check(residual, "residual", shape, dtype, device)
+    _check(h_out, "h_out", shape, dtype, device)
+    _check(y_out, "y_out", shape, dtype, device)
+    if post != 0:
+        _require(post_gamma is not None and (post != 1 or post_beta is not None), "post_norm needs its gamma (and beta)")
+        _check(post_gamma, "post_gamma", row, dtype, device)
+        if post == 1:
+            _check(post_beta, "post_beta", row, dtype, device)
+    if pre != 0:
+        _require(pre_gamma is not None and (pre != 1 or pre_beta is not None), "pre_norm needs its gamma (and beta)")
+        _check(pre_gamma, "pre_gamma", row, dtype, device)
+        if pre == 1:
+            _check(pre_beta, "pre_beta", row, dtype, device)
+    _check(bias, "bias", row, dtype, device)
+    gate_rows, idx = 0, None
     if gate is not None:
         gate_rows = 1 if gate.dim() == 1 else gate.shape[0]
-        _check(gate, "gate", (n,) if gate.dim() == 1 else (gate_rows, n), dtype, device)
+        _check(gate, "gate", row if gate.dim() == 1 else (gate_rows, n), dtype, device)
         _require(gate_rows >= 1, "gate must have a row")
-    if gate_rows > 1:
-        _require(isinstance(batch_idx, torch.Tensor) and batch_idx.dtype == torch.int32 and batch_idx.is_contiguous()
-                 and batch_idx.device == device and batch_idx.numel() >= rows,
-                 "a gate of several rows needs batch_idx, int32, one entry per row of x")
-    _check_count(valid_rows, device)
+        if gate_rows > 1:
+            _require(isinstance(batch_idx, torch.Tensor) and batch_idx.dtype is torch.int32
+                     and batch_idx.is_contiguous() and batch_idx.get_device() == device and batch_idx.numel() >= rows,
+                     "a gate of several rows needs batch_idx, int32, one entry per row of x")
+            idx = batch_idx.data_ptr()
     if mx_out is not None:
         _check_mx(mx_out, "mx_out", rows, n, device)
     p = _capi.GatedNormParam(
-        x.data_ptr(), _ptr(bias), _ptr(residual), _ptr(gate), _ptr(batch_idx) if gate_rows > 1 else None,
-        _ptr(post_gamma), _ptr(post_beta), _ptr(pre_gamma), _ptr(pre_beta), h_out.data_ptr(), _ptr(y_out),
-        None if mx_out is None else mx_out.data.data_ptr(), _ptr(valid_rows), None, rows, n, gate_rows,
-        _KIND[post_norm], _KIND[pre_norm], residual_scale, eps)
-    with _On(device) as stream:
-        p.stream = stream
-        _capi.check(_capi.load().et_gated_residual_norm(_DTYPE[dtype], C.byref(p)))
+        x.data_ptr(), _ptr(bias), _ptr(residual), _ptr(gate), idx, _ptr(post_gamma) if post != 0 else None,
+        _ptr(post_beta) if post == 1 else None, _ptr(pre_gamma) if pre != 0 else None,
+        _ptr(pre_beta) if pre == 1 else None, h_ptr, y_ptr, None if mx_out is None else mx_out.ptr,
+        _count(valid_rows, device), rows, n, gate_rows, post, pre, residual_scale, eps)
+    _call(device, "et_gated_residual_norm", _DTYPE[dtype], C.byref(p))
     return h_out, y_out

@@ -587,13 +587,13 @@ int et_gemm_fp32_tensor(const float* a_hi, const float* a_lo, const float* w_hi,
  * No reference counterpart.
  *
  * An MXFP4 tensor of `rows` rows of k values (k a multiple of 32) is an opaque
- * buffer of et_mxfp4_bytes(rows, k) bytes of device memory, 16-byte aligned
+ * buffer of et_mxfp4_bytes(rows, k) bytes of device memory, 128-byte aligned
  * (0 for shapes that are not served).  It holds rows in the form the tensor
  * core reads: tiles of 128 rows x 256 values with their scales.
  *
  * dtype is the element type of what is not MXFP4 (x, w, bias, residual, c, out);
  * m_ptr is a DEVICE pointer to the number of valid rows, NULL = all max_m; rows
- * past it are neither read nor written.  All pointers 16-byte aligned.  The text
+ * past it are neither read nor written.  All other pointers 16-byte aligned.  The text
  * of a refusal is et_last_error(NULL).  Calls that overlap on the GPU may share
  * what they only read. */
 size_t et_mxfp4_bytes(int rows, int k);
@@ -643,7 +643,6 @@ typedef struct {
   void* y_out;            /* [max_m, n] or NULL; may be x or residual, not h_out */
   void* y_mx;             /* MXFP4 tensor of max_m rows or NULL (n a multiple of 32) */
   const int* m_ptr;       /* device row count, NULL = max_m */
-  void* stream;
   int max_m;
   int n;                  /* a multiple of 16 bytes, at most 8192 (ET_FP16) or 4096 (ET_FP32) */
   int gate_rows;
@@ -652,7 +651,7 @@ typedef struct {
   float residual_scale;
   float eps;              /* <= 0 selects 1e-6 */
 } et_gated_norm_param_t;
-int et_gated_residual_norm(int dtype, const et_gated_norm_param_t* param);
+int et_gated_residual_norm(int dtype, const et_gated_norm_param_t* param, void* stream);
 
 #ifdef __cplusplus
 }

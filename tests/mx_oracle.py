@@ -42,13 +42,14 @@ def mx_unpack(data, rows, k):
     """(codes, scale bytes) read out of the buffer of an MXFP4 tensor, by the layout's formula."""
     tiles = data.reshape(-(-rows // 128), -(-k // 256), 17408)
     r, c = np.arange(rows)[:, None], np.arange(k)[None, :]
+    p = (r & ~0x1e) | ((r & 0x18) >> 2) | ((r & 0x06) << 2)     # where a row stands: bits 1-2 and 3-4 change places
     b = (c % 256) // 32
-    pos = (r % 128) * 128 + ((b ^ (r % 8)) * 16) + (c % 32) // 2
+    pos = (p % 128) * 128 + ((b ^ (p % 8)) * 16) + (c % 32) // 2
     byte = tiles[r // 128, c // 256, pos]
     codes = np.where(c % 2 == 0, byte & 15, byte >> 4).astype(np.uint8)
     cb = np.arange(k // 32)[None, :]
     bb = cb % 8
-    spos = 16384 + (bb // 4) * 512 + (r % 32) * 16 + ((r % 128) // 32) * 4 + bb % 4
+    spos = 16384 + (bb // 4) * 512 + (p % 32) * 16 + ((p % 128) // 32) * 4 + bb % 4
     return codes, tiles[r // 128, cb // 8, spos]
 
 

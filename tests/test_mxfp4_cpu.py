@@ -80,7 +80,7 @@ GEMM_BAD = [
     (dict(n=0), "n a"), (dict(m=-3), "negative"), (dict(epi=4), "epilogue"), (dict(epi=-1), "epilogue"),
     (dict(c=None), "exactly one"), (dict(c_mx=P), "exactly one"), (dict(c=None, c_mx=P, n=96), "multiple of 64"),
     (dict(c=None, c_mx=P, residual=P), "no residual"), (dict(a=None), "null"), (dict(w=None), "null"),
-    (dict(epi=2, bias=None), "null"), (dict(a=P + 8), "aligned"), (dict(w=P + 8), "aligned"), (dict(c=P + 2), "aligned"),
+    (dict(epi=2, bias=None), "null"), (dict(a=P + 8), "aligned"), (dict(w=P + 16), "aligned"), (dict(c=None, c_mx=P + 64), "aligned"), (dict(c=P + 2), "aligned"),
     (dict(bias=P + 2, epi=1), "aligned"), (dict(residual=P + 2), "aligned")]
 
 
@@ -107,7 +107,7 @@ NORM_BAD = [
     (dict(post_norm=1, post_gamma=P), "gamma"), (dict(post_norm=2), "gamma"), (dict(pre_norm=1), "gamma"),
     (dict(h_out=None), "at least one"), (dict(y_mx=P, n=48), "multiple of 32"), (dict(gate=P, gate_rows=0), "gate"),
     (dict(gate=P, gate_rows=2), "gate"), (dict(x=None), "null"), (dict(x=P + 8), "aligned"),
-    (dict(residual=P + 4), "aligned"), (dict(gate=P + 2, gate_rows=1), "aligned"), (dict(y_out=P + 2), "aligned")]
+    (dict(residual=P + 4), "aligned"), (dict(gate=P + 2, gate_rows=1), "aligned"), (dict(y_out=P + 2), "aligned"), (dict(y_mx=P + 16), "aligned")]
 
 
 @pytest.mark.parametrize("change,text", NORM_BAD)
@@ -116,15 +116,15 @@ def test_norm_refusals(change, text):
     p.x, p.h_out, p.max_m, p.n, p.residual_scale = P, P, 4, 64, 1.0
     for k, v in change.items():
         setattr(p, k, v)
-    refused(LIB.et_gated_residual_norm(1, C.byref(p)), text)
+    refused(LIB.et_gated_residual_norm(1, C.byref(p), None), text)
 
 
 def test_norm_refuses_types_and_null():
     p = _capi.GatedNormParam()
-    refused(LIB.et_gated_residual_norm(9, C.byref(p)), "dtype")
-    refused(LIB.et_gated_residual_norm(1, None), "null")
+    refused(LIB.et_gated_residual_norm(9, C.byref(p), None), "dtype")
+    refused(LIB.et_gated_residual_norm(1, None, None), "null")
     p.x, p.h_out, p.max_m, p.n = P, P, 4, 4100
-    refused(LIB.et_gated_residual_norm(0, C.byref(p)), "limited")
+    refused(LIB.et_gated_residual_norm(0, C.byref(p), None), "limited")
 
 
 def test_empty_batches_are_fine():
@@ -133,7 +133,7 @@ def test_empty_batches_are_fine():
     assert LIB.et_mxfp4_gemm(1, P, P, None, None, P, None, None, 0, 64, 64, 0, None, None) == 0
     p = _capi.GatedNormParam()
     p.h_out, p.n = P, 64
-    assert LIB.et_gated_residual_norm(1, C.byref(p)) == 0
+    assert LIB.et_gated_residual_norm(1, C.byref(p), None) == 0
 
 
 def test_python_refuses_before_any_launch():
@@ -147,3 +147,14 @@ def test_python_refuses_before_any_launch():
         with pytest.raises(ValueError):
             call()
     assert mxfp4.empty(129, 288, "cpu").data.numel() == X.mx_bytes(129, 288)
+
+
+def test_the_ring_of_the_products_is_drained():
+    """What tests/test_kernel_sources_cpu.py asks of the other rings: the producer waits for its stages once inside the
+    loop and once behind it, since commits arrive asynchronously; copies in flight land behind a wait that ran out."""
+    from test_kernel_sources_cpu import kernels, read
+    bodies = {k: b for k, _, b in kernels(read("gemm_mxfp4.cu"))}
+    assert len(bodies) == 2
+    for body in bodies.values():
+        assert body.count("mbar_wait(free_bar(") == 2
+        assert body.count("mbar_drain(full_bar(") == 1 and body.count("mbar_drain(drain_bar") == 1
