@@ -9,7 +9,7 @@
 //   warp 0    producer: operand tiles of 256 values of K, codes and scales, into a ring of kStages stages
 //   warp 1    MMA issuer: the stage's scales go to tensor memory (tcgen05.cp), then tcgen05.mma kind::mxf4 of K = 64,
 //             accumulating in one of two TMEM buffers
-//   the rest  epilogue: one TMEM lane quadrant and 64 of a buffer's columns each
+//   the rest  epilogue
 // gemm_mxfp4_kernel works on tiles of 128 x 128, gemm_mxfp4_pair_kernel on tiles of 256 x 192 by CTA pairs.
 // Scales have a TMEM region per stage, so a stage's are replaced only after the MMAs that read them have retired.
 #include "common.cuh"
@@ -23,8 +23,10 @@ namespace {
 using namespace ptx;
 
 constexpr int BM = 128;
-constexpr int kEpilogueWarps = 8;
-constexpr int kNumThreads = 64 + kEpilogueWarps * 32;
+// Epilogue warps: two sets of eight that take the tiles in turn, a set per accumulator buffer, so that one loads and
+// computes while the other stores; in a set, a TMEM lane quadrant and one half of the columns each.
+constexpr int kEpilogueSet = 8;
+constexpr int kNumThreads = 64 + 2 * kEpilogueSet * 32;
 constexpr int kUmmaK = 64;
 constexpr int kPairTiles = 512;  // from so many 128 x 128 tiles on, CTA pairs
 
@@ -147,137 +149,123 @@ __device__ __forceinline__ void store_oct(T* p, const float* f) {
   for (int i = 0; i < 8; i += VecTraits<T>::kElems) st_global_v4(p + i, VecTraits<T>::pack(f + i));
 }
 
-// The epilogue of one warp for a piece of 32 rows x 64 columns of a finished accumulator: row0, col0 its first row and
-// column, (TMEM lanes at the lane field of t_row).  prepare() runs before the accumulator is waited for, finish()
-// behind; release() in it once the warp's values are in registers.
+// A column group of 32 columns of a warp's 32 rows: what is fetched for it ahead, how it comes from tensor memory, and
+// what becomes of it.
 //
-// fp16 and fp32 results: a thread has, for each of 2 column groups of 32 and 4 row groups of 8, eight neighbouring
-// columns of one row (see mxfp4.cuh): bias and residual come in, and the result goes out, as 16 or 32 bytes a thread
-// and 64 or 128 contiguous bytes a row.
+// fp16 and fp32 results: a thread has, for each of 4 row groups of 8, eight neighbouring columns of one row (see
+// mxfp4.cuh): bias and residual come in, and the result goes out, as 16 or 32 bytes a thread and 64 or 128 contiguous
+// bytes a row.
 template <typename T, typename OUT, int ACT>
-struct Piece {
-  static constexpr int kParts = 2 / (sizeof(T) / 2);  // column groups whose residual is fetched ahead
-  Oct<T> bias[2];
-  Oct<T> res[kParts][4];
+struct Group {
+  Oct<T> bias, res[4];
 
   // Row of row group i (rows are lanes in the order of mx_row).
   static __device__ __forceinline__ int row_of(int i, int lane) { return mx_row(8 * i + (lane >> 2)); }
 
-  __device__ __forceinline__ void fetch(const MxArgs& g, int part, int slot, int row0, int col0, int M, int lane) {
-    const int col = col0 + part * 32 + (lane & 3) * 8;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int row = row0 + row_of(i, lane);
-      res[slot][i].zero();
-      if (row < M && col < g.n)
-        res[slot][i].load_activation(static_cast<const T*>(g.residual) + static_cast<size_t>(row) * g.n + col);
-    }
-  }
-  __device__ __forceinline__ void prepare(const MxArgs& g, const T* __restrict__ bias_ptr, int row0, int col0, int M,
-                                          int lane) {
-#pragma unroll
-    for (int c = 0; c < 2; ++c) {
-      const int col = col0 + c * 32 + (lane & 3) * 8;
-      bias[c].zero();
-      if (bias_ptr != nullptr && col < g.n) bias[c].load(bias_ptr + col);
-    }
+  __device__ __forceinline__ void fetch(const MxArgs& g, const T* __restrict__ bias_ptr, int row0, int col0, int M,
+                                        int lane) {
+    const int col = col0 + (lane & 3) * 8;
+    bias.zero();
+    if (bias_ptr != nullptr && col < g.n) bias.load(bias_ptr + col);
     if (g.residual != nullptr) {
-#pragma unroll
-      for (int c = 0; c < kParts; ++c) fetch(g, c, c, row0, col0, M, lane);
-    }
-  }
-  template <typename Release>
-  __device__ __forceinline__ void finish(const MxArgs& g, uint32_t t_row, int row0, int col0, int M, int lane,
-                                         Release release) {
-    uint32_t r[2][2][16];  // column group, upper or lower 16 lanes
-#pragma unroll
-    for (int c = 0; c < 2; ++c)
-#pragma unroll
-      for (int h = 0; h < 2; ++h) tmem_ld_16x256b_x4(t_row + (static_cast<uint32_t>(16 * h) << 16) + 32 * c, r[c][h]);
-    tmem_ld_wait();
-    tc_fence_before();
-    __syncwarp();
-    release();
-    T* base = static_cast<T*>(g.c) + static_cast<size_t>(row0) * g.n + col0 + (lane & 3) * 8;
-#pragma unroll
-    for (int c = 0; c < 2; ++c) {
-      if (c >= kParts && g.residual != nullptr) fetch(g, c, 0, row0, col0, M, lane);
-      const bool in = col0 + c * 32 < g.n;
+      const T* src = static_cast<const T*>(g.residual) + static_cast<size_t>(row0) * g.n + col;
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        float f[8];
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          f[2 * j] = __uint_as_float(r[c][i >> 1][4 * j + 2 * (i & 1)]);
-          f[2 * j + 1] = __uint_as_float(r[c][i >> 1][4 * j + 2 * (i & 1) + 1]);
-        }
-        bias[c].add_to(f);
-        activate<8, ACT, sizeof(T) == 2>(f);
-        if (g.residual != nullptr) res[c < kParts ? c : 0][i].add_to(f);
         const int row = row_of(i, lane);
-        if (in && row0 + row < M) store_oct<T>(base + static_cast<size_t>(row) * g.n + c * 32, f);
+        res[i].zero();
+        if (row0 + row < M && col < g.n) res[i].load_activation(src + static_cast<size_t>(row) * g.n);
       }
+    }
+  }
+  static __device__ __forceinline__ void load(uint32_t t_row, uint32_t* r) {
+    tmem_ld_16x256b_x4(t_row, r);
+    tmem_ld_16x256b_x4(t_row + (16u << 16), r + 16);
+  }
+  __device__ __forceinline__ void finish(const MxArgs& g, const uint32_t* r, int row0, int col0, int M, int lane) {
+    if (col0 >= g.n) return;  // (n is a multiple of 32)
+    T* dst = static_cast<T*>(g.c) + static_cast<size_t>(row0) * g.n + col0 + (lane & 3) * 8;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      float f[8];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        f[2 * j] = __uint_as_float(r[16 * (i >> 1) + 4 * j + 2 * (i & 1)]);
+        f[2 * j + 1] = __uint_as_float(r[16 * (i >> 1) + 4 * j + 2 * (i & 1) + 1]);
+      }
+      bias.add_to(f);
+      activate<8, ACT, sizeof(T) == 2>(f);
+      if (g.residual != nullptr) res[i].add_to(f);
+      const int row = row_of(i, lane);
+      if (row0 + row < M) store_oct<T>(dst + static_cast<size_t>(row) * g.n, f);
     }
   }
 };
 
-// MXFP4 results: a thread has the 64 columns of one row, two scale blocks, and needs no other's.
+// MXFP4 results: a thread has the 32 columns of one row, a scale block, and needs no other's.
 template <typename T, int ACT>
-struct Piece<T, MxOut, ACT> {
-  Oct<T> bias[8];  // of all 64 columns
+struct Group<T, MxOut, ACT> {
+  Oct<T> bias[4];
 
-  __device__ __forceinline__ void prepare(const MxArgs& g, const T* __restrict__ bias_ptr, int, int col0, int, int) {
+  __device__ __forceinline__ void fetch(const MxArgs& g, const T* __restrict__ bias_ptr, int, int col0, int, int) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
+    for (int i = 0; i < 4; ++i) {
       bias[i].zero();
-      if (bias_ptr != nullptr && col0 + 8 * i < g.n) bias[i].load(bias_ptr + col0 + 8 * i);
+      if (bias_ptr != nullptr && col0 < g.n) bias[i].load(bias_ptr + col0 + 8 * i);
     }
   }
-  template <typename Release>
-  __device__ __forceinline__ void finish(const MxArgs& g, uint32_t t_row, int row0, int col0, int M, int lane,
-                                         Release release) {
-    uint32_t r[64];
-    tmem_ld_32x32b_x32(t_row, r);
-    tmem_ld_32x32b_x32(t_row + 32, r + 32);
-    tmem_ld_wait();
-    tc_fence_before();
-    __syncwarp();
-    release();
+  static __device__ __forceinline__ void load(uint32_t t_row, uint32_t* r) { tmem_ld_32x32b_x32(t_row, r); }
+  __device__ __forceinline__ void finish(const MxArgs& g, const uint32_t* r, int row0, int col0, int M, int lane) {
     const int row = row0 + mx_row(lane);
-    if (row >= M || col0 >= g.n) return;  // (n is a multiple of 64)
-    uint8_t* tile = static_cast<uint8_t*>(g.c) + mx_tile_offset(row, col0 >> 8, mx_k_tiles(g.n));
-    const int rt = row & (kMxTileRows - 1), b0 = (col0 & 255) >> 5;
-    uint32_t scales = 0u;
-    Vec16 out[2];
+    if (row >= M || col0 >= g.n) return;
+    float f[32], top = 0.f;
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      float f[32];
+    for (int i = 0; i < 32; ++i) f[i] = __uint_as_float(r[mx_row(i)]);  // columns in their order
 #pragma unroll
-      for (int i = 0; i < 32; ++i) f[i] = __uint_as_float(r[h * 32 + mx_row(i)]);  // columns in their order
-      float top = 0.f;
+    for (int i = 0; i < 32; i += 8) {
+      bias[i / 8].add_to(f + i);
+      activate<8, ACT, true>(f + i);
 #pragma unroll
-      for (int i = 0; i < 32; i += 8) {
-        bias[h * 4 + i / 8].add_to(f + i);
-        activate<8, ACT, true>(f + i);
-#pragma unroll
-        for (int e = 0; e < 8; ++e) asm("max.NaN.f32 %0, %0, %1;" : "+f"(top) : "f"(fabsf(f[i + e])));
-      }
-      const MxScale s = mx_scale(abs_bits(top));
-      out[h].x = mx_codes8(f, s);
-      out[h].y = mx_codes8(f + 8, s);
-      out[h].z = mx_codes8(f + 16, s);
-      out[h].w = mx_codes8(f + 24, s);
-      scales |= s.byte << (8 * h);
+      for (int e = 0; e < 8; ++e) asm("max.NaN.f32 %0, %0, %1;" : "+f"(top) : "f"(fabsf(f[i + e])));
     }
-    // the two blocks are neighbours under the swizzle too, in either order: one 32-byte sector
-    const bool swap = (mx_row(rt) & 1) != 0;
-    const Vec16 lo = swap ? out[1] : out[0], hi = swap ? out[0] : out[1];
-    asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(tile + (mx_code_offset(rt, b0) & ~16)),
-                 "r"(lo.x), "r"(lo.y), "r"(lo.z), "r"(lo.w), "r"(hi.x), "r"(hi.y), "r"(hi.z), "r"(hi.w)
-                 : "memory");
-    *reinterpret_cast<uint16_t*>(tile + mx_scale_offset(rt, b0)) = static_cast<uint16_t>(scales);
+    const MxScale s = mx_scale(abs_bits(top));
+    uint8_t* tile = static_cast<uint8_t*>(g.c) + mx_tile_offset(row, col0 >> 8, mx_k_tiles(g.n));
+    const int rt = row & (kMxTileRows - 1), b = (col0 & 255) >> 5;
+    Vec16 v;
+    v.x = mx_codes8(f, s);
+    v.y = mx_codes8(f + 8, s);
+    v.z = mx_codes8(f + 16, s);
+    v.w = mx_codes8(f + 24, s);
+    st_global_v4(tile + mx_code_offset(rt, b), v);
+    tile[mx_scale_offset(rt, b)] = static_cast<uint8_t>(s.byte);
   }
 };
+
+// The epilogue of one warp: kGroups column groups of its 32 rows from (row0, col0) of a finished accumulator buffer
+// (TMEM lanes at the lane field of t_row).  wait() returns whether the accumulator has come; release() hands the buffer
+// back, when the last group is in registers.  What a group needs from global memory is on its way while its columns
+// come from tensor memory; the other warps of the scheduler (four in all) hide the rest.
+template <typename T, typename OUT, int ACT, int kGroups, typename Wait, typename Release>
+__device__ __forceinline__ bool epilogue_warp(const MxArgs& g, const T* __restrict__ bias_ptr, uint32_t t_row, int row0,
+                                              int col0, int M, int lane, Wait wait, Release release) {
+  Group<T, OUT, ACT> group;
+  group.fetch(g, bias_ptr, row0, col0, M, lane);
+  if (!wait()) return false;
+  tc_fence_after();
+#pragma unroll 1
+  for (int c = 0; c < kGroups; ++c) {
+    uint32_t r[32];
+    group.load(t_row + 32 * c, r);
+    if (c > 0) group.fetch(g, bias_ptr, row0, col0 + 32 * c, M, lane);
+    tmem_ld_wait();
+    if (c == kGroups - 1) {
+      tc_fence_before();
+      __syncwarp();
+      release();
+    }
+    group.finish(g, r, row0, col0 + 32 * c, M, lane);
+  }
+  return true;
+}
 
 // What one thread issues for a stage: the scales' copies and the MMAs of kSteps x 64 values of K.  The instruction
 // stream of that thread is what the tensor core waits for when it is longer than an MMA (64 cycles at N = 128), so it is
@@ -365,7 +353,7 @@ gemm_mxfp4_kernel(const MxArgs g, const T* __restrict__ bias) {
     }
     for (int a = 0; a < 2; ++a) {
       mbar_init(tmem_full_bar(a), 1);
-      mbar_init(tmem_empty_bar(a), kEpilogueWarps);
+      mbar_init(tmem_empty_bar(a), kEpilogueSet);
     }
     mbar_init(drain_bar, 1);
     *abort_flag = 0;
@@ -487,23 +475,21 @@ gemm_mxfp4_kernel(const MxArgs g, const T* __restrict__ bias) {
     }
     __syncwarp();
   } else {
-    const int quad = warp & 3, half = (warp - 2) >> 2;
-    int it = 0;
-    for (int tile = blockIdx.x; tile < num_tiles; tile += gridDim.x, ++it) {
+    const int quad = warp & 3, half = ((warp - 2) >> 2) & 1, acc = (warp - 2) / kEpilogueSet;
+    const uint32_t t_row = tmem_base + (static_cast<uint32_t>(quad * 32) << 16) + acc * BN + half * (BN / 2);
+    uint32_t phase = 0;
+    for (int tile = blockIdx.x + acc * gridDim.x; tile < num_tiles; tile += 2 * gridDim.x, phase ^= 1u) {
       const int m_tile = tile / n_tiles, n_tile = tile - m_tile * n_tiles;
-      const int acc = it & 1, row0 = m_tile * BM + quad * 32, col0 = n_tile * BN + half * 64;
-      Piece<T, OUT, ACT> piece;
-      piece.prepare(g, bias, row0, col0, M, lane);
-      const bool got = mbar_wait(tmem_full_bar(acc), (it >> 1) & 1, abort_flag);
-      if (!__all_sync(0xffffffffu, got)) {
+      const bool got = epilogue_warp<T, OUT, ACT, BN / 64>(
+          g, bias, t_row, m_tile * BM + quad * 32, n_tile * BN + half * (BN / 2), M, lane,
+          [&] { return __all_sync(0xffffffffu, mbar_wait(tmem_full_bar(acc), phase, abort_flag)) != 0; },
+          [&] {
+            if (lane == 0) mbar_arrive(tmem_empty_bar(acc));
+          });
+      if (!got) {
         if (lane == 0) fail(kSiteEpilogueFull);
         break;
       }
-      tc_fence_after();
-      piece.finish(g, tmem_base + (static_cast<uint32_t>(quad * 32) << 16) + acc * BN + half * 64, row0, col0, M, lane,
-                   [&] {
-                     if (lane == 0) mbar_arrive(tmem_empty_bar(acc));
-                   });
     }
   }
 
@@ -531,8 +517,6 @@ gemm_mxfp4_kernel(const MxArgs g, const T* __restrict__ bias) {
 // in the second case the MMAs read them from two columns (64 rows) further on.
 struct PairCfg {
   static constexpr int BN = 192;
-  static constexpr int kEpiWarps = 12;  // three per TMEM lane quadrant, 64 columns each
-  static constexpr int kThreads = 64 + kEpiWarps * 32;
   static constexpr int kStages = 5;
   static constexpr int kBCodes = BN / 2 * 128;
   static constexpr int kStageBytes = kMxTileBytes + kBCodes + 2 * kMxScaleBytes;
@@ -545,7 +529,7 @@ struct PairCfg {
 };
 
 template <typename T, typename OUT, int ACT>
-__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PairCfg::kThreads, 1)
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kNumThreads, 1)
 gemm_mxfp4_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant__ CUtensorMap tmap_w,
                        const __grid_constant__ CUtensorMap tmap_ws, const MxArgs g, const T* __restrict__ bias) {
   using cfg = PairCfg;
@@ -579,7 +563,7 @@ gemm_mxfp4_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_
     }
     for (int a = 0; a < 2; ++a) {
       mbar_init(tmem_full_bar(a), 1);
-      mbar_init(tmem_empty_bar(a), 2 * cfg::kEpiWarps);
+      mbar_init(tmem_empty_bar(a), 2 * kEpilogueSet);
     }
     mbar_init(drain_bar, 1);
     *abort_flag = 0;
@@ -735,23 +719,22 @@ gemm_mxfp4_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_
     }
   } else {
     // ------------------------- epilogue (both CTAs) -------------------------
-    const int quad = warp & 3, third = (warp - 2) >> 2;
-    int it = 0;
-    for (int tile = pair_id; tile < num_tiles; tile += num_pairs, ++it) {
-      const int m_tile = tile / n_tiles, n_tile = tile - m_tile * n_tiles, acc = it & 1;
-      const int col0 = n_tile * cfg::BN + third * 64, row0 = m_tile * 256 + static_cast<int>(rank) * BM + quad * 32;
-      Piece<T, OUT, ACT> piece;
-      piece.prepare(g, bias, row0, col0, M, lane);
-      const bool got = mbar_wait(tmem_full_bar(acc), (it >> 1) & 1, abort_flag);
-      if (!__all_sync(0xffffffffu, got)) {
+    const int quad = warp & 3, half = ((warp - 2) >> 2) & 1, acc = (warp - 2) / kEpilogueSet;
+    const uint32_t t_row = tmem_base + (static_cast<uint32_t>(quad * 32) << 16) + acc * cfg::BN + half * (cfg::BN / 2);
+    uint32_t phase = 0;
+    for (int tile = pair_id + acc * num_pairs; tile < num_tiles; tile += 2 * num_pairs, phase ^= 1u) {
+      const int m_tile = tile / n_tiles, n_tile = tile - m_tile * n_tiles;
+      const bool got = epilogue_warp<T, OUT, ACT, cfg::BN / 64>(
+          g, bias, t_row, m_tile * 256 + static_cast<int>(rank) * BM + quad * 32,
+          n_tile * cfg::BN + half * (cfg::BN / 2), M, lane,
+          [&] { return __all_sync(0xffffffffu, mbar_wait(tmem_full_bar(acc), phase, abort_flag)) != 0; },
+          [&] {
+            if (lane == 0) mbar_arrive_cluster(mapa_shared(tmem_empty_bar(acc), 0));
+          });
+      if (!got) {
         if (lane == 0) fail(kSiteEpilogueFull);
         break;
       }
-      tc_fence_after();
-      piece.finish(g, tmem_base + (static_cast<uint32_t>(quad * 32) << 16) + acc * cfg::BN + third * 64, row0, col0, M,
-                   lane, [&] {
-                     if (lane == 0) mbar_arrive_cluster(mapa_shared(tmem_empty_bar(acc), 0));
-                   });
     }
   }
 
@@ -794,7 +777,7 @@ cudaError_t launch_pair(const MxArgs& g, const T* bias, cudaStream_t stream) {
     return cudaErrorInvalidValue;
   const long long tiles = static_cast<long long>((g.max_m + 255) / 256) * ((g.n + cfg::BN - 1) / cfg::BN);
   const int pairs = static_cast<int>(tiles < sm_count() / 2 ? tiles : sm_count() / 2);
-  return launch_pdl(gemm_mxfp4_pair_kernel<T, OUT, ACT>, dim3(2 * pairs), dim3(cfg::kThreads), cfg::kSmemBytes, stream,
+  return launch_pdl(gemm_mxfp4_pair_kernel<T, OUT, ACT>, dim3(2 * pairs), dim3(kNumThreads), cfg::kSmemBytes, stream,
                     ta, tw, tws, g, bias);
 }
 
