@@ -14,6 +14,7 @@
 // Scales have a TMEM region per stage, so a stage's are replaced only after the MMAs that read them have retired.
 #include "common.cuh"
 #include "mxfp4.cuh"
+#include "packed_f32.cuh"
 #include "ptx_sm100.cuh"
 
 namespace etb {
@@ -53,44 +54,19 @@ struct MxArgs {
 // Rows as MXFP4 instead of T.
 struct MxOut {};
 
-// Two fp32 values in one 64-bit register: the packed fp32 instructions do two elements an issue slot.
-__device__ __forceinline__ uint64_t pack2(float a, float b) {
-  uint64_t r;
-  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
-  return r;
-}
-__device__ __forceinline__ void unpack2(uint64_t v, float& a, float& b) {
-  asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v));
-}
-__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
-  uint64_t r;
-  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-  return r;
-}
-__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
-  uint64_t r;
-  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-  return r;
-}
-__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
-  uint64_t r;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
-  return r;
-}
-
 // tanh-form GELU of a pair whose result is rounded to fp16 or to 4 bits: 0.5 x (1 + tanh u) with the hardware's
 // tanh (relative error 2^-11, so at most 0.5 |x| 2^-11 here, the size of the fp16 rounding behind it; in 4 bits a
 // sixteenth of half a step at the least).  One special-function operation an element where exp and a reciprocal
 // would be two: those alone take 36 us of a 39778 x 4096 result.
 __device__ __forceinline__ void gelu_pair(float& a, float& b) {
-  const uint64_t x = pack2(a, b);
-  const uint64_t c1 = pack2(0.7978845608028654f, 0.7978845608028654f);
-  const uint64_t c2 = pack2(0.7978845608028654f * 0.044715f, 0.7978845608028654f * 0.044715f);
+  const Pair x = pack2(a, b);
+  const Pair c1 = pack2(0.7978845608028654f, 0.7978845608028654f);
+  const Pair c2 = pack2(0.7978845608028654f * 0.044715f, 0.7978845608028654f * 0.044715f);
   float ua, ub;
   unpack2(mul2(x, fma2(mul2(x, x), c2, c1)), ua, ub);
   asm("tanh.approx.f32 %0, %0;" : "+f"(ua));
   asm("tanh.approx.f32 %0, %0;" : "+f"(ub));
-  const uint64_t h = mul2(x, pack2(0.5f, 0.5f));
+  const Pair h = mul2(x, pack2(0.5f, 0.5f));
   unpack2(fma2(h, pack2(ua, ub), h), a, b);
 }
 
@@ -122,13 +98,10 @@ struct Oct {
 #pragma unroll
     for (int i = 0; i < static_cast<int>(sizeof(T)) / 2; ++i) v[i] = Vec16{0u, 0u, 0u, 0u};
   }
-  __device__ __forceinline__ void load_activation(const T* p) {
-#pragma unroll
-    for (int i = 0; i < static_cast<int>(sizeof(T)) / 2; ++i) v[i] = ld_activation_v4(p + i * VecTraits<T>::kElems);
-  }
+  // (coherent loads for the bias too: a caller may have written it just before)
   __device__ __forceinline__ void load(const T* p) {
 #pragma unroll
-    for (int i = 0; i < static_cast<int>(sizeof(T)) / 2; ++i) v[i] = ld_global_v4(p + i * VecTraits<T>::kElems);
+    for (int i = 0; i < static_cast<int>(sizeof(T)) / 2; ++i) v[i] = ld_activation_v4(p + i * VecTraits<T>::kElems);
   }
   __device__ __forceinline__ void add_to(float* f) const {
 #pragma unroll
@@ -162,7 +135,7 @@ struct Group {
   // Row of row group i (rows are lanes in the order of mx_row).
   static __device__ __forceinline__ int row_of(int i, int lane) { return mx_row(8 * i + (lane >> 2)); }
 
-  __device__ __forceinline__ void fetch(const MxArgs& g, const T* __restrict__ bias_ptr, int row0, int col0, int M,
+  __device__ __forceinline__ void fetch(const MxArgs& g, const T* bias_ptr, int row0, int col0, int M,
                                         int lane) {
     const int col = col0 + (lane & 3) * 8;
     bias.zero();
@@ -173,7 +146,7 @@ struct Group {
       for (int i = 0; i < 4; ++i) {
         const int row = row_of(i, lane);
         res[i].zero();
-        if (row0 + row < M && col < g.n) res[i].load_activation(src + static_cast<size_t>(row) * g.n);
+        if (row0 + row < M && col < g.n) res[i].load(src + static_cast<size_t>(row) * g.n);
       }
     }
   }
@@ -206,7 +179,7 @@ template <typename T, int ACT>
 struct Group<T, MxOut, ACT> {
   Oct<T> bias[4];
 
-  __device__ __forceinline__ void fetch(const MxArgs& g, const T* __restrict__ bias_ptr, int, int col0, int, int) {
+  __device__ __forceinline__ void fetch(const MxArgs& g, const T* bias_ptr, int, int col0, int, int) {
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       bias[i].zero();
@@ -245,7 +218,7 @@ struct Group<T, MxOut, ACT> {
 // back, when the last group is in registers.  What a group needs from global memory is on its way while its columns
 // come from tensor memory; the other warps of the scheduler (four in all) hide the rest.
 template <typename T, typename OUT, int ACT, int kGroups, typename Wait, typename Release>
-__device__ __forceinline__ bool epilogue_warp(const MxArgs& g, const T* __restrict__ bias_ptr, uint32_t t_row, int row0,
+__device__ __forceinline__ bool epilogue_warp(const MxArgs& g, const T* bias_ptr, uint32_t t_row, int row0,
                                               int col0, int M, int lane, Wait wait, Release release) {
   Group<T, OUT, ACT> group;
   group.fetch(g, bias_ptr, row0, col0, M, lane);
@@ -322,7 +295,7 @@ struct Cfg {
 // T: element type of bias, residual and C; OUT: T, or MxOut.
 template <typename T, typename OUT, int ACT>
 __global__ void __launch_bounds__(kNumThreads, 1)
-gemm_mxfp4_kernel(const MxArgs g, const T* __restrict__ bias) {
+gemm_mxfp4_kernel(const MxArgs g, const T* bias) {
   constexpr int BN = 128;
   using cfg = Cfg<BN>;
   constexpr int S = cfg::kStages;
@@ -531,7 +504,7 @@ struct PairCfg {
 template <typename T, typename OUT, int ACT>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kNumThreads, 1)
 gemm_mxfp4_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant__ CUtensorMap tmap_w,
-                       const __grid_constant__ CUtensorMap tmap_ws, const MxArgs g, const T* __restrict__ bias) {
+                       const __grid_constant__ CUtensorMap tmap_ws, const MxArgs g, const T* bias) {
   using cfg = PairCfg;
   constexpr int S = cfg::kStages;
   pdl_trigger();

@@ -20,6 +20,8 @@
 #include <stddef.h>
 #include <stdint.h>
 
+#include "packed_f32.cuh"
+
 namespace etb {
 
 constexpr int kMxBlock = 32;
@@ -71,13 +73,9 @@ __device__ __forceinline__ float mx_scale_value(uint32_t byte) {
 // Eight values as codes, the first in the lowest nibble; round to nearest, ties to the even code, saturating at 6.
 __device__ __forceinline__ uint32_t mx_codes8(const float* x, const MxScale& s) {
   float f[8];
-  uint64_t inv;  // (two products an issue slot)
-  asm("mov.b64 %0, {%1, %1};" : "=l"(inv) : "f"(s.inverse));
+  const Pair inv = pack2(s.inverse, s.inverse);
 #pragma unroll
-  for (int i = 0; i < 8; i += 2)
-    asm("{\n\t.reg .b64 t;\n\tmov.b64 t, {%2, %3};\n\tmul.rn.f32x2 t, t, %4;\n\tmov.b64 {%0, %1}, t;\n\t}"
-        : "=f"(f[i]), "=f"(f[i + 1])
-        : "f"(x[i]), "f"(x[i + 1]), "l"(inv));
+  for (int i = 0; i < 8; i += 2) unpack2(mul2(pack2(x[i], x[i + 1]), inv), f[i], f[i + 1]);
   uint32_t w;
   asm("{\n\t.reg .b8 b0, b1, b2, b3;\n\t"
       "cvt.rn.satfinite.e2m1x2.f32 b0, %2, %1;\n\t"

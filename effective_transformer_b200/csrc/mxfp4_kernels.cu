@@ -9,34 +9,57 @@ namespace etb {
 namespace {
 
 constexpr int kThreads = 256;
-constexpr int kTasks = 4;  // (row, k-tile) pairs a warp has in flight
+constexpr int kTasks = 2;  // pieces of 512 values a warp has in flight
 
-// Eight consecutive values of a row, 16 or 32 bytes.
+// Sixteen consecutive values of a row: largest magnitude as fp32 bits, and the values.
 template <typename T>
-struct Oct;
+struct Sixteen;
 template <>
-struct Oct<__half> {
-  Vec16 v;
-  __device__ void load(const __half* p) { v = ld_activation_v4(p); }
-  __device__ void zero() { v = Vec16{0u, 0u, 0u, 0u}; }
-  __device__ void unpack(float* f) const { VecTraits<__half>::unpack(v, f); }
+struct Sixteen<__half> {
+  Vec16 v[2];
+  __device__ __forceinline__ void load(const __half* p) {
+    v[0] = ld_activation_v4(p);
+    v[1] = ld_activation_v4(p + 8);
+  }
+  // (the bits of non-negative fp16 numbers are in the order of the numbers, infinity and NaN on top)
+  __device__ __forceinline__ uint32_t top() const {
+    uint32_t m = v[0].x & 0x7fff7fffu;
+    const uint32_t w[7] = {v[0].y, v[0].z, v[0].w, v[1].x, v[1].y, v[1].z, v[1].w};
+#pragma unroll
+    for (int i = 0; i < 7; ++i) asm("max.u16x2 %0, %0, %1;" : "+r"(m) : "r"(w[i] & 0x7fff7fffu));
+    const uint32_t h = max(m & 0xffffu, m >> 16);
+    return __float_as_uint(__half2float(__ushort_as_half(static_cast<unsigned short>(h))));
+  }
+  __device__ __forceinline__ void unpack(float* f) const {
+    VecTraits<__half>::unpack(v[0], f);
+    VecTraits<__half>::unpack(v[1], f + 8);
+  }
 };
 template <>
-struct Oct<float> {
-  Vec16 a, b;
-  __device__ void load(const float* p) {
-    a = ld_activation_v4(p);
-    b = ld_activation_v4(p + 4);
+struct Sixteen<float> {
+  Vec16 v[4];
+  __device__ __forceinline__ void load(const float* p) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] = ld_activation_v4(p + 4 * i);
   }
-  __device__ void zero() { a = b = Vec16{0u, 0u, 0u, 0u}; }
-  __device__ void unpack(float* f) const {
-    VecTraits<float>::unpack(a, f);
-    VecTraits<float>::unpack(b, f + 4);
+  __device__ __forceinline__ uint32_t top() const {
+    uint32_t m = 0u;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const uint32_t w[4] = {v[i].x, v[i].y, v[i].z, v[i].w};
+#pragma unroll
+      for (int j = 0; j < 4; ++j) m = max(m, w[j] & 0x7fffffffu);
+    }
+    return m;
+  }
+  __device__ __forceinline__ void unpack(float* f) const {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) VecTraits<float>::unpack(v[i], f + 4 * i);
   }
 };
 
-// One warp per (row, k-tile): a lane holds eight values, four lanes a scale block, so that a warp reads 512 (fp16) or
-// 1024 contiguous bytes and writes one 128-byte line of codes.
+// A warp takes kTasks pieces of 512 values (two k-tiles of a row) at a time: a lane holds sixteen values, two lanes a
+// scale block.  (Pieces of 256, four lanes a block, cost twice the instructions for maxima, scales and addresses.)
 template <typename T>
 __global__ void __launch_bounds__(kThreads)
 mx_quantize_kernel(const T* x, long long row_stride, const int* m_ptr, int max_m, int k, uint8_t* mx) {
@@ -45,43 +68,51 @@ mx_quantize_kernel(const T* x, long long row_stride, const int* m_ptr, int max_m
   if (m_ptr != nullptr) rows = pdl_wait_row_count(m_ptr, max_m, 0);
   else pdl_wait();
   const int lane = threadIdx.x & 31;
-  const int k_tiles = mx_k_tiles(k);
-  const long long tasks = static_cast<long long>(rows) * k_tiles;
-  const long long warps = static_cast<long long>(gridDim.x) * (kThreads / 32);
-  const long long first = static_cast<long long>(blockIdx.x) * (kThreads / 32) + (threadIdx.x >> 5);
-  for (long long t0 = first * kTasks; t0 < tasks; t0 += warps * kTasks) {
-    Oct<T> v[kTasks];
-    int row[kTasks], kt[kTasks];
+  const uint32_t k_tiles = mx_k_tiles(k), pieces = (k_tiles + 1) / 2;
+  const uint32_t tasks = static_cast<uint32_t>(rows) * pieces;  // (2^32 of them would not fit any memory)
+  const uint32_t warps = gridDim.x * (kThreads / 32);
+  for (uint32_t t0 = (blockIdx.x * (kThreads / 32) + (threadIdx.x >> 5)) * kTasks; t0 < tasks; t0 += warps * kTasks) {
+    Sixteen<T> v[kTasks];
+    uint32_t row = t0 / pieces, piece = t0 - row * pieces;
+    uint32_t rows_of[kTasks], cols[kTasks];
+    bool in[kTasks], tile_in[kTasks];
 #pragma unroll
     for (int i = 0; i < kTasks; ++i) {
-      const long long t = t0 + i;
-      row[i] = t < tasks ? static_cast<int>(t / k_tiles) : -1;
-      kt[i] = static_cast<int>(t - t / k_tiles * k_tiles);
-      const int col = kt[i] * kMxTileK + lane * 8;
-      if (row[i] >= 0 && col < k) v[i].load(x + static_cast<size_t>(row[i]) * row_stride + col);
-      else v[i].zero();
+      cols[i] = piece * 512 + lane * 16;
+      rows_of[i] = row;
+      tile_in[i] = t0 + i < tasks && cols[i] < k_tiles * kMxTileK;  // (the row's last piece may be one k-tile)
+      in[i] = tile_in[i] && cols[i] < static_cast<uint32_t>(k);
+      if (in[i]) {
+        v[i].load(x + static_cast<size_t>(row) * row_stride + cols[i]);
+      } else {
+#pragma unroll
+        for (auto& w : v[i].v) w = Vec16{0u, 0u, 0u, 0u};
+      }
+      if (++piece == pieces) piece = 0, ++row;
     }
 #pragma unroll
     for (int i = 0; i < kTasks; ++i) {
-      float f[8];
-      v[i].unpack(f);
-      uint32_t top = 0u;
-#pragma unroll
-      for (int e = 0; e < 8; ++e) top = max(top, abs_bits(f[e]));
+      uint32_t top = v[i].top();
       top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
-      top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
       const MxScale s = mx_scale(top);
-      uint32_t scales = s.byte | (__shfl_down_sync(0xffffffffu, s.byte, 4) << 8);
-      scales |= __shfl_down_sync(0xffffffffu, scales, 8) << 16;  // four blocks' bytes in lanes 0 and 16
-      if (row[i] < 0) continue;
-      uint8_t* tile = mx + mx_tile_offset(row[i], kt[i], k_tiles);
-      const int r = row[i] & (kMxTileRows - 1);
-      *reinterpret_cast<uint32_t*>(tile + mx_code_offset(r, lane >> 2) + (lane & 3) * 4) = mx_codes8(f, s);
-      if ((lane & 15) == 0) *reinterpret_cast<uint32_t*>(tile + mx_scale_offset(r, lane >> 2)) = scales;
+      uint32_t scales = s.byte | (__shfl_down_sync(0xffffffffu, s.byte, 2) << 8);
+      scales |= __shfl_down_sync(0xffffffffu, scales, 4) << 16;  // four blocks' bytes in every eighth lane
+      if (!tile_in[i]) continue;
+      float f[16];
+      v[i].unpack(f);
+      uint8_t* tile = mx + mx_tile_offset(rows_of[i], cols[i] >> 8, k_tiles);
+      const int r = rows_of[i] & (kMxTileRows - 1), b = (cols[i] & 255) >> 5;
+      *reinterpret_cast<uint2*>(tile + mx_code_offset(r, b) + (lane & 1) * 8) =
+          make_uint2(mx_codes8(f, s), mx_codes8(f + 8, s));
+      if ((lane & 7) == 0) *reinterpret_cast<uint32_t*>(tile + mx_scale_offset(r, b)) = scales;
     }
   }
 }
 
+constexpr int kBackTasks = 4;  // (row, k-tile) pairs a warp has in flight
+
+// One warp per (row, k-tile): a lane holds eight values, so that a warp reads one 128-byte line of codes and writes 512
+// or 1024 contiguous bytes.
 template <typename T>
 __global__ void __launch_bounds__(kThreads)
 mx_dequantize_kernel(const uint8_t* mx, const int* m_ptr, int max_m, int k, T* out) {
@@ -90,31 +121,31 @@ mx_dequantize_kernel(const uint8_t* mx, const int* m_ptr, int max_m, int k, T* o
   if (m_ptr != nullptr) rows = pdl_wait_row_count(m_ptr, max_m, 0);
   else pdl_wait();
   const int lane = threadIdx.x & 31;
-  const int k_tiles = mx_k_tiles(k);
-  const long long tasks = static_cast<long long>(rows) * k_tiles;
-  const long long warps = static_cast<long long>(gridDim.x) * (kThreads / 32);
-  const long long first = static_cast<long long>(blockIdx.x) * (kThreads / 32) + (threadIdx.x >> 5);
-  for (long long t0 = first * kTasks; t0 < tasks; t0 += warps * kTasks) {
-    uint32_t code[kTasks], scale[kTasks];
-    int row[kTasks], col[kTasks];
+  const uint32_t k_tiles = mx_k_tiles(k);
+  const uint32_t tasks = static_cast<uint32_t>(rows) * k_tiles;
+  const uint32_t warps = gridDim.x * (kThreads / 32);
+  for (uint32_t t0 = (blockIdx.x * (kThreads / 32) + (threadIdx.x >> 5)) * kBackTasks; t0 < tasks;
+       t0 += warps * kBackTasks) {
+    uint32_t code[kBackTasks], scale[kBackTasks];
+    uint32_t row = t0 / k_tiles, kt = t0 - row * k_tiles;
+    T* dst[kBackTasks];
 #pragma unroll
-    for (int i = 0; i < kTasks; ++i) {
-      const long long t = t0 + i;
-      row[i] = t < tasks ? static_cast<int>(t / k_tiles) : -1;
-      const int kt = static_cast<int>(t - t / k_tiles * k_tiles);
-      col[i] = kt * kMxTileK + lane * 8;
-      if (col[i] >= k) row[i] = -1;
+    for (int i = 0; i < kBackTasks; ++i) {
+      const int col = kt * kMxTileK + lane * 8;
+      dst[i] = nullptr;
       code[i] = scale[i] = 0u;
-      if (row[i] >= 0) {
-        const uint8_t* tile = mx + mx_tile_offset(row[i], kt, k_tiles);
-        const int r = row[i] & (kMxTileRows - 1);
+      if (t0 + i < tasks && col < k) {
+        const uint8_t* tile = mx + mx_tile_offset(row, kt, k_tiles);
+        const int r = row & (kMxTileRows - 1);
         code[i] = *reinterpret_cast<const uint32_t*>(tile + mx_code_offset(r, lane >> 2) + (lane & 3) * 4);
         scale[i] = tile[mx_scale_offset(r, lane >> 2)];
+        dst[i] = out + static_cast<size_t>(row) * k + col;
       }
+      if (++kt == k_tiles) kt = 0, ++row;
     }
 #pragma unroll
-    for (int i = 0; i < kTasks; ++i) {
-      if (row[i] < 0) continue;
+    for (int i = 0; i < kBackTasks; ++i) {
+      if (dst[i] == nullptr) continue;
       const float s = mx_scale_value(scale[i]);
       float f[8];
 #pragma unroll
@@ -128,10 +159,8 @@ mx_dequantize_kernel(const uint8_t* mx, const int* m_ptr, int max_m, int k, T* o
         f[2 * j] = p.x * s;
         f[2 * j + 1] = p.y * s;
       }
-      T* dst = out + static_cast<size_t>(row[i]) * k + col[i];
 #pragma unroll
-      for (int e = 0; e < 8; e += VecTraits<T>::kElems)
-        st_global_v4(dst + e, VecTraits<T>::pack(f + e));
+      for (int e = 0; e < 8; e += VecTraits<T>::kElems) st_global_v4(dst[i] + e, VecTraits<T>::pack(f + e));
     }
   }
 }
@@ -164,8 +193,9 @@ mx_pack_weight_kernel(const T* w, uint8_t* mx, int k, int n) {
   tile[mx_scale_offset(r, b & 7)] = static_cast<uint8_t>(s.byte);
 }
 
-inline int mx_grid(long long rows, int k) {
-  const long long tasks = rows * mx_k_tiles(k), per_cta = static_cast<long long>(kThreads / 32) * kTasks;
+// CTAs for `tasks` warp tasks, `each` to a warp at a time, at most 8 per SM.
+inline int mx_grid(long long tasks, int each) {
+  const long long per_cta = static_cast<long long>(kThreads / 32) * each;
   long long ctas = (tasks + per_cta - 1) / per_cta;
   const long long cap = static_cast<long long>(sm_count()) * 8;
   if (ctas > cap) ctas = cap;
@@ -182,7 +212,8 @@ cudaError_t launch_mx_quantize(const T* x, long long row_stride, const int* m_pt
   if ((reinterpret_cast<uintptr_t>(x) & 15u) || (row_stride * sizeof(T)) % 16 != 0 ||
       (reinterpret_cast<uintptr_t>(mx) & 127u))
     return cudaErrorMisalignedAddress;
-  return launch_pdl(mx_quantize_kernel<T>, dim3(mx_grid(max_m, k)), dim3(kThreads), 0, stream, x, row_stride, m_ptr,
+  return launch_pdl(mx_quantize_kernel<T>,
+                    dim3(mx_grid(static_cast<long long>(max_m) * ((mx_k_tiles(k) + 1) / 2), kTasks)), dim3(kThreads), 0, stream, x, row_stride, m_ptr,
                     max_m, k, static_cast<uint8_t*>(mx));
 }
 
@@ -192,7 +223,7 @@ cudaError_t launch_mx_dequantize(const void* mx, const int* m_ptr, int max_m, in
   if (k <= 0 || k % kMxBlock != 0) return cudaErrorInvalidValue;
   if ((reinterpret_cast<uintptr_t>(out) & 15u) || (reinterpret_cast<uintptr_t>(mx) & 127u))
     return cudaErrorMisalignedAddress;
-  return launch_pdl(mx_dequantize_kernel<T>, dim3(mx_grid(max_m, k)), dim3(kThreads), 0, stream,
+  return launch_pdl(mx_dequantize_kernel<T>, dim3(mx_grid(static_cast<long long>(max_m) * mx_k_tiles(k), kBackTasks)), dim3(kThreads), 0, stream,
                     static_cast<const uint8_t*>(mx), m_ptr, max_m, k, out);
 }
 

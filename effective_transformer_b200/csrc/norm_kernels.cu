@@ -7,220 +7,354 @@
 // cuda/cuda_kernels.cu:157-236) is post = nothing, gate = 1, residual_scale = 1, y only.
 //
 // Everything between the loads of x and residual and the stores of h and y stays in fp32 registers, so x and residual
-// are read once and h and y written once: the kernel is bound by those bytes.  A row belongs to a group of WPR warps,
-// a lane holds up to kMaxVec vectors of 16 bytes of it; means and variances are taken in two passes over the
-// registers.  y can leave as MXFP4 too (mxfp4.cuh): four (fp16) or eight (fp32) neighbouring lanes hold a scale block.
+// are read once and h and y written once: the kernel is bound by those bytes once it spends few enough instructions.  A
+// group of warps (at most 16) takes R rows at a time; a lane holds V vectors of 16 bytes of each, 1 where the row allows
+// it.  So bias, gamma and beta stay in registers for all rows, and the R rows' sums go through their shuffles side by
+// side.  Means and variances are taken in two passes over the registers.  y can leave as MXFP4 too (mxfp4.cuh): four
+// (fp16) or eight (fp32) neighbouring lanes hold a scale block.
+//
+// 39778 rows of 1024 fp16 values with both norms and a gate, by layout: one row to a warp with the parameters read from
+// L1 for every row 118 us, from shared memory in fp32 88 us (128 registers, and what is fetched ahead spills), four
+// warps to one row 154 us, to two rows at a time 81 us, to four 82 us without and 96 us with fetching ahead.
 #include "common.cuh"
 #include "mxfp4.cuh"
+#include "packed_f32.cuh"
 
 namespace etb {
 
 namespace {
 
-constexpr int kThreads = 256;
-constexpr int kWarps = kThreads / 32;
-constexpr int kMaxVec = 4;
+constexpr int kMaxWarps = 16;  // of a row
+constexpr int kCtaWarps = 4;   // a CTA has as many whole groups as fit these, at least one
 
 enum NormKind : int { kNormNone = 0, kNormLayer = 1, kNormRms = 2 };
 
-// Sum over the WPR warps of a row group; every lane gets it.  `red`: WPR floats per group, double-buffered by `turn`.
-template <int WPR>
-__device__ __forceinline__ float group_sum(float v, float* red, int& turn, int group, int wig) {
-  v = warp_sum(v);
-  if (WPR == 1) return v;
-  float* slot = red + turn * kWarps + group * WPR;
-  turn ^= 1;
-  if ((threadIdx.x & 31) == 0) slot[wig] = v;
-  asm volatile("bar.sync %0, %1;" ::"r"(group + 1), "r"(WPR * 32) : "memory");
-  float t = 0.f;
+// A vector of 16 bytes as pairs of fp32 values (packed_f32.cuh).
+template <typename T>
+struct Pairs {
+  static constexpr int kCount = VecTraits<T>::kElems / 2;
+  static __device__ __forceinline__ void unpack(const Vec16& v, Pair* p) {
+    float f[2 * kCount];
+    VecTraits<T>::unpack(v, f);
 #pragma unroll
-  for (int i = 0; i < WPR; ++i) t += slot[i];
-  return t;
+    for (int i = 0; i < kCount; ++i) p[i] = pack2(f[2 * i], f[2 * i + 1]);
+  }
+  static __device__ __forceinline__ Vec16 pack(const Pair* p) {
+    float f[2 * kCount];
+#pragma unroll
+    for (int i = 0; i < kCount; ++i) unpack2(p[i], f[2 * i], f[2 * i + 1]);
+    return VecTraits<T>::pack(f);
+  }
+};
+__device__ __forceinline__ Pair both(float x) { return pack2(x, x); }
+
+// One vector a lane of an MXFP4 row: c is the lane's vector, whose first column in the warp is that of lane 0.
+template <typename T>
+__device__ __forceinline__ void store_mx(const Pair* v, void* y_mx, int row, int c, int n, int lane) {
+  constexpr int E = VecTraits<T>::kElems;
+  constexpr int kLanes = kMxBlock / E;  // lanes of a scale block
+  const int col = c * E;
+  if ((c - lane) * E >= n) return;  // (uniform for the warp)
+  float f[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+  uint32_t top = 0u;
+  if (col < n) {  // (zeros behind the row's end)
+#pragma unroll
+    for (int i = 0; i < E / 2; ++i) unpack2(v[i], f[2 * i], f[2 * i + 1]);
+  }
+#pragma unroll
+  for (int e = 0; e < E; ++e) top = max(top, abs_bits(f[e]));
+#pragma unroll
+  for (int o = 1; o < kLanes; o <<= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
+  const MxScale s = mx_scale(top);
+  uint32_t scales = s.byte | (__shfl_down_sync(0xffffffffu, s.byte, kLanes) << 8);
+  scales |= __shfl_down_sync(0xffffffffu, scales, 2 * kLanes) << 16;
+  const int r = row & (kMxTileRows - 1), b = (col & 255) >> 5;
+  uint8_t* tile = static_cast<uint8_t*>(y_mx) + mx_tile_offset(row, col >> 8, mx_k_tiles(n));
+  const uint32_t code = mx_codes8(f, s);
+  uint8_t* dst = tile + mx_code_offset(r, b) + (lane & (kLanes - 1)) * (E / 2);
+  if (E == 8) *reinterpret_cast<uint32_t*>(dst) = code;
+  else *reinterpret_cast<uint16_t*>(dst) = static_cast<uint16_t>(code);
+  if ((lane & (4 * kLanes - 1)) == 0) *reinterpret_cast<uint32_t*>(tile + mx_scale_offset(r, b)) = scales;
 }
 
-// v := norm(v) over the row; elements past the row's end are zero before and are not read behind.
-template <typename T, int V, int WPR>
-__device__ __forceinline__ void normalise(float (&v)[V][VecTraits<T>::kElems], int kind, const T* gamma, const T* beta,
-                                          int n, float eps, int vec0, int vecs, float* red, int& turn, int group,
-                                          int wig) {
-  constexpr int E = VecTraits<T>::kElems;
-  const float inv_n = 1.0f / static_cast<float>(n);
-  float mean = 0.f;
+// Where a lane stands: its group, the group's warps, the lane's first vector of a row.
+struct Place {
+  int group, wpr, wig, lane, vec0, vecs, turn;
+  float* red;  // [2][kMaxWarps][R] of the group, used in turn
+};
+
+// Sums of R values over the lanes of a group, to every lane: in a warp the R rows' shuffles are merged (a lane passes on
+// what its half of the warp is not to keep), between warps through shared memory.
+template <int R>
+__device__ __forceinline__ void group_sum(float (&v)[R], Place& p) {
+  int o = 16, row = 0;
+#pragma unroll
+  for (int h = R / 2; h >= 1; h >>= 1, o >>= 1) {
+    const bool upper = (p.lane & o) != 0;
+    row = 2 * row + (upper ? 1 : 0);
+#pragma unroll
+    for (int j = 0; j < h; ++j) {
+      const float send = upper ? v[j] : v[j + h], keep = upper ? v[j + h] : v[j];
+      v[j] = keep + __shfl_xor_sync(0xffffffffu, send, o);
+    }
+  }
+  // row: the index of v that a lane ends with, most significant halving first
+  const int lanes = o * 2;  // lanes that share it
+#pragma unroll
+  for (; o >= 1; o >>= 1) v[0] += __shfl_xor_sync(0xffffffffu, v[0], o);
+  float* slot = p.red + p.turn * kMaxWarps * R;
+  p.turn ^= 1;
+  if ((p.lane & (lanes - 1)) == 0) slot[p.wig * R + row] = v[0];
+  if (p.wpr == 1) __syncwarp();
+  else asm volatile("bar.sync %0, %1;" ::"r"(p.group + 1), "r"(p.wpr * 32) : "memory");
+  // (slots of warps that the group does not have are zero)
+#pragma unroll
+  for (int r = 0; r < R; ++r) v[r] = slot[r];
+#pragma unroll
+  for (int i = 1; i < 4; ++i)
+#pragma unroll
+    for (int r = 0; r < R; ++r) v[r] += slot[i * R + r];
+  for (int i = 4; i < p.wpr; ++i)
+#pragma unroll
+    for (int r = 0; r < R; ++r) v[r] += slot[i * R + r];
+}
+
+// v := norm(v) of R rows; elements past the row's end are zero before and behind.  kFull: no lane has such elements.
+template <typename T, int V, int R, bool kFull>
+__device__ __forceinline__ void normalise(Pair (&v)[R][V][Pairs<T>::kCount], int kind, const Vec16 (&gamma)[V],
+                                          const Vec16 (&beta)[V], float inv_n, float eps, Place& p) {
+  constexpr int P = Pairs<T>::kCount;
+  float s[R];
   if (kind == kNormLayer) {
-    float s = 0.f;
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      Pair a = v[r][0][0];
+#pragma unroll
+      for (int j = 0; j < V; ++j)
+#pragma unroll
+        for (int i = 0; i < P; ++i)
+          if (i + j > 0) a = add2(a, v[r][j][i]);
+      s[r] = a.x + a.y;
+    }
+    group_sum<R>(s, p);
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+      const float inside = kFull || p.vec0 + j * 32 * p.wpr < p.vecs ? -inv_n : 0.f;
+#pragma unroll
+      for (int r = 0; r < R; ++r)
+#pragma unroll
+        for (int i = 0; i < P; ++i) v[r][j][i] = add2(v[r][j][i], both(s[r] * inside));
+    }
+  }
+#pragma unroll
+  for (int r = 0; r < R; ++r) {
+    Pair a = mul2(v[r][0][0], v[r][0][0]);
 #pragma unroll
     for (int j = 0; j < V; ++j)
 #pragma unroll
-      for (int e = 0; e < E; ++e) s += v[j][e];
-    mean = group_sum<WPR>(s, red, turn, group, wig) * inv_n;
+      for (int i = 0; i < P; ++i)
+        if (i + j > 0) a = fma2(v[r][j][i], v[r][j][i], a);
+    s[r] = a.x + a.y;
   }
-  float sq = 0.f;
+  group_sum<R>(s, p);
+#pragma unroll
+  for (int r = 0; r < R; ++r) s[r] = rsqrtf(fmaf(s[r], inv_n, eps));
 #pragma unroll
   for (int j = 0; j < V; ++j) {
-    if (vec0 + j * 32 * WPR < vecs) {
+    Pair g[P], b[P];
+    Pairs<T>::unpack(gamma[j], g);
+    Pairs<T>::unpack(beta[j], b);  // (zeros for an RMS norm)
 #pragma unroll
-      for (int e = 0; e < E; ++e) {
-        v[j][e] -= mean;
-        sq = fmaf(v[j][e], v[j][e], sq);
-      }
-    }
-  }
-  const float rstd = rsqrtf(group_sum<WPR>(sq, red, turn, group, wig) * inv_n + eps);
+    for (int r = 0; r < R; ++r)
 #pragma unroll
-  for (int j = 0; j < V; ++j) {
-    const int c = vec0 + j * 32 * WPR;
-    if (c < vecs) {
-      float g[E], b[E];
-      VecTraits<T>::unpack(ld_global_v4(gamma + c * E), g);
-      if (kind == kNormLayer) VecTraits<T>::unpack(ld_global_v4(beta + c * E), b);
-#pragma unroll
-      for (int e = 0; e < E; ++e)
-        v[j][e] = kind == kNormLayer ? fmaf(v[j][e] * rstd, g[e], b[e]) : v[j][e] * rstd * g[e];
-    }
+      for (int i = 0; i < P; ++i) v[r][j][i] = fma2(mul2(v[r][j][i], both(s[r])), g[i], b[i]);
   }
 }
 
-template <typename T, int V, int WPR>
-__global__ void __launch_bounds__(kThreads)
-gated_norm_kernel(const GatedNorm p) {
-  constexpr int E = VecTraits<T>::kElems;
-  constexpr int kGroups = kWarps / WPR;
-  __shared__ float red[2 * kWarps];
+// 128 for a CTA of 512 threads; fewer where that brings a second CTA of a wide fp32 row's nine warps to the SM.
+__host__ __device__ constexpr int max_registers(size_t elem, int v) { return elem == 4 && v == 2 ? 96 : 128; }
+
+template <typename T, int V, int R, bool kFull>
+__global__ void __maxnreg__(max_registers(sizeof(T), V))
+gated_norm_kernel(const GatedNorm p, int wpr) {
+  constexpr int E = VecTraits<T>::kElems, P = E / 2;
+  __shared__ float red[kCtaWarps][2 * kMaxWarps * R];
   pdl_trigger();
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int groups = static_cast<int>(blockDim.x >> 5) / wpr;
+  for (int i = threadIdx.x; i < kCtaWarps * 2 * kMaxWarps * R; i += blockDim.x) (&red[0][0])[i] = 0.f;
+  __syncthreads();
+  Place at;
+  at.group = warp / wpr;
+  at.wpr = wpr;
+  at.wig = warp - at.group * wpr;
+  at.lane = lane;
+  at.vec0 = at.wig * 32 + lane;
+  at.vecs = p.n / E;
+  at.turn = 0;
+  at.red = red[at.group];
+  const int n = p.n;
   int rows = p.max_m;
   if (p.m_ptr != nullptr) rows = pdl_wait_row_count(p.m_ptr, p.max_m, 0);
   else pdl_wait();
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int group = warp / WPR, wig = warp % WPR;
-  const int n = p.n, vecs = n / E;
-  const int vec0 = wig * 32 + lane;
-  const T* x = static_cast<const T*>(p.x);
-  const T* bias = static_cast<const T*>(p.bias);
-  const T* residual = static_cast<const T*>(p.residual);
-  const T* gate = static_cast<const T*>(p.gate);
-  int turn = 0;
-  for (long long row = static_cast<long long>(blockIdx.x) * kGroups + group; row < rows;
-       row += static_cast<long long>(gridDim.x) * kGroups) {
-    const size_t base = static_cast<size_t>(row) * n;
-    float v[V][E];
-    Vec16 vx[V], vr[V];
+  auto inside = [&](int j) { return kFull || at.vec0 + j * 32 * wpr < at.vecs; };
+  // (a caller may have written the parameters just before: they come behind the wait too)
+  Vec16 bias[V], pog[V], pob[V], prg[V], prb[V];
+  auto param = [&](const void* src, bool used, Vec16(&dst)[V]) {
 #pragma unroll
     for (int j = 0; j < V; ++j) {
-      const int c = vec0 + j * 32 * WPR;
-      vx[j] = vr[j] = Vec16{0u, 0u, 0u, 0u};
-      if (c < vecs) {
-        vx[j] = ld_activation_v4(x + base + c * E);
-        if (residual != nullptr) vr[j] = ld_activation_v4(residual + base + c * E);
+      dst[j] = Vec16{0u, 0u, 0u, 0u};
+      if (used && inside(j)) dst[j] = ld_global_v4(static_cast<const T*>(src) + (at.vec0 + j * 32 * wpr) * E);
+    }
+  };
+  const int post_kind = p.post_kind, pre_kind = p.pre_kind, gate_rows = p.gate_rows;
+  param(p.bias, p.bias != nullptr, bias);
+  param(p.post_gamma, post_kind != kNormNone, pog);
+  param(p.post_beta, post_kind == kNormLayer, pob);
+  param(p.pre_gamma, pre_kind != kNormNone, prg);
+  param(p.pre_beta, pre_kind == kNormLayer, prb);
+  const float inv_n = 1.0f / static_cast<float>(n), eps = p.eps;
+  const Pair scale = both(p.residual_scale);
+
+  const long long stride = static_cast<long long>(gridDim.x) * groups * R;
+  long long row0 = (static_cast<long long>(blockIdx.x) * groups + at.group) * R;
+  // This lane's first vector of the first row in work, in bytes, and what lies between rows, vectors and rounds.
+  const size_t pitch = static_cast<size_t>(n) * sizeof(T), lead = static_cast<size_t>(at.vec0) * 16;
+  const size_t advance = static_cast<size_t>(stride) * pitch;
+  const int vec_bytes = 512 * wpr;
+  size_t off = static_cast<size_t>(row0) * pitch + lead;
+  const char* const gate = p.gate != nullptr ? static_cast<const char*>(p.gate) + lead : nullptr;
+  // The next round's vectors are fetched as soon as this round's have been unpacked, into the same registers; the gate
+  // rows, through which the gate is found, a round before that.
+  Vec16 vx[R][V], vr[R][V], vg[R][V];
+  int gate_row[R], gate_next[R];
+  auto fetch = [&](const void* base, size_t at_off, long long from, Vec16(&dst)[R][V]) {
+    const char* src = static_cast<const char*>(base) + at_off;
+#pragma unroll
+    for (int r = 0; r < R; ++r)
+#pragma unroll
+      for (int j = 0; j < V; ++j)
+        if (inside(j) && from + r < rows) dst[r][j] = ld_activation_v4(src + r * pitch + j * vec_bytes);
+  };
+  auto fetch_gate_rows = [&](long long from) {
+#pragma unroll
+    for (int r = 0; r < R; ++r) gate_next[r] = p.batch_idx != nullptr && from + r < rows ? p.batch_idx[from + r] : 0;
+  };
+  auto fetch_gate = [&](long long from) {  // and the gate rows of the round behind
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      gate_row[r] = gate_next[r];
+      if (gate_row[r] >= 0 && gate_row[r] < gate_rows) {
+        const char* src = gate + static_cast<size_t>(gate_row[r]) * pitch;
+#pragma unroll
+        for (int j = 0; j < V; ++j)
+          if (inside(j)) vg[r][j] = ld_activation_v4(src + j * vec_bytes);
       }
     }
+    fetch_gate_rows(from + stride);
+  };
+#pragma unroll
+  for (int r = 0; r < R; ++r)
+#pragma unroll
+    for (int j = 0; j < V; ++j) vx[r][j] = vr[r][j] = vg[r][j] = Vec16{0u, 0u, 0u, 0u};  // (zeros behind the row's end)
+  fetch(p.x, off, row0, vx);
+  if (p.residual != nullptr) fetch(p.residual, off, row0, vr);
+  if (gate != nullptr) {
+    fetch_gate_rows(row0);
+    fetch_gate(row0);
+  }
+  for (; row0 < rows; row0 += stride, off += advance) {
+    Pair v[R][V][P];
 #pragma unroll
     for (int j = 0; j < V; ++j) {
-      const int c = vec0 + j * 32 * WPR;
-      VecTraits<T>::unpack(vx[j], v[j]);
-      if (bias != nullptr && c < vecs) {
-        float b[E];
-        VecTraits<T>::unpack(ld_global_v4(bias + c * E), b);
+      Pair b[P];
+      Pairs<T>::unpack(bias[j], b);
 #pragma unroll
-        for (int e = 0; e < E; ++e) v[j][e] += b[e];
+      for (int r = 0; r < R; ++r) {
+        Pairs<T>::unpack(vx[r][j], v[r][j]);
+#pragma unroll
+        for (int i = 0; i < P; ++i) v[r][j][i] = add2(v[r][j][i], b[i]);
       }
     }
-    if (p.post_kind != kNormNone)
-      normalise<T, V, WPR>(v, p.post_kind, static_cast<const T*>(p.post_gamma), static_cast<const T*>(p.post_beta), n,
-                           p.eps, vec0, vecs, red, turn, group, wig);
-    // a sequence number outside the gate's rows opens no gate: its row is zero
-    const int gate_row = gate != nullptr && p.batch_idx != nullptr ? p.batch_idx[row] : 0;
-    const bool gate_in = gate_row >= 0 && gate_row < p.gate_rows;
+    fetch(p.x, off + advance, row0 + stride, vx);
+    if (post_kind != kNormNone) normalise<T, V, R, kFull>(v, post_kind, pog, pob, inv_n, eps, at);
+    if (gate != nullptr) {
 #pragma unroll
-    for (int j = 0; j < V; ++j) {
-      const int c = vec0 + j * 32 * WPR;
-      if (gate != nullptr) {
-        float g[E];
-        Vec16 vg = {0u, 0u, 0u, 0u};
-        if (gate_in && c < vecs) vg = ld_activation_v4(gate + static_cast<size_t>(gate_row) * n + c * E);
-        VecTraits<T>::unpack(vg, g);
+      for (int r = 0; r < R; ++r) {
+        if (gate_row[r] >= 0 && gate_row[r] < gate_rows) {
 #pragma unroll
-        for (int e = 0; e < E; ++e) v[j][e] = gate_in ? v[j][e] * g[e] : 0.f;
-      }
-      if (residual != nullptr) {
-        float r[E];
-        VecTraits<T>::unpack(vr[j], r);
+          for (int j = 0; j < V; ++j) {
+            Pair g[P];
+            Pairs<T>::unpack(vg[r][j], g);
 #pragma unroll
-        for (int e = 0; e < E; ++e) v[j][e] = fmaf(r[e], p.residual_scale, v[j][e]);
-      }
-      if (p.h != nullptr && c < vecs) st_global_v4(static_cast<T*>(p.h) + base + c * E, VecTraits<T>::pack(v[j]));
-    }
-    if (p.pre_kind != kNormNone)
-      normalise<T, V, WPR>(v, p.pre_kind, static_cast<const T*>(p.pre_gamma), static_cast<const T*>(p.pre_beta), n,
-                           p.eps, vec0, vecs, red, turn, group, wig);
-    if (p.y != nullptr) {
+            for (int i = 0; i < P; ++i) v[r][j][i] = mul2(v[r][j][i], g[i]);
+          }
+        } else {  // a sequence number outside the gate's rows opens no gate
 #pragma unroll
-      for (int j = 0; j < V; ++j) {
-        const int c = vec0 + j * 32 * WPR;
-        if (c < vecs) st_global_v4(static_cast<T*>(p.y) + base + c * E, VecTraits<T>::pack(v[j]));
-      }
-    }
-    if (p.y_mx != nullptr) {
-      constexpr int kLanes = kMxBlock / E;     // lanes of a scale block
-      constexpr int kBlocks = 32 / kLanes;     // blocks a warp holds per vector
-      uint8_t* mx = static_cast<uint8_t*>(p.y_mx);
-      const int k_tiles = mx_k_tiles(n), r = static_cast<int>(row) & (kMxTileRows - 1);
+          for (int j = 0; j < V; ++j)
 #pragma unroll
-      for (int j = 0; j < V; ++j) {
-        const int c = vec0 + j * 32 * WPR, col = c * E;
-        // (whole warps: the first column of a warp's vector decides)
-        if ((c - lane) * E >= n) continue;
-        float f[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-        uint32_t top = 0u;
-#pragma unroll
-        for (int e = 0; e < E; ++e) {
-          f[e] = c < vecs ? v[j][e] : 0.f;
-          top = max(top, abs_bits(f[e]));
+            for (int i = 0; i < P; ++i) v[r][j][i] = both(0.f);
         }
-#pragma unroll
-        for (int o = 1; o < kLanes; o <<= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
-        const MxScale s = mx_scale(top);
-        uint32_t scales = s.byte | (__shfl_down_sync(0xffffffffu, s.byte, kLanes) << 8);
-        scales |= __shfl_down_sync(0xffffffffu, scales, 2 * kLanes) << 16;
-        uint8_t* tile = mx + mx_tile_offset(static_cast<int>(row), col >> 8, k_tiles);
-        const int b = (col & 255) >> 5;
-        const uint32_t code = mx_codes8(f, s);
-        uint8_t* dst = tile + mx_code_offset(r, b) + (lane & (kLanes - 1)) * (E / 2);
-        if (E == 8) *reinterpret_cast<uint32_t*>(dst) = code;
-        else *reinterpret_cast<uint16_t*>(dst) = static_cast<uint16_t>(code);
-        if ((lane & (4 * kLanes - 1)) == 0) *reinterpret_cast<uint32_t*>(tile + mx_scale_offset(r, b)) = scales;
-        (void)kBlocks;
       }
+      fetch_gate(row0 + stride);
+    }
+    if (p.residual != nullptr) {
+#pragma unroll
+      for (int r = 0; r < R; ++r)
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+          Pair res[P];
+          Pairs<T>::unpack(vr[r][j], res);
+#pragma unroll
+          for (int i = 0; i < P; ++i) v[r][j][i] = fma2(res[i], scale, v[r][j][i]);
+        }
+      fetch(p.residual, off + advance, row0 + stride, vr);
+    }
+    auto store = [&](void* base) {
+      char* to = static_cast<char*>(base) + off;
+#pragma unroll
+      for (int r = 0; r < R; ++r)
+#pragma unroll
+        for (int j = 0; j < V; ++j)
+          if (inside(j) && row0 + r < rows) st_global_v4(to + r * pitch + j * vec_bytes, Pairs<T>::pack(v[r][j]));
+    };
+    if (p.h != nullptr) store(p.h);
+    if (pre_kind != kNormNone) normalise<T, V, R, kFull>(v, pre_kind, prg, prb, inv_n, eps, at);
+    if (p.y != nullptr) store(p.y);
+    if (p.y_mx != nullptr) {
+#pragma unroll
+      for (int r = 0; r < R; ++r)
+#pragma unroll
+        for (int j = 0; j < V; ++j)
+          if (row0 + r < rows)
+            store_mx<T>(v[r][j], p.y_mx, static_cast<int>(row0) + r, at.vec0 + j * 32 * wpr, n, lane);
     }
   }
 }
 
-template <typename T, int V, int WPR>
-cudaError_t launch_one(const GatedNorm& p, cudaStream_t stream) {
-  auto kernel = gated_norm_kernel<T, V, WPR>;
-  static std::atomic<int> resident[kMaxDevices] = {};
+template <typename T, int V, int R, bool kFull>
+cudaError_t launch_full(const GatedNorm& p, int wpr, cudaStream_t stream) {
+  auto kernel = gated_norm_kernel<T, V, R, kFull>;
+  const int groups = wpr >= kCtaWarps ? 1 : kCtaWarps / wpr, threads = groups * wpr * 32;
+  static std::atomic<int> resident[kMaxDevices][kMaxWarps + 1] = {};
   const int dev = current_device();
-  int per_sm = dev >= 0 ? resident[dev].load(std::memory_order_relaxed) : 0;
+  int per_sm = dev >= 0 ? resident[dev][wpr].load(std::memory_order_relaxed) : 0;
   if (per_sm == 0) {
-    if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, kernel, kThreads, 0) != cudaSuccess || per_sm < 1)
+    if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, kernel, threads, 0) != cudaSuccess || per_sm < 1)
       per_sm = 1;
-    if (dev >= 0) resident[dev].store(per_sm, std::memory_order_relaxed);
+    if (dev >= 0) resident[dev][wpr].store(per_sm, std::memory_order_relaxed);
   }
-  constexpr int kGroups = kWarps / WPR;
-  long long ctas = (static_cast<long long>(p.max_m) + kGroups - 1) / kGroups;
+  const long long rows_per_cta = static_cast<long long>(groups) * R;
+  long long ctas = (p.max_m + rows_per_cta - 1) / rows_per_cta;
   const long long cap = static_cast<long long>(sm_count()) * per_sm;
   if (ctas > cap) ctas = cap;
-  return launch_pdl(kernel, dim3(static_cast<int>(ctas)), dim3(kThreads), 0, stream, p);
+  return launch_pdl(kernel, dim3(static_cast<int>(ctas)), dim3(threads), 0, stream, p, wpr);
 }
 
-template <typename T, int WPR>
-cudaError_t launch_wpr(const GatedNorm& p, int v, cudaStream_t stream) {
-  switch (v) {
-    case 1: return launch_one<T, 1, WPR>(p, stream);
-    case 2: return launch_one<T, 2, WPR>(p, stream);
-    case 3: return launch_one<T, 3, WPR>(p, stream);
-    case 4: return launch_one<T, 4, WPR>(p, stream);
-    default: return cudaErrorInvalidValue;
-  }
+template <typename T, int V, int R>
+cudaError_t launch_rows(const GatedNorm& p, int wpr, cudaStream_t stream) {
+  if (p.n == 32 * wpr * V * VecTraits<T>::kElems) return launch_full<T, V, R, true>(p, wpr, stream);
+  return launch_full<T, V, R, false>(p, wpr, stream);
 }
 
 }  // namespace
@@ -242,17 +376,12 @@ cudaError_t launch_gated_norm(const GatedNorm& p, cudaStream_t stream) {
     if (reinterpret_cast<uintptr_t>(q) & 15u) return cudaErrorMisalignedAddress;
   if (reinterpret_cast<uintptr_t>(p.y_mx) & 127u) return cudaErrorMisalignedAddress;
   const int vecs = p.n / E;
-  for (int wpr = 1; wpr <= kWarps; wpr *= 2) {
-    const int v = (vecs + 32 * wpr - 1) / (32 * wpr);
-    if (v > kMaxVec) continue;
-    switch (wpr) {
-      case 1: return launch_wpr<T, 1>(p, v, stream);
-      case 2: return launch_wpr<T, 2>(p, v, stream);
-      case 4: return launch_wpr<T, 4>(p, v, stream);
-      default: return launch_wpr<T, 8>(p, v, stream);
-    }
-  }
-  return cudaErrorInvalidValue;  // wider than 8 warps of 4 vectors a lane
+  const int v = vecs <= 32 * kMaxWarps ? 1 : 2, wpr = (vecs + 32 * v - 1) / (32 * v);
+  if (wpr > kMaxWarps) return cudaErrorInvalidValue;
+  // Few rows: one at a time, so that they spread over the SMs.  Two vectors a lane: one row, for the registers.
+  const long long busy = static_cast<long long>(sm_count()) * (wpr >= kCtaWarps ? 1 : kCtaWarps / wpr);
+  if (v == 2) return launch_rows<T, 2, 1>(p, wpr, stream);
+  return p.max_m <= busy ? launch_rows<T, 1, 1>(p, wpr, stream) : launch_rows<T, 1, 2>(p, wpr, stream);
 }
 
 template cudaError_t launch_gated_norm<__half>(const GatedNorm&, cudaStream_t);
