@@ -113,6 +113,12 @@ class EffectiveTransformer:
         only the last one runs as a kernel.  Off: a LayerNorm kernel behind each hidden-wide projection."""
         _capi.check(self._lib.et_set_deferred_layernorm(self._h, 1 if on else 0), self._h)
 
+    def set_mxfp4_projections(self, on: bool) -> None:
+        """On: the layers' projections run on weights and activations in 4-bit microscaled floating point (MXFP4,
+        effective_transformer_b200.mxfp4); attention, residual stream and LayerNorms keep the handle's dtype.  Weights
+        are quantised at the first call, and with every later set_weights.  Drops recorded graphs."""
+        _capi.check(self._lib.et_set_mxfp4(self._h, 1 if on else 0), self._h)
+
     def workspace_bytes(self, batch_size: int, seq_len: int) -> int:
         n = C.c_size_t(0)
         _capi.check(self._lib.et_workspace_bytes(self._h, batch_size, seq_len, C.byref(n)), self._h)

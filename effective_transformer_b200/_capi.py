@@ -123,12 +123,14 @@ SIGNATURES = {
     "et_gemm": (i32, [i32, vp, vp, vp, vp, vp, vp, i32, i32, i32, i32, i32, vp, vp]),
     "et_pack_weight": (i32, [i32, vp, vp, i32, i32, vp]),
     "et_split_tf32": (i32, [vp, vp, vp, vp, i32, i32, vp]),
+    "et_set_mxfp4": (i32, [vp, i32]),
     "et_mxfp4_bytes": (C.c_size_t, [i32, i32]),
     "et_mxfp4_quantize": (i32, [i32, vp, i64, vp, i32, i32, vp, vp]),
     "et_mxfp4_dequantize": (i32, [i32, vp, vp, i32, i32, vp, vp]),
     "et_mxfp4_pack_weight": (i32, [i32, vp, vp, i32, i32, vp]),
     "et_mxfp4_gemm": (i32, [i32, vp, vp, vp, vp, vp, vp, vp, i32, i32, i32, i32, vp, vp]),
     "et_mxfp4_linear": (i32, [i32, vp, i64, vp, vp, vp, vp, vp, vp, vp, i32, i32, i32, i32, vp, vp]),
+    "et_mxfp4_route": (i32, [i32, i32, i32, i32, ip, ip, ip]),
     "et_gated_residual_norm": (i32, [i32, C.POINTER(GatedNormParam), vp]),
     "et_gemm_fp32_tensor": (i32, [vp, vp, vp, vp, vp, vp, vp, i32, i32, i32, i32, vp, vp]),
 }

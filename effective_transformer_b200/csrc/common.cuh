@@ -527,12 +527,21 @@ struct MxGemm {
   void* c_mx = nullptr;  // MXFP4 output instead of c
   const int* m_ptr = nullptr;
   int max_m = 0, n = 0, k = 0;
+  int route_rows = 0;    // rows by which the kernel is chosen, 0 = max_m (GemmHints::route_rows)
   int* status_word = nullptr;
 };
 // epilogue: kEpiNone to kEpiBiasTanh; residual (may be c) added behind the activation.
 template <typename T>
 cudaError_t launch_gemm_mxfp4(const MxGemm& p, const T* bias, const T* residual, T* c, int epilogue,
                               cudaStream_t stream);
+// The same from rows of T (row_stride elements apart), quantised on the way; x_mx: workspace for them in MXFP4.
+template <typename T>
+cudaError_t launch_linear_mxfp4(const MxGemm& p, const T* x, long long row_stride, void* x_mx, const T* bias,
+                                const T* residual, T* c, int epilogue, cudaStream_t stream);
+// Which kernel a product of so many rows runs, and whether one from rows of T is a single kernel.
+enum MxRoute : int { kMxSingle = 0, kMxPair = 1 };
+MxRoute mxfp4_route(bool fp32_result, int rows, int n, int k);
+bool mxfp4_rows_supported(int rows, int n, int k);
 // p = post(x + bias), h = residual_scale * residual + gate * p, y = pre(h): see norm_kernels.cu.
 struct GatedNorm {
   const void *x = nullptr, *bias = nullptr, *residual = nullptr, *gate = nullptr;

@@ -17,6 +17,7 @@
 #include <vector>
 
 #include "common.cuh"
+#include "mxfp4.cuh"
 #include "ptx_sm100.cuh"
 
 using namespace etb;
@@ -59,6 +60,11 @@ struct LayerWeights {
   void* w1_f = nullptr;
   void* c1 = nullptr;
   void* b1_f = nullptr;
+  // 4-bit projections (et_set_mxfp4): rows of the [out, in] weights in MXFP4, made when the mode is first switched on
+  void* wqkv_mx = nullptr;
+  void* wo_mx = nullptr;
+  void* w1_mx = nullptr;
+  void* w2_mx = nullptr;
   bool ready = false;
 };
 
@@ -114,6 +120,8 @@ struct Workspace {
   float* stats_att = nullptr; // ... and of att
   int* valid_word_num = nullptr;
   int* status = nullptr;
+  void* x_mx = nullptr;       // 4-bit projections: [cap, H] and [cap, F] in MXFP4
+  void* ffn_mx = nullptr;
   std::vector<void*> allocations;
 };
 
@@ -212,6 +220,8 @@ struct et_handle_s {
   bool defer_ln = true;   // used where the configuration allows it (defer_eligible)
   bool folded_ready = false;
   bool defer_active = false;
+  // et_set_mxfp4: the layers' projections run on 4-bit weights and activations.
+  bool mx = false;
   TensorMapCache maps;  // TMA descriptors of this handle's launches
   // general [B,S,S] mask of the pass being enqueued (null: key-only mask, fast kernels)
   const void* cur_attr_mask = nullptr;
@@ -419,9 +429,22 @@ int pack_layer(et_handle_t h, LayerWeights& lw, const void* const* w, cudaStream
   return ET_OK;
 }
 
+// 4-bit copies of a layer's projections, from the row-major [in, out] ones.
+template <typename T>
+int pack_layer_mx(et_handle_t h, LayerWeights& lw, cudaStream_t s) {
+  const int hid = h->hidden, f = h->cfg.ffn_dim;
+  struct { const void* w; void* mx; int k, n; } parts[] = {
+      {lw.wqkv, lw.wqkv_mx, hid, 3 * hid}, {lw.wo, lw.wo_mx, hid, hid}, {lw.w1, lw.w1_mx, hid, f}, {lw.w2, lw.w2_mx, f, hid}};
+  for (auto& p : parts) ET_CUDA(h, launch_mx_pack_weight<T>(static_cast<const T*>(p.w), p.mx, p.k, p.n, s));
+  return ET_OK;
+}
+
 int pack_layer_any(et_handle_t h, int layer, const void* const* w, cudaStream_t s) {
   LayerWeights& lw = h->layers[layer];
-  return h->cfg.dtype == ET_FP16 ? pack_layer<__half>(h, lw, w, s) : pack_layer<float>(h, lw, w, s);
+  int rc = h->cfg.dtype == ET_FP16 ? pack_layer<__half>(h, lw, w, s) : pack_layer<float>(h, lw, w, s);
+  if (rc == ET_OK && h->ws.ffn_mx != nullptr)
+    rc = h->cfg.dtype == ET_FP16 ? pack_layer_mx<__half>(h, lw, s) : pack_layer_mx<float>(h, lw, s);
+  return rc;
 }
 
 inline const __half* as_half(const void* p) { return static_cast<const __half*>(p); }
@@ -473,6 +496,118 @@ int refold_layer(et_handle_t h, size_t l, cudaStream_t s) {
   return rc;
 }
 
+// The attention of a layer: qkv [T, 3H] -> ctx [T, H] (fp32 on tensor cores, ctx_lo given: split for the tf32
+// projection behind it).
+template <typename T>
+int run_attention(et_handle_t h, const T* qkv, T* ctx, T* ctx_lo, int max_m, const int* cu_seqlens, int batch, int seq,
+                  cudaStream_t s) {
+  const int hid = h->hidden, heads = h->cfg.head_num, d = h->cfg.size_per_head;
+  Workspace& ws = h->ws;
+  auto B = [](const void* p) { return static_cast<const T*>(p); };
+  const bool tc = std::is_same<T, __half>::value && !h->use_simt;
+  const bool tc32 = std::is_same<T, float>::value && !h->use_simt;
+  auto turn = [&]() {
+    const bool reverse = h->prev_ascending;
+    h->prev_ascending = !reverse;
+    return reverse;
+  };
+  const bool masked = h->cur_attr_mask != nullptr;
+  if (masked && tc && seq <= 128)
+    // general mask on the tensor cores: the packed-tile kernel with the mask read per (query, key)
+    ET_LAUNCH(h, ET_PROF_ATTENTION, 1, s,
+              launch_attention_tcgen05(reinterpret_cast<const __half*>(qkv),
+                                       reinterpret_cast<const __half*>(qkv) + hid,
+                                       reinterpret_cast<const __half*>(qkv) + 2 * hid, 3LL * hid, d,
+                                       reinterpret_cast<__half*>(ctx), ws.attn_plan, batch, max_m, heads, d,
+                                       ws.status, s, turn(), &h->maps,
+                                       static_cast<const __half*>(h->cur_attr_mask), h->cur_batch_idx,
+                                       h->cur_word_idx, seq, h->mask_bits_ready ? ws.mask_bits() : nullptr,
+                                       true));
+  else if (masked)
+    ET_LAUNCH(h, ET_PROF_ATTENTION, 1, s,
+              launch_attention_masked_simt<T>(qkv, qkv + hid, qkv + 2 * hid, 3LL * hid, d, ctx,
+                                              B(h->cur_attr_mask), cu_seqlens, h->cur_word_idx, ws.pos_row,
+                                              batch, seq, heads, d, s));
+  else if (tc && seq <= 128)
+    ET_LAUNCH(h, ET_PROF_ATTENTION, 1, s,
+              launch_attention_tcgen05(reinterpret_cast<const __half*>(qkv),
+                                       reinterpret_cast<const __half*>(qkv) + hid,
+                                       reinterpret_cast<const __half*>(qkv) + 2 * hid, 3LL * hid, d,
+                                       reinterpret_cast<__half*>(ctx), ws.attn_plan, batch, max_m, heads, d,
+                                       ws.status, s, turn(), &h->maps, nullptr, nullptr, nullptr, 0, nullptr,
+                                       true));
+  else if (tc)
+    ET_LAUNCH(h, ET_PROF_ATTENTION, 1, s, launch_attention_tc(reinterpret_cast<const __half*>(qkv),
+                                   reinterpret_cast<const __half*>(qkv) + hid,
+                                   reinterpret_cast<const __half*>(qkv) + 2 * hid, 3LL * hid, d,
+                                   reinterpret_cast<__half*>(ctx), cu_seqlens, batch, seq, max_m, heads, d,
+                                   ws.status, s, &h->maps));
+  else if (tc32)
+    // fp32 handle: tensor cores at fp32 accuracy (three tf32 products per product), as its projections
+    ET_LAUNCH(h, ET_PROF_ATTENTION, 1, s,
+              launch_attention_tf32x3(reinterpret_cast<const float*>(qkv), reinterpret_cast<const float*>(qkv) + hid,
+                                      reinterpret_cast<const float*>(qkv) + 2 * hid, 3LL * hid, d,
+                                      reinterpret_cast<float*>(ctx), cu_seqlens, batch, seq, heads, d, s,
+                                      reinterpret_cast<float*>(ctx_lo)));
+  else
+    ET_LAUNCH(h, ET_PROF_ATTENTION, 1, s, launch_attention_simt<T>(qkv, qkv + hid, qkv + 2 * hid, 3LL * hid, d, ctx, cu_seqlens,
+                                        batch, seq, heads, d, s, ctx_lo));
+  if (!(tc && seq <= 128)) h->prev_ascending = true;  // (those kernels only run first-to-last)
+  return ET_OK;
+}
+
+// One encoder layer with 4-bit projections.  What enters a projection is in MXFP4: the layer's input (in_mx: the layer
+// before left it in ws.x_mx, beside x_in), the context, the attention block's LayerNorm and the GELU, the last two
+// written so by the kernels that make them.  out_mx: leave the layer's output in ws.x_mx too.
+template <typename T>
+int run_layer_mx(et_handle_t h, const LayerWeights& lw, const T* x_in, T* x_out, const int* t_ptr, int max_m,
+                 const int* cu_seqlens, int batch, int seq, cudaStream_t s, bool in_mx, bool out_mx) {
+  const int hid = h->hidden, f = h->cfg.ffn_dim;
+  Workspace& ws = h->ws;
+  auto B = [](const void* p) { return static_cast<const T*>(p); };
+  T* qkv = static_cast<T*>(ws.qkv);
+  T* ctx = static_cast<T*>(ws.ctx);
+  T* att = static_cast<T*>(ws.att);
+  auto args = [&](const void* a, const void* w, void* c_mx, int n, int k) {
+    MxGemm g;
+    g.a = a, g.w = w, g.c_mx = c_mx;
+    g.m_ptr = t_ptr, g.max_m = max_m, g.n = n, g.k = k;
+    g.route_rows = h->route_rows;
+    g.status_word = ws.status;
+    return g;
+  };
+  auto gemm = [&](const void* a, const void* w, const void* bias, T* c, void* c_mx, int n, int k, int epi) {
+    return launch_gemm_mxfp4<T>(args(a, w, c_mx, n, k), B(bias), nullptr, c, epi, s);
+  };
+  // from rows of T, which only this projection needs in 4 bits
+  auto linear = [&](const T* x, const void* w, const void* bias, T* c, int n, int epi) {
+    return launch_linear_mxfp4<T>(args(nullptr, w, nullptr, n, hid), x, hid, ws.x_mx, B(bias), nullptr, c, epi, s);
+  };
+  const int route = h->route_rows > 0 ? h->route_rows : max_m;
+  auto kernels = [&](int n) { return mxfp4_rows_supported(route, n, hid) ? 1 : 2; };
+  auto norm = [&](const T* x, const void* bias, const T* residual, const void* gamma, const void* beta, T* y, bool mx) {
+    GatedNorm g;
+    g.x = x, g.bias = bias, g.residual = residual;
+    g.pre_kind = ET_NORM_LAYER, g.pre_gamma = gamma, g.pre_beta = beta;
+    g.eps = h->eps;
+    g.y = y;
+    g.y_mx = mx ? ws.x_mx : nullptr;
+    g.m_ptr = t_ptr, g.max_m = max_m, g.n = hid;
+    return launch_gated_norm<T>(g, s);
+  };
+  if (in_mx)
+    ET_LAUNCH(h, ET_PROF_GEMM_QKV, 1, s, gemm(ws.x_mx, lw.wqkv_mx, lw.bqkv, qkv, nullptr, 3 * hid, hid, kEpiBias));
+  else
+    ET_LAUNCH(h, ET_PROF_GEMM_QKV, kernels(3 * hid), s, linear(x_in, lw.wqkv_mx, lw.bqkv, qkv, 3 * hid, kEpiBias));
+  if (int rc = run_attention<T>(h, qkv, ctx, nullptr, max_m, cu_seqlens, batch, seq, s); rc != ET_OK) return rc;
+  ET_LAUNCH(h, ET_PROF_GEMM_ATTN_OUT, kernels(hid), s, linear(ctx, lw.wo_mx, nullptr, att, hid, kEpiNone));
+  ET_LAUNCH(h, ET_PROF_LAYERNORM, 1, s, norm(att, lw.bo, x_in, lw.ln1_gamma, lw.ln1_beta, att, true));
+  ET_LAUNCH(h, ET_PROF_GEMM_FFN1, 1, s, gemm(ws.x_mx, lw.w1_mx, lw.b1, nullptr, ws.ffn_mx, f, hid, kEpiBiasGelu));
+  ET_LAUNCH(h, ET_PROF_GEMM_FFN2, 1, s, gemm(ws.ffn_mx, lw.w2_mx, nullptr, x_out, nullptr, hid, f, kEpiNone));
+  ET_LAUNCH(h, ET_PROF_LAYERNORM, 1, s, norm(x_out, lw.b2, att, lw.ln2_gamma, lw.ln2_beta, x_out, out_mx));
+  return ET_OK;
+}
+
 // One encoder layer on the packed layout.  x_out may alias x_in.
 // fp32 tensor path only: in_split_ready = the workspace's a_hi / a_lo already hold the tf32
 // halves of x_in (the layer before wrote them); out_split = write those of x_out for the next
@@ -481,7 +616,10 @@ template <typename T>
 int run_layer(et_handle_t h, const LayerWeights& lw, const T* x_in, T* x_out, const int* t_ptr,
               int max_m, const int* cu_seqlens, int batch, int seq, cudaStream_t s,
               bool in_split_ready = false, bool out_split = false, int layer_index = -1) {
-  const int hid = h->hidden, f = h->cfg.ffn_dim, heads = h->cfg.head_num, d = h->cfg.size_per_head;
+  if (h->mx && !h->use_simt)
+    return run_layer_mx<T>(h, lw, x_in, x_out, t_ptr, max_m, cu_seqlens, batch, seq, s, layer_index > 0,
+                           layer_index >= 0 && layer_index + 1 < h->cfg.num_layers);
+  const int hid = h->hidden, f = h->cfg.ffn_dim;
   Workspace& ws = h->ws;
   T* qkv = static_cast<T*>(ws.qkv);
   T* ctx = static_cast<T*>(ws.ctx);
@@ -550,48 +688,7 @@ int run_layer(et_handle_t h, const LayerWeights& lw, const T* x_in, T* x_out, co
   else
     ET_LAUNCH(h, ET_PROF_GEMM_QKV, tc32 ? 2 : 1, s, gemm(x_in, lw.wqkv, lw.wqkv_t, lw.wqkv_lo, lw.bqkv, qkv, 3 * hid, hid, kEpiBias));
   // attention straight from the [T, 3H] buffer to packed context [T, H]
-  const bool masked = h->cur_attr_mask != nullptr;
-  if (masked && tc && seq <= 128)
-    // general mask on the tensor cores: the packed-tile kernel with the mask read per (query, key)
-    ET_LAUNCH(h, ET_PROF_ATTENTION, 1, s,
-              launch_attention_tcgen05(reinterpret_cast<const __half*>(qkv),
-                                       reinterpret_cast<const __half*>(qkv) + hid,
-                                       reinterpret_cast<const __half*>(qkv) + 2 * hid, 3LL * hid, d,
-                                       reinterpret_cast<__half*>(ctx), ws.attn_plan, batch, max_m, heads, d,
-                                       ws.status, s, turn(), &h->maps,
-                                       static_cast<const __half*>(h->cur_attr_mask), h->cur_batch_idx,
-                                       h->cur_word_idx, seq, h->mask_bits_ready ? ws.mask_bits() : nullptr,
-                                       true));
-  else if (masked)
-    ET_LAUNCH(h, ET_PROF_ATTENTION, 1, s,
-              launch_attention_masked_simt<T>(qkv, qkv + hid, qkv + 2 * hid, 3LL * hid, d, ctx,
-                                              B(h->cur_attr_mask), cu_seqlens, h->cur_word_idx, ws.pos_row,
-                                              batch, seq, heads, d, s));
-  else if (tc && seq <= 128)
-    ET_LAUNCH(h, ET_PROF_ATTENTION, 1, s,
-              launch_attention_tcgen05(reinterpret_cast<const __half*>(qkv),
-                                       reinterpret_cast<const __half*>(qkv) + hid,
-                                       reinterpret_cast<const __half*>(qkv) + 2 * hid, 3LL * hid, d,
-                                       reinterpret_cast<__half*>(ctx), ws.attn_plan, batch, max_m, heads, d,
-                                       ws.status, s, turn(), &h->maps, nullptr, nullptr, nullptr, 0, nullptr,
-                                       true));
-  else if (tc)
-    ET_LAUNCH(h, ET_PROF_ATTENTION, 1, s, launch_attention_tc(reinterpret_cast<const __half*>(qkv),
-                                   reinterpret_cast<const __half*>(qkv) + hid,
-                                   reinterpret_cast<const __half*>(qkv) + 2 * hid, 3LL * hid, d,
-                                   reinterpret_cast<__half*>(ctx), cu_seqlens, batch, seq, max_m, heads, d,
-                                   ws.status, s, &h->maps));
-  else if (tc32)
-    // fp32 handle: tensor cores at fp32 accuracy (three tf32 products per product), as its projections
-    ET_LAUNCH(h, ET_PROF_ATTENTION, 1, s,
-              launch_attention_tf32x3(reinterpret_cast<const float*>(qkv), reinterpret_cast<const float*>(qkv) + hid,
-                                      reinterpret_cast<const float*>(qkv) + 2 * hid, 3LL * hid, d,
-                                      reinterpret_cast<float*>(ctx), cu_seqlens, batch, seq, heads, d, s,
-                                      reinterpret_cast<float*>(ctx_lo)));
-  else
-    ET_LAUNCH(h, ET_PROF_ATTENTION, 1, s, launch_attention_simt<T>(qkv, qkv + hid, qkv + 2 * hid, 3LL * hid, d, ctx, cu_seqlens,
-                                        batch, seq, heads, d, s, ctx_lo));
-  if (!(tc && seq <= 128)) forward_only();
+  if (int rc = run_attention<T>(h, qkv, ctx, ctx_lo, max_m, cu_seqlens, batch, seq, s); rc != ET_OK) return rc;
   // fp16 tensor-core path: bias + residual + LayerNorm run inside the projection kernels (rows are
   // normalised in place as soon as their last column tile has been stored), no LayerNorm launch
   if (deferred) {
@@ -803,7 +900,7 @@ int stack_impl(et_handle_t h, int batch, int seq, cudaStream_t s) {
   // No LayerNorm between the projections: x holds un-normalised sums from the first layer's end on,
   // and the last layer's LayerNorm is the one kernel that runs, behind the loop.
   h->defer_active =
-      h->defer_ln && !h->fuse_ln && h->folded_ready && !h->use_simt && defer_eligible(h->cfg) && max_m > 0;
+      h->defer_ln && !h->fuse_ln && !h->mx && h->folded_ready && !h->use_simt && defer_eligible(h->cfg) && max_m > 0;
   for (int l = 0; l < h->cfg.num_layers; ++l) {
     if (h->cfg.dtype == ET_FP16)
       rc = run_layer<__half>(h, h->layers[l], static_cast<const __half*>(ws.x), static_cast<__half*>(ws.x),
@@ -811,7 +908,7 @@ int stack_impl(et_handle_t h, int batch, int seq, cudaStream_t s) {
     else
       rc = run_layer<float>(h, h->layers[l], static_cast<const float*>(ws.x), static_cast<float*>(ws.x),
                             ws.valid_word_num, max_m, ws.cu_seqlens, batch, seq, s, l > 0,
-                            l + 1 < h->cfg.num_layers);
+                            l + 1 < h->cfg.num_layers, l);
     if (rc != ET_OK) {
       h->defer_active = false;
       return rc;
@@ -1210,6 +1307,46 @@ int et_set_deferred_layernorm(et_handle_t h, int enable) {
   }
   h->defer_ln = enable != 0;
   return ET_OK;
+}
+
+int et_set_mxfp4(et_handle_t h, int enable) {
+  ET_TRY
+  if (h == nullptr) return ET_INVALID_ARGUMENT;
+  if (h->mx == (enable != 0)) return ET_OK;
+  DeviceGuard guard(h->cfg.device);
+  ET_CUDA(h, cudaDeviceSynchronize());
+  if (enable != 0 && h->ws.ffn_mx == nullptr) {
+    const int hid = h->hidden, f = h->cfg.ffn_dim;
+    const long long cap = static_cast<long long>(h->ws.cap_tokens);
+    std::vector<WsItem> items = {{&h->ws.x_mx, mx_bytes(cap, hid)}};
+    for (auto& lw : h->layers) {
+      items.push_back({&lw.wqkv_mx, mx_bytes(3 * hid, hid)});
+      items.push_back({&lw.wo_mx, mx_bytes(hid, hid)});
+      items.push_back({&lw.w1_mx, mx_bytes(f, hid)});
+      items.push_back({&lw.w2_mx, mx_bytes(hid, f)});
+    }
+    items.push_back({&h->ws.ffn_mx, mx_bytes(cap, f)});  // (last: its pointer says that all are there)
+    for (const WsItem& it : items)
+      if (*it.slot == nullptr)
+        if (int rc = ws_alloc(h, it.slot, it.bytes); rc != ET_OK) {
+          cudaGetLastError();  // (out of memory; what is there is kept for a later call)
+          return rc;
+        }
+  }
+  if (enable != 0) {
+    for (auto& lw : h->layers) {
+      if (!lw.ready) continue;
+      const int rc = h->cfg.dtype == ET_FP16 ? pack_layer_mx<__half>(h, lw, h->own_stream)
+                                             : pack_layer_mx<float>(h, lw, h->own_stream);
+      if (rc != ET_OK) return rc;
+    }
+    ET_CUDA(h, cudaStreamSynchronize(h->own_stream));
+  }
+  graph_release(h);  // recorded passes hold the other kernel sequence
+  host_graphs_release(h);
+  h->mx = enable != 0;
+  return ET_OK;
+  ET_CATCH(h)
 }
 
 int et_workspace_allocated_bytes(et_handle_t h, size_t* out_bytes) {

@@ -56,19 +56,28 @@ int check_gemm(int dtype, const void* a, const void* w_mx, const void* bias, con
   return ET_OK;
 }
 
-int run_gemm(int dtype, const void* a_mx, const void* w_mx, const void* bias, const void* residual, void* c, void* c_mx,
-             const int* m_ptr, int max_m, int n, int k, int epilogue, int* status_word, cudaStream_t s) {
+MxGemm gemm_of(const void* a_mx, const void* w_mx, void* c_mx, const int* m_ptr, int max_m, int n, int k,
+               int* status_word) {
   MxGemm g;
   g.a = a_mx, g.w = w_mx, g.c_mx = c_mx;
   g.m_ptr = m_ptr, g.max_m = max_m, g.n = n, g.k = k;
   g.status_word = status_word;
-  if (dtype == ET_FP16)
-    return status_of(launch_gemm_mxfp4<__half>(g, static_cast<const __half*>(bias), static_cast<const __half*>(residual),
-                                               static_cast<__half*>(c), epilogue, s),
-                     "et_mxfp4_gemm");
-  return status_of(launch_gemm_mxfp4<float>(g, static_cast<const float*>(bias), static_cast<const float*>(residual),
-                                            static_cast<float*>(c), epilogue, s),
+  return g;
+}
+
+template <typename T>
+int run_gemm(const MxGemm& g, const void* bias, const void* residual, void* c, int epilogue, cudaStream_t s) {
+  return status_of(launch_gemm_mxfp4<T>(g, static_cast<const T*>(bias), static_cast<const T*>(residual),
+                                        static_cast<T*>(c), epilogue, s),
                    "et_mxfp4_gemm");
+}
+
+template <typename T>
+int run_linear(const MxGemm& g, const void* x, long long row_stride, void* x_mx, const void* bias, const void* residual,
+               void* c, int epilogue, cudaStream_t s) {
+  return status_of(launch_linear_mxfp4<T>(g, static_cast<const T*>(x), row_stride, x_mx, static_cast<const T*>(bias),
+                                          static_cast<const T*>(residual), static_cast<T*>(c), epilogue, s),
+                   "et_mxfp4_linear");
 }
 
 int run_quantize(int dtype, const void* x, long long row_stride, const int* m_ptr, int max_m, int k, void* mx,
@@ -141,8 +150,10 @@ int et_mxfp4_gemm(int dtype, const void* a_mx, const void* w_mx, const void* bia
     if (int rc = check_gemm(dtype, a_mx, w_mx, bias, residual, c, c_mx, max_m, n, k, epilogue)) return rc;
     if (misaligned_mx(a_mx)) return refuse(kAlignment);
     if (max_m == 0) return static_cast<int>(ET_OK);
-    return run_gemm(dtype, a_mx, w_mx, bias, residual, c, c_mx, m_ptr, max_m, n, k, epilogue, status_word,
-                    static_cast<cudaStream_t>(stream));
+    const MxGemm g = gemm_of(a_mx, w_mx, c_mx, m_ptr, max_m, n, k, status_word);
+    cudaStream_t s = static_cast<cudaStream_t>(stream);
+    return dtype == ET_FP16 ? run_gemm<__half>(g, bias, residual, c, epilogue, s)
+                            : run_gemm<float>(g, bias, residual, c, epilogue, s);
   });
 }
 
@@ -156,8 +167,23 @@ int et_mxfp4_linear(int dtype, const void* x, long long row_stride, void* x_mx, 
     if (max_m == 0) return static_cast<int>(ET_OK);
     if (x_mx == nullptr || misaligned_mx(x_mx)) return refuse("x_mx must be 128-byte aligned device memory");
     cudaStream_t s = static_cast<cudaStream_t>(stream);
-    if (int rc = run_quantize(dtype, x, row_stride, m_ptr, max_m, k, x_mx, s)) return rc;
-    return run_gemm(dtype, x_mx, w_mx, bias, residual, c, c_mx, m_ptr, max_m, n, k, epilogue, status_word, s);
+    const MxGemm g = gemm_of(nullptr, w_mx, c_mx, m_ptr, max_m, n, k, status_word);
+    return dtype == ET_FP16 ? run_linear<__half>(g, x, row_stride, x_mx, bias, residual, c, epilogue, s)
+                            : run_linear<float>(g, x, row_stride, x_mx, bias, residual, c, epilogue, s);
+  });
+}
+
+int et_mxfp4_route(int dtype, int rows, int n, int k, int* tile_m, int* tile_n, int* one_kernel) {
+  return guarded([&] {
+    if (!known_dtype(dtype)) return refuse("dtype must be ET_FP16 or ET_FP32");
+    if (int rc = check_width(k)) return rc;
+    if (rows <= 0 || n <= 0 || n % 32 != 0) return refuse("rows must be positive, n a positive multiple of 32");
+    if (!tile_m || !tile_n || !one_kernel) return refuse("null pointer");
+    const bool pair = mxfp4_route(dtype == ET_FP32, rows, n, k) == kMxPair;
+    *tile_m = pair ? 256 : 128;
+    *tile_n = pair ? 192 : 128;
+    *one_kernel = mxfp4_rows_supported(rows, n, k) ? 1 : 0;
+    return static_cast<int>(ET_OK);
   });
 }
 

@@ -213,8 +213,8 @@ def linear(x: torch.Tensor, weight: MxTensor, bias: Optional[torch.Tensor] = Non
            residual: Optional[torch.Tensor] = None, valid_rows: Optional[torch.Tensor] = None,
            workspace: Optional[MxTensor] = None,
            out: Union[torch.Tensor, MxTensor, None] = None) -> Union[torch.Tensor, MxTensor]:
-    """gemm(quantize(x), weight, ...) in one call; the result has x's dtype.  `workspace` takes x in MXFP4 (a program
-    that calls this in a loop keeps one per stream)."""
+    """gemm(quantize(x), weight, ...) in one call; the result has x's dtype.  `workspace`: an MxTensor of x's shape that
+    the call may use (a program that calls this in a loop keeps one per stream); few rows need none."""
     rows, k, stride, device = _check_rows(x, "x")
     _require(isinstance(weight, MxTensor) and weight.cols == k and weight.device == device,
              "weight must be an MxTensor of x's width and device")

@@ -328,6 +328,19 @@ int et_set_fused_layernorm(et_handle_t handle, int enable);
  * recorded graphs. */
 int et_set_deferred_layernorm(et_handle_t handle, int enable);
 
+/* 1: the layers' four projections run on weights and activations in 4-bit
+ * microscaled floating point (MXFP4, see et_mxfp4_gemm), in every call of the
+ * handle; the attention, the residual stream and the LayerNorms keep the
+ * handle's dtype, embeddings and pooler their projections.  The LayerNorm
+ * between the projections and the GELU leave their rows in 4 bits.  Results
+ * carry the error of 4-bit weights and activations.  The first call allocates
+ * 17/32 byte per weight and, for the handle's largest batch, per activation of
+ * hidden and ffn_dim (beside et_workspace_bytes), and quantises the weights;
+ * weights set later follow.  et_set_debug_simt(1) takes precedence, the two
+ * LayerNorm settings above have no effect meanwhile.  0 (default): as without.
+ * Changing the setting waits for the device and drops recorded graphs. */
+int et_set_mxfp4(et_handle_t handle, int enable);
+
 /* Chunking of the host-buffer call (et_forward_host): number of chunks, share of
  * a middle chunk when the first and the last have 1 (0: the handle found that
  * chunking does not pay for the last shape and sends the batch in one piece),
@@ -612,10 +625,17 @@ int et_mxfp4_pack_weight(int dtype, const void* w, void* w_mx, int k, int n, voi
  * is given. */
 int et_mxfp4_gemm(int dtype, const void* a_mx, const void* w_mx, const void* bias, const void* residual, void* c,
                   void* c_mx, const int* m_ptr, int max_m, int n, int k, int epilogue, int* status_word, void* stream);
-/* et_mxfp4_quantize into x_mx (workspace of et_mxfp4_bytes(max_m, k) bytes) and et_mxfp4_gemm in one call. */
+/* The same from x [max_m, k] (row_stride as for et_mxfp4_quantize), quantised on the way.  x_mx: workspace of
+ * et_mxfp4_bytes(max_m, k) bytes, whose contents are unspecified afterwards (few rows are quantised inside the
+ * product's kernel and do not use it). */
 int et_mxfp4_linear(int dtype, const void* x, long long row_stride, void* x_mx, const void* w_mx, const void* bias,
                     const void* residual, void* c, void* c_mx, const int* m_ptr, int max_m, int n, int k, int epilogue,
                     int* status_word, void* stream);
+
+/* Which kernel a product of `rows` rows (the capacity) with a result of `dtype` runs (a result in MXFP4: as ET_FP16):
+ * its tile, and whether et_mxfp4_linear is that of few rows (one kernel, tiles of 128 x 64).  Host only, as
+ * et_gemm_route. */
+int et_mxfp4_route(int dtype, int rows, int n, int k, int* tile_m, int* tile_n, int* one_kernel);
 
 /* ---- norms before and after a block, fused with its gate and residual scale --
  *   p = post(x + bias)

@@ -154,7 +154,29 @@ def test_the_ring_of_the_products_is_drained():
     loop and once behind it, since commits arrive asynchronously; copies in flight land behind a wait that ran out."""
     from test_kernel_sources_cpu import kernels, read
     bodies = {k: b for k, _, b in kernels(read("gemm_mxfp4.cu"))}
-    assert len(bodies) == 2
-    for body in bodies.values():
-        assert body.count("mbar_wait(free_bar(") == 2
+    assert len(bodies) == 3
+    for name, body in bodies.items():
+        # (the kernel of few rows uses each stage once)
+        assert body.count("mbar_wait(free_bar(") == (0 if name == "gemm_mxfp4_rows_kernel" else 2)
         assert body.count("mbar_drain(full_bar(") == 1 and body.count("mbar_drain(drain_bar") == 1
+
+
+def route(rows, n, k, dtype=1):
+    m, t, one = C.c_int(), C.c_int(), C.c_int()
+    assert LIB.et_mxfp4_route(dtype, rows, n, k, C.byref(m), C.byref(t), C.byref(one)) == 0
+    return m.value, t.value, one.value
+
+
+def test_routes():
+    assert route(1, 4096, 1024) == (128, 128, 1) and route(42, 2304, 768) == (128, 128, 1)
+    assert route(43, 2304, 768) == (128, 128, 0) and route(1, 4096, 2048) == (128, 128, 0)
+    assert route(128, 96, 256)[2] == 1 and route(129, 96, 32)[2] == 0
+    assert route(1, 148 * 64, 768)[2] == 1 and route(1, 149 * 64, 768)[2] == 0
+    assert route(40000, 4096, 1024) == (128, 128, 0) and route(40000, 1024, 4096) == (256, 192, 0)
+    assert route(128 * 18, 1024, 2048) == (128, 128, 0) and route(128 * 19, 1024, 2048) == (256, 192, 0)
+    assert route(128 * 74, 1024, 32, 0) == (128, 128, 0) and route(128 * 75, 1024, 32, 0) == (256, 192, 0)
+    a = C.c_int()
+    for rows, n, k in ((0, 32, 32), (1, 16, 32), (1, 32, 16), (1, 0, 32)):
+        assert LIB.et_mxfp4_route(dtype, rows, n, k, C.byref(a), C.byref(a), C.byref(a)) == BAD
+    assert LIB.et_mxfp4_route(2, 1, 32, 32, C.byref(a), C.byref(a), C.byref(a)) == BAD
+    assert LIB.et_mxfp4_route(1, 1, 32, 32, None, C.byref(a), C.byref(a)) == BAD

@@ -6,6 +6,8 @@ terms is off by at most K steps of 2^-23 of sum |a w| (a step each if the adder 
 Their own errors: GELU in fp32 1e-5 of the value; its tanh in fp16 and 4-bit results is the hardware's, documented as
 2^-11 relative, so 0.5 |x| 2^-11; tanhf 2^-22.
 """
+import ctypes as C
+
 import numpy as np
 import pytest
 import torch
@@ -16,6 +18,13 @@ from effective_transformer_b200 import _capi, mxfp4
 pytestmark = pytest.mark.gpu
 NP = {torch.float16: np.float16, torch.float32: np.float32}
 DTYPES = [torch.float16, torch.float32]
+DT = {torch.float16: _capi.ET_FP16, torch.float32: _capi.ET_FP32}
+
+
+def route(rows, n, k, dtype=1):
+    m, t, one = C.c_int(), C.c_int(), C.c_int()
+    assert _capi.load().et_mxfp4_route(dtype, rows, n, k, C.byref(m), C.byref(t), C.byref(one)) == 0
+    return m.value, t.value, one.value
 
 
 def rows_of(rng, rows, k, dtype, spread=True):
@@ -157,6 +166,33 @@ def test_product(dtype, m, k, n):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("m,k,n", [(1, 32, 32), (1, 1024, 4096), (2, 1536, 96), (32, 800, 160), (128, 96, 1024),
+                                   (42, 768, 2304), (25, 1056, 288)])
+def test_few_rows_in_one_kernel(dtype, m, k, n):
+    """The product that quantises its rows itself: the same bits as quantisation and product, at any stride, with rows past
+    the count left alone, into fp16, fp32 and 4 bits."""
+    assert route(m, n, k, DT[dtype])[2] == 1
+    x, kernel, bias, residual, (want, bound) = product_case(m + k, m, k, n, dtype, "gelu", True, True, True)
+    w, xt = mxfp4.pack_weight(cuda(kernel)), cuda(x)
+    got = mxfp4.linear(xt, w, bias=bias, activation="gelu", residual=residual)
+    assert ((got.double() - want).abs() <= bound).all()
+    a = mxfp4.quantize(xt)
+    assert torch.equal(got, mxfp4.gemm(a, w, bias=bias, activation="gelu", residual=residual))
+    wide = torch.full((m, k + 32), float("nan"), dtype=dtype, device="cuda")
+    wide[:, 16:k + 16] = xt
+    out = torch.full((m, n), 3.0, dtype=dtype, device="cuda")
+    for valid in {0, 1, m // 2, m, m + 5}:
+        t = min(valid, m)
+        out.fill_(3.0)
+        mxfp4.linear(wide[:, 16:k + 16], w, bias=bias, activation="gelu", residual=residual, valid_rows=count(valid), out=out)
+        assert torch.equal(out[:t], got[:t]) and (out[t:] == 3.0).all()
+    if n % 64 == 0:
+        in4, two = mxfp4.linear(xt, w, bias=bias, out=mxfp4.empty(m, n)), mxfp4.gemm(a, w, bias=bias, out=mxfp4.empty(m, n))
+        assert torch.equal(mxfp4.dequantize(in4, torch.float32), mxfp4.dequantize(two, torch.float32))
+    assert mxfp4.device_status() == 0
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("act", [None, "gelu", "tanh"])
 @pytest.mark.parametrize("with_residual", [False, True])
 @pytest.mark.parametrize("m,k,n", [(5, 128, 96), (300, 512, 640)])
@@ -173,9 +209,14 @@ def test_epilogues(dtype, act, with_residual, m, k, n):
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("m,k,n,act,with_residual", [
     (4100, 256, 2048, None, False), (8200, 800, 1088, "gelu", False), (6000, 96, 1440, None, True),
-    (20011, 1312, 1024, "tanh", True), (33000, 64, 288, "gelu", True), (4097, 2592, 2080, None, False)])
+    (20011, 1312, 1024, "tanh", True), (33000, 64, 288, "gelu", True), (4097, 2592, 2080, None, False),
+    (4100, 2048, 1216, "gelu", False), (6000, 2080, 1440, None, True), (9001, 2336, 1024, "tanh", True),
+    (33000, 2144, 288, "gelu", True), (38000, 2048, 32, None, False)])
 def test_large_products(dtype, m, k, n, act, with_residual):
-    """The kernel of large products: column tiles with one half, k-tiles with one to four steps, a row block too many."""
+    """Many tiles to a CTA; from K = 2048 on the kernel of CTA pairs: last tiles of 64, 128 and 192 columns that begin at
+    the start or in the middle of a row block of W, k-tiles with one to four steps, a row block too many."""
+    if k >= 2048:
+        assert route(m, n, k) == route(m, n, k, 0) == (256, 192, 0)
     x, kernel, bias, residual, (want, bound) = product_case(m, m, k, n, dtype, act, True, with_residual)
     got = mxfp4.linear(cuda(x), mxfp4.pack_weight(cuda(kernel)), bias=bias, activation=act, residual=residual)
     assert ((got.double() - want).abs() <= bound).all()
@@ -198,7 +239,8 @@ def test_products_of_small_numbers_are_exact(m, k, n):
     assert torch.equal(got.double(), cuda(x).double() @ cuda(kernel).double())
 
 
-@pytest.mark.parametrize("m,k,n", [(1, 256, 64), (77, 768, 320), (300, 512, 1024), (5001, 288, 1856)])
+@pytest.mark.parametrize("m,k,n", [(1, 256, 64), (77, 768, 320), (300, 512, 1024), (5001, 288, 1856),
+                                   (5001, 2080, 1856)])
 @pytest.mark.parametrize("act", [None, "gelu"])
 def test_product_in_4_bits(m, k, n, act):
     """c_mx is the quantised form of the fp32 result: scales and codes agree except where the fp32 result lies within
