@@ -24,7 +24,7 @@ __all__ = ["MxTensor", "empty", "quantize", "dequantize", "pack_weight", "gemm",
 
 _DTYPE = {torch.float16: _capi.ET_FP16, torch.float32: _capi.ET_FP32}
 _EPILOGUE = {None: 1, "gelu": 2, "tanh": 3}
-_status: Dict[int, torch.Tensor] = {}
+_status: Dict[int, tuple] = {}
 _lib = None
 
 
@@ -51,10 +51,13 @@ def _require(ok: bool, message: str) -> None:
 # and the text of an error is put together only when it is raised.  Devices are compared by index (get_device(), -1 on
 # the CPU).
 
-def _check(t: Optional[torch.Tensor], name: str, shape, dtype: torch.dtype, device: int) -> None:
-    if t is not None and not (isinstance(t, torch.Tensor) and t.dtype is dtype and t.shape == shape
-                              and t.get_device() == device and t.is_contiguous()):
-        raise ValueError(f"{name} must be a contiguous {list(shape)} tensor of dtype {dtype} on cuda:{device}")
+def _check(t: torch.Tensor, name: str, shape, dtype: torch.dtype, device: int) -> None:
+    try:
+        if t.dtype is dtype and t.shape == shape and t.get_device() == device and t.is_contiguous():
+            return
+    except AttributeError:  # not a tensor
+        pass
+    raise ValueError(f"{name} must be a contiguous {list(shape)} tensor of dtype {dtype} on cuda:{device}")
 
 
 def _check_rows(x: torch.Tensor, name: str):
@@ -73,19 +76,17 @@ def _check_rows(x: torch.Tensor, name: str):
 def _count(valid_rows: Optional[torch.Tensor], device: int) -> Optional[int]:
     if valid_rows is None:
         return None
-    if not (isinstance(valid_rows, torch.Tensor) and valid_rows.dtype is torch.int32 and valid_rows.numel() == 1
-            and valid_rows.get_device() == device):
-        raise ValueError("valid_rows must be one int32 on the rows' device")
-    return valid_rows.data_ptr()
+    try:
+        if valid_rows.dtype is torch.int32 and valid_rows.numel() == 1 and valid_rows.get_device() == device:
+            return valid_rows.data_ptr()
+    except AttributeError:  # not a tensor
+        pass
+    raise ValueError("valid_rows must be one int32 on the rows' device")
 
 
 def _check_mx(t: "MxTensor", name: str, rows: int, cols: int, device: int) -> None:
     if not (isinstance(t, MxTensor) and t.cols == cols and t.rows >= rows and t.device == device):
         raise ValueError(f"{name} must be an MxTensor of at least {rows} rows of {cols} values on cuda:{device}")
-
-
-def _ptr(t: Optional[torch.Tensor]) -> Optional[int]:
-    return None if t is None else t.data_ptr()
 
 
 def _call(device: int, name: str, *args) -> None:
@@ -104,12 +105,15 @@ def _call(device: int, name: str, *args) -> None:
 
 
 def _status_word(device: int) -> int:
+    """Address of the device's status word."""
     word = _status.get(device)
     if word is None:
         _require(not torch.cuda.is_current_stream_capturing(),
                  "call mxfp4.device_status(device) once before a product is captured on this device")
-        word = _status[device] = torch.zeros(1, dtype=torch.int32, device=torch.device("cuda", device))
-    return word.data_ptr()
+        data = torch.zeros(1, dtype=torch.int32, device=torch.device("cuda", device))
+        torch.cuda.current_stream(device).synchronize()  # (other streams may use it from now on)
+        word = _status[device] = (data.data_ptr(), data)
+    return word[0]
 
 
 def device_status(device: Union[int, str, torch.device] = "cuda") -> int:
@@ -118,9 +122,11 @@ def device_status(device: Union[int, str, torch.device] = "cuda") -> int:
     device = torch.device(device) if not isinstance(device, int) else torch.device("cuda", device)
     index = torch.cuda.current_device() if device.index is None else device.index
     _status_word(index)
-    code = int(_status[index].item())
-    if code != 0:
-        _status[index].zero_()
+    data = _status[index][1]
+    with torch.cuda.device(index):
+        code = int(data.item())
+        if code != 0:
+            data.zero_()
     return code
 
 
@@ -171,22 +177,32 @@ def pack_weight(kernel: torch.Tensor) -> MxTensor:
 def _result(rows: int, device: int, weight: MxTensor, bias, activation, residual, valid_rows, out, dtype: torch.dtype):
     """(out, arguments of the entry points from the bias on) of a product of `rows` rows."""
     n = weight.rows
-    _require(activation in _EPILOGUE, "activation must be None, 'gelu' or 'tanh'")
-    _require(activation is None or bias is not None, "an activation needs a bias")
+    epilogue = _EPILOGUE.get(activation)
+    if epilogue is None:
+        raise ValueError("activation must be None, 'gelu' or 'tanh'")
+    c = c_mx = bias_ptr = res_ptr = None
     if isinstance(out, MxTensor):
         _check_mx(out, "out", rows, n, device)
         _require(n % 64 == 0 and residual is None, "MXFP4 output needs a width that is a multiple of 64, and no residual")
-        c, c_mx = None, out.ptr
+        c_mx = out.ptr
     else:
         if out is None:
             out = torch.empty(rows, n, dtype=dtype, device=torch.device("cuda", device))
         else:
             _check(out, "out", (rows, n), dtype, device)
-        c, c_mx = out.data_ptr(), None
-    _check(bias, "bias", (n,), dtype, device)
-    _check(residual, "residual", (rows, n), dtype, device)
-    return out, (_ptr(bias), _ptr(residual), c, c_mx, _count(valid_rows, device), rows, n, weight.cols,
-                 0 if bias is None else _EPILOGUE[activation], _status_word(device))
+        c = out.data_ptr()
+    if bias is not None:
+        _check(bias, "bias", (n,), dtype, device)
+        bias_ptr = bias.data_ptr()
+    elif activation is None:
+        epilogue = 0
+    else:
+        raise ValueError("an activation needs a bias")
+    if residual is not None:
+        _check(residual, "residual", (rows, n), dtype, device)
+        res_ptr = residual.data_ptr()
+    return out, (bias_ptr, res_ptr, c, c_mx, None if valid_rows is None else _count(valid_rows, device), rows, n,
+                 weight.cols, epilogue, _status_word(device))
 
 
 def gemm(a: MxTensor, weight: MxTensor, bias: Optional[torch.Tensor] = None, activation: Optional[str] = None,

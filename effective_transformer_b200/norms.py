@@ -14,7 +14,7 @@ from typing import Optional, Tuple
 import torch
 
 from . import _capi
-from .mxfp4 import MxTensor, _call, _check, _check_mx, _count, _DTYPE, _ptr, _require
+from .mxfp4 import MxTensor, _call, _check, _check_mx, _count, _DTYPE, _require
 
 __all__ = ["gated_residual_norm"]
 
@@ -44,43 +44,58 @@ def gated_residual_norm(x: torch.Tensor, bias: Optional[torch.Tensor] = None, re
     rows, n = shape
     row = (n,)
     post, pre = _KIND.get(post_norm), _KIND.get(pre_norm)
-    _require(post is not None and pre is not None, "post_norm and pre_norm must be 'none', 'layer' or 'rms'")
+    if post is None or pre is None:
+        raise ValueError("post_norm and pre_norm must be 'none', 'layer' or 'rms'")
+    bias_p = res_p = gate_p = idx_p = post_g = post_b = pre_g = pre_b = y_p = mx_p = None
     if h_out is None:
         h_out = torch.empty_like(x)
+    else:
+        _check(h_out, "h_out", shape, dtype, device)
+    h_p = h_out.data_ptr()
     if y_out is None and mx_out is None:
         y_out = torch.empty_like(x)
-    h_ptr, y_ptr = h_out.data_ptr(), _ptr(y_out)
-    _require(h_ptr != y_ptr or rows == 0, "h_out and y_out must be two buffers")
-    _check(residual, "residual", shape, dtype, device)
-    _check(h_out, "h_out", shape, dtype, device)
-    _check(y_out, "y_out", shape, dtype, device)
+        y_p = y_out.data_ptr()
+    elif y_out is not None:
+        _check(y_out, "y_out", shape, dtype, device)
+        y_p = y_out.data_ptr()
+        if y_p == h_p and rows > 0:
+            raise ValueError("h_out and y_out must be two buffers")
+    if residual is not None:
+        _check(residual, "residual", shape, dtype, device)
+        res_p = residual.data_ptr()
+    if bias is not None:
+        _check(bias, "bias", row, dtype, device)
+        bias_p = bias.data_ptr()
+    # (a norm's missing gamma or beta fails its check)
     if post != 0:
-        _require(post_gamma is not None and (post != 1 or post_beta is not None), "post_norm needs its gamma (and beta)")
         _check(post_gamma, "post_gamma", row, dtype, device)
+        post_g = post_gamma.data_ptr()
         if post == 1:
             _check(post_beta, "post_beta", row, dtype, device)
+            post_b = post_beta.data_ptr()
     if pre != 0:
-        _require(pre_gamma is not None and (pre != 1 or pre_beta is not None), "pre_norm needs its gamma (and beta)")
         _check(pre_gamma, "pre_gamma", row, dtype, device)
+        pre_g = pre_gamma.data_ptr()
         if pre == 1:
             _check(pre_beta, "pre_beta", row, dtype, device)
-    _check(bias, "bias", row, dtype, device)
-    gate_rows, idx = 0, None
+            pre_b = pre_beta.data_ptr()
+    gate_rows = 0
     if gate is not None:
+        _require(isinstance(gate, torch.Tensor) and gate.dim() in (1, 2), "gate must be [width] or [sequences, width]")
         gate_rows = 1 if gate.dim() == 1 else gate.shape[0]
         _check(gate, "gate", row if gate.dim() == 1 else (gate_rows, n), dtype, device)
         _require(gate_rows >= 1, "gate must have a row")
+        gate_p = gate.data_ptr()
         if gate_rows > 1:
             _require(isinstance(batch_idx, torch.Tensor) and batch_idx.dtype is torch.int32
                      and batch_idx.is_contiguous() and batch_idx.get_device() == device and batch_idx.numel() >= rows,
                      "a gate of several rows needs batch_idx, int32, one entry per row of x")
-            idx = batch_idx.data_ptr()
+            idx_p = batch_idx.data_ptr()
     if mx_out is not None:
         _check_mx(mx_out, "mx_out", rows, n, device)
-    p = _capi.GatedNormParam(
-        x.data_ptr(), _ptr(bias), _ptr(residual), _ptr(gate), idx, _ptr(post_gamma) if post != 0 else None,
-        _ptr(post_beta) if post == 1 else None, _ptr(pre_gamma) if pre != 0 else None,
-        _ptr(pre_beta) if pre == 1 else None, h_ptr, y_ptr, None if mx_out is None else mx_out.ptr,
-        _count(valid_rows, device), rows, n, gate_rows, post, pre, residual_scale, eps)
+        mx_p = mx_out.ptr
+    p = _capi.GatedNormParam(x.data_ptr(), bias_p, res_p, gate_p, idx_p, post_g, post_b, pre_g, pre_b, h_p, y_p, mx_p,
+                             None if valid_rows is None else _count(valid_rows, device), rows, n, gate_rows, post, pre,
+                             residual_scale, eps)
     _call(device, "et_gated_residual_norm", _DTYPE[dtype], C.byref(p))
     return h_out, y_out

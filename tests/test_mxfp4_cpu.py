@@ -177,6 +177,6 @@ def test_routes():
     assert route(128 * 74, 1024, 32, 0) == (128, 128, 0) and route(128 * 75, 1024, 32, 0) == (256, 192, 0)
     a = C.c_int()
     for rows, n, k in ((0, 32, 32), (1, 16, 32), (1, 32, 16), (1, 0, 32)):
-        assert LIB.et_mxfp4_route(dtype, rows, n, k, C.byref(a), C.byref(a), C.byref(a)) == BAD
+        assert LIB.et_mxfp4_route(1, rows, n, k, C.byref(a), C.byref(a), C.byref(a)) == BAD
     assert LIB.et_mxfp4_route(2, 1, 32, 32, C.byref(a), C.byref(a), C.byref(a)) == BAD
     assert LIB.et_mxfp4_route(1, 1, 32, 32, None, C.byref(a), C.byref(a)) == BAD
