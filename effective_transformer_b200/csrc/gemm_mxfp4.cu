@@ -60,36 +60,21 @@ struct MxOut {};
 // tanh (relative error 2^-11, so at most 0.5 |x| 2^-11 here, the size of the fp16 rounding behind it; in 4 bits a
 // sixteenth of half a step at the least).  One special-function operation an element where exp and a reciprocal
 // would be two: those alone take 36 us of a 39778 x 4096 result.
-__device__ __forceinline__ void gelu_pair(float& a, float& b) {
-  const Pair x = pack2(a, b);
+__device__ __forceinline__ Pair gelu_rough(const Pair& x) {
   const Pair c1 = pack2(0.7978845608028654f, 0.7978845608028654f);
   const Pair c2 = pack2(0.7978845608028654f * 0.044715f, 0.7978845608028654f * 0.044715f);
-  float ua, ub;
-  unpack2(mul2(x, fma2(mul2(x, x), c2, c1)), ua, ub);
-  asm("tanh.approx.f32 %0, %0;" : "+f"(ua));
-  asm("tanh.approx.f32 %0, %0;" : "+f"(ub));
+  Pair t = mul2(x, fma2(mul2(x, x), c2, c1));
+  asm("tanh.approx.f32 %0, %0;" : "+f"(t.x));
+  asm("tanh.approx.f32 %0, %0;" : "+f"(t.y));
   const Pair h = mul2(x, pack2(0.5f, 0.5f));
-  unpack2(fma2(h, pack2(ua, ub), h), a, b);
+  return fma2(h, t, h);
 }
 
-// Activation of kCount values.
-template <int kCount, int ACT, bool kRough>
-__device__ __forceinline__ void activate(float* f) {
-  if (ACT == kEpiBiasGelu) {
-#pragma unroll
-    for (int i = 0; i < kCount; i += 2) {
-      if (kRough) {
-        gelu_pair(f[i], f[i + 1]);
-      } else {
-        f[i] = gelu_tanh(f[i]);
-        f[i + 1] = gelu_tanh(f[i + 1]);
-      }
-    }
-  }
-  if (ACT == kEpiBiasTanh) {
-#pragma unroll
-    for (int i = 0; i < kCount; ++i) f[i] = tanhf(f[i]);
-  }
+template <int ACT, bool kRough>
+__device__ __forceinline__ Pair activate(const Pair& x) {
+  if (ACT == kEpiBiasGelu) return kRough ? gelu_rough(x) : pack2(gelu_tanh(x.x), gelu_tanh(x.y));
+  if (ACT == kEpiBiasTanh) return pack2(tanhf(x.x), tanhf(x.y));
+  return x;
 }
 
 // Eight neighbouring values of a row of T.
@@ -105,31 +90,44 @@ struct Oct {
 #pragma unroll
     for (int i = 0; i < static_cast<int>(sizeof(T)) / 2; ++i) v[i] = ld_activation_v4(p + i * VecTraits<T>::kElems);
   }
-  __device__ __forceinline__ void add_to(float* f) const {
+  __device__ __forceinline__ void unpack(Pair* p) const {
 #pragma unroll
     for (int i = 0; i < static_cast<int>(sizeof(T)) / 2; ++i) {
       float x[VecTraits<T>::kElems];
       VecTraits<T>::unpack(v[i], x);
 #pragma unroll
-      for (int e = 0; e < VecTraits<T>::kElems; e += 2) {
-        float* d = f + i * VecTraits<T>::kElems + e;
-        unpack2(add2(pack2(d[0], d[1]), pack2(x[e], x[e + 1])), d[0], d[1]);
-      }
+      for (int e = 0; e < VecTraits<T>::kElems; e += 2)
+        p[(i * VecTraits<T>::kElems + e) / 2] = pack2(x[e], x[e + 1]);
     }
   }
 };
-__device__ __forceinline__ void store_oct(__half* p, const float* f, bool) { st_global_v4(p, VecTraits<__half>::pack(f)); }
+__device__ __forceinline__ void store_oct(__half* p, const Pair* f, bool) {
+  uint32_t w[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const __half2 h = __float22half2_rn(f[i]);
+    w[i] = *reinterpret_cast<const uint32_t*>(&h);
+  }
+  st_global_v4(p, Vec16{w[0], w[1], w[2], w[3]});
+}
 // (one whole sector where the result begins on one)
-__device__ __forceinline__ void store_oct(float* p, const float* f, bool sectors) {
+__device__ __forceinline__ void store_oct(float* p, const Pair* f, bool sectors) {
   if (sectors) {
-    asm volatile("st.global.v8.f32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(p), "f"(f[0]), "f"(f[1]), "f"(f[2]), "f"(f[3]),
-                 "f"(f[4]), "f"(f[5]), "f"(f[6]), "f"(f[7])
+    asm volatile("st.global.v8.f32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(p), "f"(f[0].x), "f"(f[0].y), "f"(f[1].x),
+                 "f"(f[1].y), "f"(f[2].x), "f"(f[2].y), "f"(f[3].x), "f"(f[3].y)
                  : "memory");
   } else {
-    st_global_v4(p, VecTraits<float>::pack(f));
-    st_global_v4(p + 4, VecTraits<float>::pack(f + 4));
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const float v[4] = {f[2 * i].x, f[2 * i].y, f[2 * i + 1].x, f[2 * i + 1].y};
+      st_global_v4(p + 4 * i, VecTraits<float>::pack(v));
+    }
   }
 }
+
+// Epilogues of the kernels: kEpiNone to kEpiBiasTanh, and this with a residual.  (Compile-time: as run-time branches
+// they cost the plain epilogue an addition and two moves a value.)
+constexpr int kWithResidual = 16;
 
 // A column group of 32 columns of a warp's 32 rows: what is fetched for it ahead, how it comes from tensor memory, and
 // what becomes of it.
@@ -137,48 +135,66 @@ __device__ __forceinline__ void store_oct(float* p, const float* f, bool sectors
 // fp16 and fp32 results: a thread has, for each of 4 row groups of 8, eight neighbouring columns of one row (see
 // mxfp4.cuh): bias and residual come in, and the result goes out, as 16 or 32 bytes a thread and 64 or 128 contiguous
 // bytes a row.
-template <typename T, typename OUT, int ACT>
+template <typename T, typename OUT, int EPI>
 struct Group {
+  static constexpr int ACT = EPI & ~kWithResidual;
+  static constexpr bool kBias = ACT != kEpiNone, kRes = (EPI & kWithResidual) != 0;
   Oct<T> bias, res[4];
 
-  // Row of row group i (rows are lanes in the order of mx_row).
-  static __device__ __forceinline__ int row_of(int i, int lane) { return mx_row(8 * i + (lane >> 2)); }
+  // Row of row group 0 (rows are lanes in the order of mx_row); the next groups' are 2, 4 and 6 further on.
+  static __device__ __forceinline__ int first_row(int lane) { return mx_row(lane >> 2); }
+  static_assert(mx_row(8 + 5) == mx_row(5) + 2 && mx_row(16 + 5) == mx_row(5) + 4 && mx_row(24 + 2) == mx_row(2) + 6, "");
 
-  __device__ __forceinline__ void fetch(const MxArgs& g, const T* bias_ptr, int row0, int col0, int M,
-                                        int lane) {
-    const int col = col0 + (lane & 3) * 8;
-    bias.zero();
-    if (bias_ptr != nullptr && col < g.n) bias.load(bias_ptr + col);
-    if (g.residual != nullptr) {
-      const T* src = static_cast<const T*>(g.residual) + static_cast<size_t>(row0) * g.n + col;
+  __device__ __forceinline__ void fetch(const MxArgs& g, const T* bias_ptr, int row0, int col0, int M, int lane) {
+    const int col = col0 + (lane & 3) * 8, row = row0 + first_row(lane);
+    if (kBias) {
+      bias.zero();
+      if (col < g.n) bias.load(bias_ptr + col);
+    }
+    if (kRes) {
+      const T* src = static_cast<const T*>(g.residual) + static_cast<size_t>(row) * g.n + col;
+      const size_t step = 2 * static_cast<size_t>(g.n);
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const int row = row_of(i, lane);
         res[i].zero();
-        if (row0 + row < M && col < g.n) res[i].load(src + static_cast<size_t>(row) * g.n);
+        if (row + 2 * i < M && col < g.n) res[i].load(src + i * step);
       }
     }
   }
-  static __device__ __forceinline__ void load(uint32_t t_row, uint32_t* r) {
+  static __device__ __forceinline__ void load(uint32_t t_row, float* r) {
     tmem_ld_16x256b_x4(t_row, r);
     tmem_ld_16x256b_x4(t_row + (16u << 16), r + 16);
   }
-  __device__ __forceinline__ void finish(const MxArgs& g, const uint32_t* r, int row0, int col0, int M, int lane) {
+  __device__ __forceinline__ void finish(const MxArgs& g, const T* bias_ptr, const float* r, int row0, int col0, int M,
+                                         int lane) {
     if (col0 >= g.n) return;  // (n is a multiple of 32)
-    T* dst = static_cast<T*>(g.c) + static_cast<size_t>(row0) * g.n + col0 + (lane & 3) * 8;
+    const int row = row0 + first_row(lane);
+    T* dst = static_cast<T*>(g.c) + static_cast<size_t>(row) * g.n + col0 + (lane & 3) * 8;
+    const size_t step = 2 * static_cast<size_t>(g.n);
+    Pair b[4];
+    if (kBias) bias.unpack(b);
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      float f[8];
+      Pair f[4];
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        f[2 * j] = __uint_as_float(r[16 * (i >> 1) + 4 * j + 2 * (i & 1)]);
-        f[2 * j + 1] = __uint_as_float(r[16 * (i >> 1) + 4 * j + 2 * (i & 1) + 1]);
+        const int at = 16 * (i >> 1) + 4 * j + 2 * (i & 1);
+        f[j] = pack2(r[at], r[at + 1]);
       }
-      bias.add_to(f);
-      activate<8, ACT, sizeof(T) == 2>(f);
-      if (g.residual != nullptr) res[i].add_to(f);
-      const int row = row_of(i, lane);
-      if (row0 + row < M) store_oct(dst + static_cast<size_t>(row) * g.n, f, g.sectors);
+      if (kBias) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) f[j] = add2(f[j], b[j]);
+      }
+#pragma unroll
+      for (int j = 0; j < 4; ++j) f[j] = activate<ACT, sizeof(T) == 2>(f[j]);
+      if (kRes) {
+        Pair x[4];
+        res[i].unpack(x);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) f[j] = add2(f[j], x[j]);
+      }
+      if (row + 2 * i < M) store_oct(dst, f, g.sectors);
+      dst += step;
     }
   }
 };
@@ -186,37 +202,52 @@ struct Group {
 // MXFP4 results: a thread has the 32 columns of one row, a scale block, and needs no other's.
 template <typename T, int ACT>
 struct Group<T, MxOut, ACT> {
+  static constexpr bool kBias = ACT != kEpiNone;
   Oct<T> bias[4];
 
   __device__ __forceinline__ void fetch(const MxArgs& g, const T* bias_ptr, int, int col0, int, int) {
+    if (kBias) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      bias[i].zero();
-      if (bias_ptr != nullptr && col0 < g.n) bias[i].load(bias_ptr + col0 + 8 * i);
+      for (int i = 0; i < 4; ++i) {
+        bias[i].zero();
+        if (col0 < g.n) bias[i].load(bias_ptr + col0 + 8 * i);
+      }
     }
   }
-  static __device__ __forceinline__ void load(uint32_t t_row, uint32_t* r) { tmem_ld_32x32b_x32(t_row, r); }
-  __device__ __forceinline__ void finish(const MxArgs& g, const uint32_t* r, int row0, int col0, int M, int lane) {
+  static __device__ __forceinline__ void load(uint32_t t_row, float* r) { tmem_ld_32x32b_x32(t_row, r); }
+  __device__ __forceinline__ void finish(const MxArgs& g, const T* bias_ptr, const float* r, int row0, int col0, int M,
+                                         int lane) {
     const int row = row0 + mx_row(lane);
     if (row >= M || col0 >= g.n) return;
-    float f[32], top = 0.f;
+    Pair f[16];
+    float top = 0.f;
+    // neighbouring columns 2 m, 2 m + 1 are neighbours in tensor memory too, as a pair
 #pragma unroll
-    for (int i = 0; i < 32; ++i) f[i] = __uint_as_float(r[mx_row(i)]);  // columns in their order
+    for (int m = 0; m < 16; ++m)
+      f[m] = pack2(r[mx_row(2 * m)], r[mx_row(2 * m) + 1]);
 #pragma unroll
-    for (int i = 0; i < 32; i += 8) {
-      bias[i / 8].add_to(f + i);
-      activate<8, ACT, true>(f + i);
+    for (int i = 0; i < 4; ++i) {
+      if (kBias) {
+        Pair b[4];
+        bias[i].unpack(b);
 #pragma unroll
-      for (int e = 0; e < 8; ++e) asm("max.NaN.f32 %0, %0, %1;" : "+f"(top) : "f"(fabsf(f[i + e])));
+        for (int j = 0; j < 4; ++j) f[4 * i + j] = add2(f[4 * i + j], b[j]);
+      }
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        Pair& v = f[4 * i + j];
+        v = activate<ACT, true>(v);
+        asm("max.NaN.f32 %0, %0, %1, %2;" : "+f"(top) : "f"(fabsf(v.x)), "f"(fabsf(v.y)));
+      }
     }
     const MxScale s = mx_scale(abs_bits(top));
     uint8_t* tile = static_cast<uint8_t*>(g.c) + mx_tile_offset(row, col0 >> 8, mx_k_tiles(g.n));
     const int rt = row & (kMxTileRows - 1), b = (col0 & 255) >> 5;
     Vec16 v;
     v.x = mx_codes8(f, s);
-    v.y = mx_codes8(f + 8, s);
-    v.z = mx_codes8(f + 16, s);
-    v.w = mx_codes8(f + 24, s);
+    v.y = mx_codes8(f + 4, s);
+    v.z = mx_codes8(f + 8, s);
+    v.w = mx_codes8(f + 12, s);
     st_global_v4(tile + mx_code_offset(rt, b), v);
     tile[mx_scale_offset(rt, b)] = static_cast<uint8_t>(s.byte);
   }
@@ -235,7 +266,7 @@ __device__ __forceinline__ bool epilogue_warp(const MxArgs& g, const T* bias_ptr
   tc_fence_after();
 #pragma unroll 1
   for (int c = 0; c < kGroups; ++c) {
-    uint32_t r[32];
+    float r[32];
     group.load(t_row + 32 * c, r);
     if (c > 0) group.fetch(g, bias_ptr, row0, col0 + 32 * c, M, lane);
     tmem_ld_wait();
@@ -244,7 +275,7 @@ __device__ __forceinline__ bool epilogue_warp(const MxArgs& g, const T* bias_ptr
       __syncwarp();
       release();
     }
-    group.finish(g, r, row0, col0 + 32 * c, M, lane);
+    group.finish(g, bias_ptr, r, row0, col0 + 32 * c, M, lane);
   }
   return true;
 }
@@ -711,7 +742,8 @@ gemm_mxfp4_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_
           n_tile * cfg::BN + half * (cfg::BN / 2), M, lane,
           [&] { return __all_sync(0xffffffffu, mbar_wait(tmem_full_bar(acc), phase, abort_flag)) != 0; },
           [&] {
-            if (lane == 0) mbar_arrive_cluster(mapa_shared(tmem_empty_bar(acc), 0));
+            // (relaxed: the accumulator's values are in registers, and this tile's stores must not be waited for)
+            if (lane == 0) mbar_arrive_cluster_relaxed(mapa_shared(tmem_empty_bar(acc), 0));
           });
       if (!got) {
         if (lane == 0) fail(kSiteEpilogueFull);
@@ -980,18 +1012,20 @@ cudaError_t launch_from(const MxArgs& g, const T* x, long long row_stride, const
 template <typename T, typename OUT>
 cudaError_t launch_out(const MxArgs& g, const T* x, long long row_stride, const T* bias, int epilogue,
                        cudaStream_t stream) {
+  constexpr int kRes = sizeof(OUT) == sizeof(T) ? kWithResidual : 0;  // (MXFP4 results take none)
+#define ETB_MX_CASE(E)                                                                            \
+  case E:                                                                                         \
+    if (g.residual != nullptr) return launch_from<T, OUT, E + kRes>(g, x, row_stride, bias, stream); \
+    return launch_from<T, OUT, E>(g, x, row_stride, bias, stream)
   switch (epilogue) {
-    case kEpiNone:
-      return launch_from<T, OUT, kEpiBias>(g, x, row_stride, nullptr, stream);
-    case kEpiBias:
-      return launch_from<T, OUT, kEpiBias>(g, x, row_stride, bias, stream);
-    case kEpiBiasGelu:
-      return launch_from<T, OUT, kEpiBiasGelu>(g, x, row_stride, bias, stream);
-    case kEpiBiasTanh:
-      return launch_from<T, OUT, kEpiBiasTanh>(g, x, row_stride, bias, stream);
+    ETB_MX_CASE(kEpiNone);
+    ETB_MX_CASE(kEpiBias);
+    ETB_MX_CASE(kEpiBiasGelu);
+    ETB_MX_CASE(kEpiBiasTanh);
     default:
       return cudaErrorInvalidValue;
   }
+#undef ETB_MX_CASE
 }
 
 template <typename T>

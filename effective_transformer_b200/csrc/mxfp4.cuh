@@ -71,11 +71,11 @@ __device__ __forceinline__ float mx_scale_value(uint32_t byte) {
   return __uint_as_float(byte == 0u ? 0x00400000u : byte == 255u ? 0x7fffffffu : byte << 23);
 }
 // Eight values as codes, the first in the lowest nibble; round to nearest, ties to the even code, saturating at 6.
-__device__ __forceinline__ uint32_t mx_codes8(const float* x, const MxScale& s) {
-  float f[8];
+__device__ __forceinline__ uint32_t mx_codes8(const Pair* x, const MxScale& s) {
   const Pair inv = pack2(s.inverse, s.inverse);
+  Pair f[4];
 #pragma unroll
-  for (int i = 0; i < 8; i += 2) unpack2(mul2(pack2(x[i], x[i + 1]), inv), f[i], f[i + 1]);
+  for (int i = 0; i < 4; ++i) f[i] = mul2(x[i], inv);
   uint32_t w;
   asm("{\n\t.reg .b8 b0, b1, b2, b3;\n\t"
       "cvt.rn.satfinite.e2m1x2.f32 b0, %2, %1;\n\t"
@@ -84,8 +84,12 @@ __device__ __forceinline__ uint32_t mx_codes8(const float* x, const MxScale& s) 
       "cvt.rn.satfinite.e2m1x2.f32 b3, %8, %7;\n\t"
       "mov.b32 %0, {b0, b1, b2, b3};\n\t}"
       : "=r"(w)
-      : "f"(f[0]), "f"(f[1]), "f"(f[2]), "f"(f[3]), "f"(f[4]), "f"(f[5]), "f"(f[6]), "f"(f[7]));
+      : "f"(f[0].x), "f"(f[0].y), "f"(f[1].x), "f"(f[1].y), "f"(f[2].x), "f"(f[2].y), "f"(f[3].x), "f"(f[3].y));
   return s.byte == 255u ? 0u : w;
+}
+__device__ __forceinline__ uint32_t mx_codes8(const float* x, const MxScale& s) {
+  const Pair p[4] = {pack2(x[0], x[1]), pack2(x[2], x[3]), pack2(x[4], x[5]), pack2(x[6], x[7])};
+  return mx_codes8(p, s);
 }
 // |x| as fp32 bits: the integer maximum of these is the largest magnitude, with NaN above infinity above the rest.
 __device__ __forceinline__ uint32_t abs_bits(float x) { return __float_as_uint(x) & 0x7fffffffu; }
