@@ -1061,17 +1061,18 @@ cudaError_t launch_checked(const MxGemm& p, const T* x, long long row_stride, co
 
 }  // namespace
 
-// Tiles of 256 x 192 by CTA pairs pay where K is long and 128 x 128 would take more than a round: they need half the L2
-// traffic per product and 40 % fewer issue slots (4096 x 4096 by 4096: 26 us against 36 us; 2000 of 3200 rows of 4096 by
-// 1024: 15.8 us against 17.3; 1024 x 2048 by 2048, one round: 6.9 against 6.5).  Shorter K is bound by the epilogue,
-// where the smaller tiles waste less (39778 x 1024 by 1024 x 4096 with GELU: 114 us by pairs, 109 us by 128 x 128;
-// 40000 x 768 by 768: 25.8 against 21.4) -- but for fp32 results that do not stay in L2, which leave for memory
-// better from the wider tiles (20011 x 1024 by 1024, quantisation included: 45 us against 66 us; while the result does
-// stay in L2, 4096 x 1024 by 1024, 10.8 against 8.5).
+// Tiles of 256 x 192 by CTA pairs need half the L2 traffic per product and 40 % fewer issue slots; tiles of 128 x 128
+// start sooner, waste less at the edges and have the shorter epilogue.  Measured, 128 x 128 / pairs, us:
+//   at least three rounds of 128 x 128 tiles, K = 4096: 8192 x 1024 23.2 / 17.0; K = 2048: 4096 x 2048 14.1 / 11.6;
+//     K = 1024: 40000 x 4096 108 / 92, with GELU 114 / 102; K = 768: 16000 x 2304 22.8 / 20.3, with a residual 48 / 38
+//     (fp32 31.8 / 31.2 and 93 / 58); but K = 256: 40000 x 1024 20.0 / 20.7, with GELU 22.5 / 24.4;
+//   one to three rounds, K = 4096: 4096 x 1024 13.7 / 12.6; K = 2048: 2048 x 2048 9.1 / 8.7 (fp32 9.1 / 10.0);
+//     K = 1024: 4096 x 1024 with GELU 6.8 / 7.2;
+//   one round, K = 2048: 1024 x 2048 6.4 / 6.6.
 MxRoute mxfp4_route(bool fp32_result, int rows, int n, int k) {
   const long long tiles = static_cast<long long>((rows + BM - 1) / BM) * ((n + 127) / 128);
-  if (k >= 2048 && tiles > sm_count()) return kMxPair;
-  return fp32_result && tiles > 4 * sm_count() ? kMxPair : kMxSingle;
+  if (tiles > 3ll * sm_count()) return k >= 768 ? kMxPair : kMxSingle;
+  return !fp32_result && k >= 2048 && tiles > sm_count() ? kMxPair : kMxSingle;
 }
 // The kernel that quantises the rows itself pays while its tiles are one round of CTAs, K fits its shared memory and the
 // rows, which every CTA quantises again, are few: 128 pieces of 256 values.  1024 x 1024, 1 / 16 / 32 / 64 rows: 3.6 /

@@ -172,9 +172,12 @@ def test_routes():
     assert route(43, 2304, 768) == (128, 128, 0) and route(1, 4096, 2048) == (128, 128, 0)
     assert route(128, 96, 256)[2] == 1 and route(129, 96, 32)[2] == 0
     assert route(1, 148 * 64, 768)[2] == 1 and route(1, 149 * 64, 768)[2] == 0
-    assert route(40000, 4096, 1024) == (128, 128, 0) and route(40000, 1024, 4096) == (256, 192, 0)
-    assert route(128 * 18, 1024, 2048) == (128, 128, 0) and route(128 * 19, 1024, 2048) == (256, 192, 0)
-    assert route(128 * 74, 1024, 32, 0) == (128, 128, 0) and route(128 * 75, 1024, 32, 0) == (256, 192, 0)
+    pair = (256, 192, 0)
+    assert route(40000, 4096, 1024) == route(40000, 1024, 4096) == route(128 * 445, 32, 768) == pair
+    assert route(128 * 444, 32, 768) == route(128 * 445, 32, 736) == (128, 128, 0)
+    assert route(128 * 18, 1024, 2048) == (128, 128, 0) and route(128 * 19, 1024, 2048) == pair
+    assert route(128 * 19, 1024, 2016) == route(128 * 55, 1024, 4096, 0) == (128, 128, 0)
+    assert route(128 * 56, 1024, 768, 0) == pair
     a = C.c_int()
     for rows, n, k in ((0, 32, 32), (1, 16, 32), (1, 32, 16), (1, 0, 32)):
         assert LIB.et_mxfp4_route(1, rows, n, k, C.byref(a), C.byref(a), C.byref(a)) == BAD
