@@ -25,8 +25,8 @@ namespace {
 using namespace ptx;
 
 constexpr int BM = 128;
-// Epilogue warps: two sets of eight that take the tiles in turn, a set per accumulator buffer, so that one loads and
-// computes while the other stores; in a set, a TMEM lane quadrant and one half of the columns each.
+// Epilogue warps of the 128 x 128 tiles: two sets of eight that take the tiles in turn, a set per accumulator buffer,
+// so that one loads and computes while the other stores; in a set, a TMEM lane quadrant and one half of the columns each.
 constexpr int kEpilogueSet = 8;
 constexpr int kNumThreads = 64 + 2 * kEpilogueSet * 32;
 constexpr int kUmmaK = 64;
@@ -255,27 +255,32 @@ struct Group<T, MxOut, ACT> {
 
 // The epilogue of one warp: kGroups column groups of its 32 rows from (row0, col0) of a finished accumulator buffer
 // (TMEM lanes at the lane field of t_row).  wait() returns whether the accumulator has come; release() hands the buffer
-// back, when the last group is in registers.  What a group needs from global memory is on its way while its columns
-// come from tensor memory; the other warps of the scheduler (four in all) hide the rest.
-template <typename T, typename OUT, int ACT, int kGroups, typename Wait, typename Release>
+// back, when the last group is in registers.
+// kAhead: what all groups need from global memory is fetched before the wait, and not a group's while its columns come
+// from tensor memory.  kWhole: all groups are taken into registers first, so that the buffer goes back at once.
+template <typename T, typename OUT, int EPI, int kGroups, bool kAhead, bool kWhole, typename Wait, typename Release>
 __device__ __forceinline__ bool epilogue_warp(const MxArgs& g, const T* bias_ptr, uint32_t t_row, int row0,
                                               int col0, int M, int lane, Wait wait, Release release) {
-  Group<T, OUT, ACT> group;
-  group.fetch(g, bias_ptr, row0, col0, M, lane);
+  static_assert(kAhead || !kWhole, "");
+  Group<T, OUT, EPI> group[kAhead ? kGroups : 1];
+#pragma unroll
+  for (int c = 0; c < (kAhead ? kGroups : 1); ++c) group[c].fetch(g, bias_ptr, row0, col0 + 32 * c, M, lane);
   if (!wait()) return false;
   tc_fence_after();
-#pragma unroll 1
+  float r[kWhole ? kGroups : 1][32];
+#pragma unroll
+  for (int c = 0; kWhole && c < kGroups; ++c) group[0].load(t_row + 32 * c, r[kWhole ? c : 0]);
+#pragma unroll (kAhead ? kGroups : 1)
   for (int c = 0; c < kGroups; ++c) {
-    float r[32];
-    group.load(t_row + 32 * c, r);
-    if (c > 0) group.fetch(g, bias_ptr, row0, col0 + 32 * c, M, lane);
-    tmem_ld_wait();
-    if (c == kGroups - 1) {
+    if (!kWhole) group[0].load(t_row + 32 * c, r[0]);
+    if (!kAhead && c > 0) group[0].fetch(g, bias_ptr, row0, col0 + 32 * c, M, lane);
+    if (!kWhole || c == 0) tmem_ld_wait();
+    if (c == (kWhole ? 0 : kGroups - 1)) {
       tc_fence_before();
       __syncwarp();
       release();
     }
-    group.finish(g, bias_ptr, r, row0, col0 + 32 * c, M, lane);
+    group[kAhead ? c : 0].finish(g, bias_ptr, r[kWhole ? c : 0], row0, col0 + 32 * c, M, lane);
   }
   return true;
 }
@@ -493,7 +498,7 @@ gemm_mxfp4_kernel(const MxArgs g, const T* bias) {
     uint32_t phase = 0;
     for (int tile = blockIdx.x + acc * gridDim.x; tile < num_tiles; tile += 2 * gridDim.x, phase ^= 1u) {
       const int m_tile = tile / n_tiles, n_tile = tile - m_tile * n_tiles;
-      const bool got = epilogue_warp<T, OUT, ACT, BN / 64>(
+      const bool got = epilogue_warp<T, OUT, ACT, BN / 64, sizeof(OUT) == 2, false>(
           g, bias, t_row, m_tile * BM + quad * 32, n_tile * BN + half * (BN / 2), M, lane,
           [&] { return __all_sync(0xffffffffu, mbar_wait(tmem_full_bar(acc), phase, abort_flag)) != 0; },
           [&] {
@@ -523,14 +528,27 @@ gemm_mxfp4_kernel(const MxArgs g, const T* bias) {
 // for its waits, copies and commits: MMAs of N = 128 (64 cycles) do not cover that, of N = 192 (96 cycles) nearly do.
 // A single accumulator buffer leaves the tensor core idle for 1000 to 1800 cycles a tile, the way from the last MMA
 // to the epilogue and back.  And two buffers have to fit 512 columns beside the scales (24 columns a stage).
-// 39778 x 1024 by 1024 x 4096, plain fp16 result / 39778 x 4096 by 4096 x 1024: 256 x 256 in two column halves with
-// three half-width buffers 120 / 82 us, 256 x 256 with one buffer 118 / 71 us, tiles of 128 x 128 105 / 87 us.
+// 39778 x 1024 by 1024 x 4096, plain fp16 result / 39778 x 4096 by 4096 x 1024: 256 x 192 85 / 67 us, tiles of 128 x 128
+// 104 / 83 us (and, with an earlier epilogue that took 104 / 76 us here: 256 x 256 in two column halves with three
+// half-width buffers 120 / 82 us, 256 x 256 with one buffer 118 / 71 us).
+//
+// What bounds it now is the way of the operands from L2 to the SMs: 7.4 KB per 64 values of K and CTA, 119 cycles at 64
+// bytes a cycle where the MMA needs 96; 47 to 57 bytes a cycle and SM are measured.
+//
+// Epilogue: all twelve warps on every tile, two column groups each that are in registers before the buffer goes back.
+// Two sets of eight warps in turn, three groups each one after the other, took the same time for plain results (which
+// the operands bound) but 190 us against 136 us with a residual, whose latency they met once per group.
 //
 // A tile's 192 W rows begin at the start or in the middle of a row block of 128: it takes the scales of two blocks, and
 // in the second case the MMAs read them from two columns (64 rows) further on.
 struct PairCfg {
   static constexpr int BN = 192;
   static constexpr int kStages = 5;
+  static constexpr int kEpilogueWarps = 12;  // a TMEM lane quadrant and a third of the columns each
+  static constexpr int kThreads = 64 + 32 * kEpilogueWarps;
+  // both groups of a warp in registers at once, where they fit beside what is added to them (128 registers a thread)
+  template <typename T, typename OUT, int EPI>
+  static constexpr bool kWhole = sizeof(T) == 2 || (sizeof(OUT) == 4 && (EPI & kWithResidual) == 0);
   static constexpr int kBCodes = BN / 2 * 128;
   static constexpr int kStageBytes = kMxTileBytes + kBCodes + 2 * kMxScaleBytes;
   static constexpr int kScaleCols = 24;  // per stage: 2 pieces of A, 2 of each block of W, 4 columns each
@@ -542,7 +560,7 @@ struct PairCfg {
 };
 
 template <typename T, typename OUT, int ACT>
-__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kNumThreads, 1)
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PairCfg::kThreads, 1)
 gemm_mxfp4_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant__ CUtensorMap tmap_w,
                        const __grid_constant__ CUtensorMap tmap_ws, const MxArgs g, const T* bias) {
   using cfg = PairCfg;
@@ -576,7 +594,7 @@ gemm_mxfp4_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_
     }
     for (int a = 0; a < 2; ++a) {
       mbar_init(tmem_full_bar(a), 1);
-      mbar_init(tmem_empty_bar(a), 2 * kEpilogueSet);
+      mbar_init(tmem_empty_bar(a), 2 * cfg::kEpilogueWarps);
     }
     mbar_init(drain_bar, 1);
     *abort_flag = 0;
@@ -732,15 +750,16 @@ gemm_mxfp4_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_
     }
   } else {
     // ------------------------- epilogue (both CTAs) -------------------------
-    const int quad = warp & 3, half = ((warp - 2) >> 2) & 1, acc = (warp - 2) / kEpilogueSet;
-    const uint32_t t_row = tmem_base + (static_cast<uint32_t>(quad * 32) << 16) + acc * cfg::BN + half * (cfg::BN / 2);
-    uint32_t phase = 0;
-    for (int tile = pair_id + acc * num_pairs; tile < num_tiles; tile += 2 * num_pairs, phase ^= 1u) {
+    const int quad = warp & 3, part = (warp - 2) >> 2;
+    const uint32_t t_row = tmem_base + (static_cast<uint32_t>(quad * 32) << 16) + part * 64;
+    int it = 0;
+    for (int tile = pair_id; tile < num_tiles; tile += num_pairs, ++it) {
+      const int acc = it & 1;
       const int m_tile = tile / n_tiles, n_tile = tile - m_tile * n_tiles;
-      const bool got = epilogue_warp<T, OUT, ACT, cfg::BN / 64>(
-          g, bias, t_row, m_tile * 256 + static_cast<int>(rank) * BM + quad * 32,
-          n_tile * cfg::BN + half * (cfg::BN / 2), M, lane,
-          [&] { return __all_sync(0xffffffffu, mbar_wait(tmem_full_bar(acc), phase, abort_flag)) != 0; },
+      const bool got = epilogue_warp<T, OUT, ACT, 2, true, cfg::kWhole<T, OUT, ACT>>(
+          g, bias, t_row + acc * cfg::BN, m_tile * 256 + static_cast<int>(rank) * BM + quad * 32,
+          n_tile * cfg::BN + part * 64, M, lane,
+          [&] { return __all_sync(0xffffffffu, mbar_wait(tmem_full_bar(acc), (it >> 1) & 1, abort_flag)) != 0; },
           [&] {
             // (relaxed: the accumulator's values are in registers, and this tile's stores must not be waited for)
             if (lane == 0) mbar_arrive_cluster_relaxed(mapa_shared(tmem_empty_bar(acc), 0));
@@ -791,7 +810,7 @@ cudaError_t launch_pair(const MxArgs& g, const T* bias, cudaStream_t stream) {
     return cudaErrorInvalidValue;
   const long long tiles = static_cast<long long>((g.max_m + 255) / 256) * ((g.n + cfg::BN - 1) / cfg::BN);
   const int pairs = static_cast<int>(tiles < sm_count() / 2 ? tiles : sm_count() / 2);
-  return launch_pdl(gemm_mxfp4_pair_kernel<T, OUT, ACT>, dim3(2 * pairs), dim3(kNumThreads), cfg::kSmemBytes, stream,
+  return launch_pdl(gemm_mxfp4_pair_kernel<T, OUT, ACT>, dim3(2 * pairs), dim3(cfg::kThreads), cfg::kSmemBytes, stream,
                     ta, tw, tws, g, bias);
 }
 
@@ -956,7 +975,7 @@ gemm_mxfp4_rows_kernel(const MxArgs g, const T* x, long long row_stride, const T
     // ---- epilogue: eight of the warps, a lane quadrant and 32 columns each ----
     if (warp < 2 + kEpilogueSet) {
       const int quad = warp & 3, half = (warp - 2) >> 2;
-      const bool got = epilogue_warp<T, OUT, ACT, 1>(
+      const bool got = epilogue_warp<T, OUT, ACT, 1, true, true>(
           g, bias, tmem_base + (static_cast<uint32_t>(quad * 32) << 16) + half * 32, row_tile + quad * 32,
           n_tile * BN + half * 32, M, lane,
           [&] { return __all_sync(0xffffffffu, mbar_wait(tmem_full_bar, 0u, abort_flag)) != 0; }, [] {});
