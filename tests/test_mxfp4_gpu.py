@@ -85,6 +85,20 @@ def test_quantize_ties_ranges_and_specials(dtype):
     assert np.isnan(got[5, :32]).all() and not np.isnan(got[5, 32:]).any()
 
 
+def test_every_code_at_every_scale_comes_back():
+    """Both directions are exact in fp32; in fp16 the one rounding of a value (2^-24 steps below 2^-14, infinity above)."""
+    codes = np.array([0, 0.5, 1, 1.5, 2, 3, 4, 6], np.float64)
+    block = np.concatenate([codes, -codes, -codes, codes])
+    x = (block[None, :] * 2.0 ** np.arange(-127, 126)[:, None]).astype(np.float32)
+    mx = mxfp4.quantize(cuda(x))
+    same_parts(mx, x)
+    assert np.array_equal(mxfp4.dequantize(mx, torch.float32).cpu().numpy(), x)
+    with np.errstate(over="ignore"):
+        want = x.astype(np.float16)
+    got = mxfp4.dequantize(mx, torch.float16).cpu().numpy()
+    assert np.array_equal(got.view(np.uint16), want.view(np.uint16))
+
+
 @pytest.mark.parametrize("dtype", DTYPES)
 def test_quantize_strided_rows_and_rows_past_the_count(dtype):
     rng = np.random.RandomState(3)
