@@ -521,6 +521,11 @@ template <typename T>
 cudaError_t launch_mx_dequantize(const void* mx, const int* m_ptr, int max_m, int k, T* out, cudaStream_t stream);
 template <typename T>
 cudaError_t launch_mx_pack_weight(const T* w, void* mx, int k, int n, cudaStream_t stream);
+// Whether [a, a + na) and [b, b + nb) share a byte; null shares none.
+inline bool overlap(const void* a, size_t na, const void* b, size_t nb) {
+  const uintptr_t x = reinterpret_cast<uintptr_t>(a), y = reinterpret_cast<uintptr_t>(b);
+  return a != nullptr && b != nullptr && x < y + nb && y < x + na;
+}
 struct MxGemm {
   const void* a = nullptr;
   const void* w = nullptr;

@@ -344,7 +344,6 @@ gemm_mxfp4_kernel(const MxArgs g, const T* bias) {
   constexpr int BN = 128;
   using cfg = Cfg<BN>;
   constexpr int S = cfg::kStages;
-  pdl_trigger();
 
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   const uint32_t tiles_addr = smem_u32(smem_raw);
@@ -385,6 +384,7 @@ gemm_mxfp4_kernel(const MxArgs g, const T* bias) {
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
+  pdl_trigger();  // (not before: a dependent's CTA must not take the tensor memory that this one waits for)
   const uint32_t tmem_base = __shfl_sync(0xffffffffu, *tmem_slot, 0);
 
   int M = g.max_m;
@@ -565,7 +565,6 @@ gemm_mxfp4_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_
                        const __grid_constant__ CUtensorMap tmap_ws, const MxArgs g, const T* bias) {
   using cfg = PairCfg;
   constexpr int S = cfg::kStages;
-  pdl_trigger();
   const uint32_t rank = cluster_ctarank();  // 0 issues the MMAs
   const int pair_id = blockIdx.x >> 1, num_pairs = gridDim.x >> 1;
 
@@ -609,6 +608,7 @@ gemm_mxfp4_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_
   __syncthreads();
   cluster_sync_all();  // the peer's barriers are initialised before anything signals them
   tc_fence_after();
+  pdl_trigger();  // (not before: a dependent's CTA must not take the tensor memory that this one waits for)
   const uint32_t tmem_base = __shfl_sync(0xffffffffu, *tmem_slot, 0);
 
   int M = g.max_m;
@@ -838,7 +838,6 @@ __global__ void __launch_bounds__(kNumThreads, 1)
 gemm_mxfp4_rows_kernel(const MxArgs g, const T* x, long long row_stride, const T* bias) {
   using cfg = RowsCfg;
   constexpr int BN = cfg::BN;
-  pdl_trigger();
   const int k_tiles = mx_k_tiles(g.k);
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   const uint32_t tiles_addr = smem_u32(smem_raw);
@@ -871,6 +870,7 @@ gemm_mxfp4_rows_kernel(const MxArgs g, const T* x, long long row_stride, const T
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
+  pdl_trigger();  // (not before: a dependent's CTA must not take the tensor memory that this one waits for)
   const uint32_t tmem_base = __shfl_sync(0xffffffffu, *tmem_slot, 0);
 
   int M = g.max_m;
@@ -1112,7 +1112,11 @@ cudaError_t launch_linear_mxfp4(const MxGemm& p, const T* x, long long row_strid
                                 const T* residual, T* c, int epilogue, cudaStream_t stream) {
   if (p.max_m <= 0) return cudaSuccess;
   if (x == nullptr || row_stride < p.k || row_stride * sizeof(T) % 16 != 0) return cudaErrorInvalidValue;
-  if (mxfp4_rows_supported(p.route_rows > 0 ? p.route_rows : p.max_m, p.n, p.k))
+  // (the kernel of few rows reads x while other CTAs of it write: not in place)
+  const size_t x_size = (static_cast<size_t>(p.max_m - 1) * row_stride + p.k) * sizeof(T);
+  const bool in_place = overlap(x, x_size, c, static_cast<size_t>(p.max_m) * p.n * sizeof(T)) ||
+                        (p.c_mx != nullptr && overlap(x, x_size, p.c_mx, mx_bytes(p.max_m, p.n)));
+  if (!in_place && mxfp4_rows_supported(p.route_rows > 0 ? p.route_rows : p.max_m, p.n, p.k))
     return launch_checked<T>(p, x, row_stride, bias, residual, c, epilogue, stream);
   const cudaError_t err = launch_mx_quantize<T>(x, row_stride, p.m_ptr, p.max_m, p.k, x_mx, stream);
   if (err != cudaSuccess) return err;

@@ -35,6 +35,10 @@ bool misaligned(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) !
 bool misaligned_mx(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 127u) != 0; }
 bool known_dtype(int dtype) { return dtype == ET_FP16 || dtype == ET_FP32; }
 size_t size_of(int dtype) { return dtype == ET_FP16 ? 2 : 4; }
+// Bytes from the first to behind the last value of `rows` rows (at least one).
+size_t rows_size(int dtype, int rows, long long row_stride, int k) {
+  return (static_cast<size_t>(rows - 1) * row_stride + k) * size_of(dtype);
+}
 
 int check_width(int k) {
   if (k <= 0 || k % kMxBlock != 0) return refuse("the width of an MXFP4 row must be a positive multiple of 32");
@@ -53,6 +57,18 @@ int check_gemm(int dtype, const void* a, const void* w_mx, const void* bias, con
   if (a == nullptr || w_mx == nullptr || (epilogue != kEpiNone && bias == nullptr)) return refuse("null pointer");
   if (misaligned(a) || misaligned(bias) || misaligned(residual) || misaligned(c) || misaligned_mx(w_mx) || misaligned_mx(c_mx))
     return refuse(kAlignment);
+  return ET_OK;
+}
+
+// The result may be the residual (every element is read where it is written), and nothing else.
+int check_result(int dtype, const void* w_mx, const void* bias, const void* residual, const void* c, const void* c_mx,
+                 const void* rows_mx, int max_m, int n, int k) {
+  const size_t elem = size_of(dtype), c_size = static_cast<size_t>(max_m) * n * elem;
+  const void* out = c != nullptr ? c : c_mx;
+  const size_t size = c != nullptr ? c_size : mx_bytes(max_m, n);
+  if (overlap(out, size, rows_mx, mx_bytes(max_m, k)) || overlap(out, size, w_mx, mx_bytes(n, k)) ||
+      overlap(out, size, bias, n * elem) || (residual != c && overlap(out, size, residual, c_size)))
+    return refuse("the result must not overlap an operand, except that c may be the residual");
   return ET_OK;
 }
 
@@ -108,6 +124,8 @@ int et_mxfp4_quantize(int dtype, const void* x, long long row_stride, const int*
     if (max_m == 0) return static_cast<int>(ET_OK);
     if (x == nullptr || mx == nullptr) return refuse("null pointer");
     if (misaligned(x) || misaligned_mx(mx)) return refuse(kAlignment);
+    if (overlap(x, rows_size(dtype, max_m, row_stride, k), mx, mx_bytes(max_m, k)))
+      return refuse("x and mx must not overlap");
     return run_quantize(dtype, x, row_stride, m_ptr, max_m, k, mx, static_cast<cudaStream_t>(stream));
   });
 }
@@ -120,6 +138,8 @@ int et_mxfp4_dequantize(int dtype, const void* mx, const int* m_ptr, int max_m, 
     if (max_m == 0) return static_cast<int>(ET_OK);
     if (mx == nullptr || out == nullptr) return refuse("null pointer");
     if (misaligned_mx(mx) || misaligned(out)) return refuse(kAlignment);
+    if (overlap(mx, mx_bytes(max_m, k), out, rows_size(dtype, max_m, k, k)))
+      return refuse("mx and out must not overlap");
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     if (dtype == ET_FP16)
       return status_of(launch_mx_dequantize<__half>(mx, m_ptr, max_m, k, static_cast<__half*>(out), s),
@@ -136,6 +156,7 @@ int et_mxfp4_pack_weight(int dtype, const void* w, void* w_mx, int k, int n, voi
     if (n <= 0 || n % 32 != 0) return refuse("n must be a positive multiple of 32");
     if (w == nullptr || w_mx == nullptr) return refuse("null pointer");
     if (misaligned_mx(w_mx)) return refuse(kAlignment);
+    if (overlap(w, rows_size(dtype, k, n, n), w_mx, mx_bytes(n, k))) return refuse("w and w_mx must not overlap");
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     if (dtype == ET_FP16)
       return status_of(launch_mx_pack_weight<__half>(static_cast<const __half*>(w), w_mx, k, n, s),
@@ -150,6 +171,7 @@ int et_mxfp4_gemm(int dtype, const void* a_mx, const void* w_mx, const void* bia
     if (int rc = check_gemm(dtype, a_mx, w_mx, bias, residual, c, c_mx, max_m, n, k, epilogue)) return rc;
     if (misaligned_mx(a_mx)) return refuse(kAlignment);
     if (max_m == 0) return static_cast<int>(ET_OK);
+    if (int rc = check_result(dtype, w_mx, bias, residual, c, c_mx, a_mx, max_m, n, k)) return rc;
     const MxGemm g = gemm_of(a_mx, w_mx, c_mx, m_ptr, max_m, n, k, status_word);
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     return dtype == ET_FP16 ? run_gemm<__half>(g, bias, residual, c, epilogue, s)
@@ -166,6 +188,12 @@ int et_mxfp4_linear(int dtype, const void* x, long long row_stride, void* x_mx, 
       return refuse("row_stride must be at least k and a multiple of 16 bytes");
     if (max_m == 0) return static_cast<int>(ET_OK);
     if (x_mx == nullptr || misaligned_mx(x_mx)) return refuse("x_mx must be 128-byte aligned device memory");
+    if (int rc = check_result(dtype, w_mx, bias, residual, c, c_mx, x_mx, max_m, n, k)) return rc;
+    const size_t elem = size_of(dtype), mx_size = mx_bytes(max_m, k);
+    if (overlap(x_mx, mx_size, x, rows_size(dtype, max_m, row_stride, k)) ||
+        overlap(x_mx, mx_size, w_mx, mx_bytes(n, k)) || overlap(x_mx, mx_size, bias, n * elem) ||
+        overlap(x_mx, mx_size, residual, static_cast<size_t>(max_m) * n * elem))
+      return refuse("x_mx must not overlap an operand");
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     const MxGemm g = gemm_of(nullptr, w_mx, c_mx, m_ptr, max_m, n, k, status_word);
     return dtype == ET_FP16 ? run_linear<__half>(g, x, row_stride, x_mx, bias, residual, c, epilogue, s)
@@ -211,6 +239,23 @@ int et_gated_residual_norm(int dtype, const et_gated_norm_param_t* p, void* stre
                           static_cast<const void*>(p->h_out), static_cast<const void*>(p->y_out)})
       if (misaligned(q)) return refuse(kAlignment);
     if (misaligned_mx(p->y_mx)) return refuse(kAlignment);
+    {
+      // every element of x and residual is read where h and y are written, nothing else is
+      const size_t row = p->n * size_of(dtype), all = p->max_m * row;
+      const struct { const void* at; size_t size; } outs[] = {
+          {p->h_out, all}, {p->y_out, all}, {p->y_mx, p->y_mx != nullptr ? mx_bytes(p->max_m, p->n) : 0}};
+      for (int i = 0; i < 3; ++i) {
+        const auto& o = outs[i];
+        bool bad = false;
+        for (const void* q : {p->x, p->residual}) bad = bad || ((q != o.at || i == 2) && overlap(o.at, o.size, q, all));
+        for (const void* q : {p->bias, p->post_gamma, p->post_beta, p->pre_gamma, p->pre_beta})
+          bad = bad || overlap(o.at, o.size, q, row);
+        bad = bad || overlap(o.at, o.size, p->gate, static_cast<size_t>(p->gate_rows) * row) ||
+              (p->gate_rows > 1 && overlap(o.at, o.size, p->batch_idx, p->max_m * sizeof(int)));
+        for (int j = 0; j < i; ++j) bad = bad || overlap(o.at, o.size, outs[j].at, outs[j].size);
+        if (bad) return refuse("outputs must not overlap each other or an input, except that h_out or y_out may be x or residual");
+      }
+    }
     GatedNorm g;
     g.x = p->x, g.bias = p->bias, g.residual = p->residual, g.gate = p->gate;
     g.batch_idx = p->gate_rows > 1 ? p->batch_idx : nullptr;

@@ -35,6 +35,11 @@ class MxTensor:
     __slots__ = ("data", "rows", "cols", "ptr", "device")
 
     def __init__(self, data: torch.Tensor, rows: int, cols: int):
+        _require(rows >= 0 and cols > 0 and cols % 32 == 0,
+                 "rows must not be negative, cols a positive multiple of 32")
+        _require(isinstance(data, torch.Tensor) and data.dtype is torch.uint8 and data.is_contiguous()
+                 and data.numel() >= _capi.load().et_mxfp4_bytes(rows, cols),
+                 "data must be a contiguous uint8 tensor that holds rows x cols values (empty() makes one)")
         self.data, self.rows, self.cols = data, rows, cols
         self.ptr, self.device = data.data_ptr(), data.get_device()
 
@@ -151,7 +156,7 @@ def quantize(x: torch.Tensor, valid_rows: Optional[torch.Tensor] = None, out: Op
 def dequantize(mx: MxTensor, dtype: torch.dtype, valid_rows: Optional[torch.Tensor] = None,
                out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """The values that an MXFP4 tensor stands for, as [rows, cols] of `dtype`."""
-    _require(isinstance(mx, MxTensor), "mx must be an MxTensor")
+    _require(isinstance(mx, MxTensor) and mx.device >= 0, "mx must be an MxTensor on a GPU")
     _require(dtype in _DTYPE, "dtype must be torch.float16 or torch.float32")
     if out is None:
         out = torch.empty(mx.rows, mx.cols, dtype=dtype, device=mx.data.device)
@@ -210,9 +215,11 @@ def gemm(a: MxTensor, weight: MxTensor, bias: Optional[torch.Tensor] = None, act
          valid_rows: Optional[torch.Tensor] = None,
          out: Union[torch.Tensor, MxTensor, None] = None) -> Union[torch.Tensor, MxTensor]:
     """act(A W + bias) (+ residual) on rows that are in MXFP4 already.  The result has the dtype of out, bias or
-    residual, or `dtype` (torch.float16 where nothing says); an MxTensor as out keeps it in 4 bits.  out may be residual."""
+    residual, or `dtype` (torch.float16 where nothing says); an MxTensor as out keeps it in 4 bits.  out may be residual;
+    it shares no memory with the other operands."""
     _require(isinstance(a, MxTensor) and isinstance(weight, MxTensor), "a and weight must be MxTensors")
-    _require(a.cols == weight.cols and a.device == weight.device, "a and weight must have one inner width and device")
+    _require(a.cols == weight.cols and a.device == weight.device >= 0,
+             "a and weight must have one inner width and be on one GPU")
     plain = isinstance(out, torch.Tensor)
     rows = out.shape[0] if plain else a.rows
     _require(rows <= a.rows, "out has more rows than a")
@@ -230,7 +237,8 @@ def linear(x: torch.Tensor, weight: MxTensor, bias: Optional[torch.Tensor] = Non
            workspace: Optional[MxTensor] = None,
            out: Union[torch.Tensor, MxTensor, None] = None) -> Union[torch.Tensor, MxTensor]:
     """gemm(quantize(x), weight, ...) in one call; the result has x's dtype.  `workspace`: an MxTensor of x's shape that
-    the call may use (a program that calls this in a loop keeps one per stream); few rows need none."""
+    the call may use (a program that calls this in a loop keeps one per stream); few rows need none.  out may be x or
+    residual; it shares no memory with the weight, the bias or the workspace."""
     rows, k, stride, device = _check_rows(x, "x")
     _require(isinstance(weight, MxTensor) and weight.cols == k and weight.device == device,
              "weight must be an MxTensor of x's width and device")

@@ -622,12 +622,13 @@ int et_mxfp4_pack_weight(int dtype, const void* w, void* w_mx, int k, int n, voi
  * made it, fp32 accumulation, one rounding at the end.  epilogue as for et_gemm (0 none, 1 +bias,
  * 2 gelu(+bias), 3 tanh(+bias)); residual [max_m, n] or NULL, may be c.  Exactly one of c [max_m, n]
  * and c_mx (the result as MXFP4, the operand of the next product: n a multiple of 64, no residual)
- * is given. */
+ * is given.  The result overlaps no operand but for that; nor do x and the MXFP4 tensor of the
+ * calls above. */
 int et_mxfp4_gemm(int dtype, const void* a_mx, const void* w_mx, const void* bias, const void* residual, void* c,
                   void* c_mx, const int* m_ptr, int max_m, int n, int k, int epilogue, int* status_word, void* stream);
 /* The same from x [max_m, k] (row_stride as for et_mxfp4_quantize), quantised on the way.  x_mx: workspace of
- * et_mxfp4_bytes(max_m, k) bytes, whose contents are unspecified afterwards (few rows are quantised inside the
- * product's kernel and do not use it). */
+ * et_mxfp4_bytes(max_m, k) bytes that overlaps nothing else, whose contents are unspecified afterwards (few rows are
+ * quantised inside the product's kernel and do not use it).  The result may overlap x. */
 int et_mxfp4_linear(int dtype, const void* x, long long row_stride, void* x_mx, const void* w_mx, const void* bias,
                     const void* residual, void* c, void* c_mx, const int* m_ptr, int max_m, int n, int k, int epilogue,
                     int* status_word, void* stream);
@@ -661,7 +662,7 @@ typedef struct {
   const void* pre_beta;
   void* h_out;            /* [max_m, n] or NULL; may be x or residual */
   void* y_out;            /* [max_m, n] or NULL; may be x or residual, not h_out */
-  void* y_mx;             /* MXFP4 tensor of max_m rows or NULL (n a multiple of 32) */
+  void* y_mx;             /* MXFP4 tensor of max_m rows or NULL (n a multiple of 32); overlaps nothing else */
   const int* m_ptr;       /* device row count, NULL = max_m */
   int max_m;
   int n;                  /* a multiple of 16 bytes, at most 8192 (ET_FP16) or 4096 (ET_FP32) */

@@ -127,6 +127,51 @@ def test_norm_refuses_types_and_null():
     refused(LIB.et_gated_residual_norm(0, C.byref(p), None), "limited")
 
 
+FAR = P + (1 << 30)
+
+
+@pytest.mark.parametrize("change", [
+    dict(c=None, c_mx=P), dict(c=P + 17408 - 16), dict(c=FAR + 16), dict(residual=FAR + (1 << 20) + 16, c=FAR + (1 << 20)),
+    dict(bias=FAR + (1 << 20) + 128, c=FAR + (1 << 20), epi=1), dict(c=None, c_mx=FAR)])
+def test_products_refuse_results_that_overlap_an_operand(change):
+    a = dict(dtype=1, a=P, w=FAR, bias=None, residual=None, c=FAR + (1 << 20), c_mx=None, m=3, n=64, k=64, epi=0)
+    a.update(change)
+    tail = (a["w"], a["bias"], a["residual"], a["c"], a["c_mx"], None, a["m"], a["n"], a["k"], a["epi"], None, None)
+    refused(LIB.et_mxfp4_gemm(a["dtype"], a["a"], *tail), "overlap")
+    refused(LIB.et_mxfp4_linear(a["dtype"], P + (1 << 20), 64, a["a"], *tail), "overlap")
+
+
+def test_rows_and_their_mxfp4_tensor_do_not_overlap():
+    refused(LIB.et_mxfp4_quantize(1, P, 96, None, 3, 64, P + 256, None), "overlap")          # (the third row's end)
+    refused(LIB.et_mxfp4_dequantize(0, P, None, 3, 64, P + 17408 - 16, None), "overlap")
+    refused(LIB.et_mxfp4_pack_weight(1, P, P, 64, 64, None), "overlap")
+    for x, w, bias, residual in ((P + 512, FAR, None, None), (FAR, P, None, None), (FAR, FAR, P, None),
+                                 (FAR, FAR, None, P)):
+        refused(LIB.et_mxfp4_linear(1, x, 64, P, w, bias, residual, FAR + (1 << 20), None, None, 3, 64, 64,
+                                    0 if bias is None else 1, None, None), "overlap")
+
+
+@pytest.mark.parametrize("change", [
+    dict(y_out=P), dict(h_out=P + 128), dict(y_out=P + 128), dict(y_mx=P), dict(y_mx=FAR, y_out=FAR),
+    dict(residual=FAR, h_out=FAR + 16), dict(bias=P + 16), dict(gate=P, gate_rows=1),
+    dict(gate=FAR, gate_rows=3, batch_idx=P), dict(pre_gamma=P, pre_beta=FAR, pre_norm=1)])
+def test_norm_refuses_outputs_that_overlap(change):
+    p = _capi.GatedNormParam()
+    p.x, p.h_out, p.max_m, p.n, p.residual_scale = P, P, 4, 64, 1.0
+    for k, v in change.items():
+        setattr(p, k, v)
+    refused(LIB.et_gated_residual_norm(1, C.byref(p), None), "overlap")
+
+
+def test_an_mxtensor_holds_what_it_says():
+    data = torch.zeros(17408, dtype=torch.uint8)
+    assert mxfp4.MxTensor(data, 128, 256).ptr == data.data_ptr()
+    for args in ((data, 129, 256), (data, 1, 288), (data, 1, 40), (data, -1, 64), (data.int(), 1, 64), (None, 1, 64),
+                 (torch.zeros(2 * 17408, dtype=torch.uint8)[::2], 1, 64)):
+        with pytest.raises(ValueError):
+            mxfp4.MxTensor(*args)
+
+
 def test_empty_batches_are_fine():
     assert LIB.et_mxfp4_quantize(1, None, 64, None, 0, 64, None, None) == 0
     assert LIB.et_mxfp4_dequantize(1, None, None, 0, 64, None, None) == 0

@@ -345,6 +345,21 @@ def test_other_streams_and_capture():
         assert ((out[:rows].double() - want[:rows]).abs() <= bound[:rows]).all() and (out[rows:] == 0).all()
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rows", [1, 32, 200])
+def test_linear_in_place(dtype, rows):
+    """out = x (and residual = x): every row has been quantised before a result is written."""
+    assert route(rows, 768, 768, DT[dtype])[2] == (rows < 100)
+    rng = np.random.RandomState(rows)
+    x, kernel = cuda(rows_of(rng, rows, 768, dtype)), cuda(rows_of(rng, 768, 768, dtype))
+    w = mxfp4.pack_weight(kernel)
+    for residual in (False, True):
+        want = mxfp4.linear(x, w, residual=x if residual else None)
+        y = x.clone()
+        got = mxfp4.linear(y, w, residual=y if residual else None, out=y)
+        assert got is y and torch.equal(got, want)
+
+
 def test_capture_needs_a_status_word_first():
     word = mxfp4._status.pop(torch.cuda.current_device(), None)
     try:
