@@ -80,7 +80,7 @@ __device__ __forceinline__ void store_mx(const Pair* v, void* y_mx, int row, int
 // Where a lane stands: its group, the group's warps, the lane's first vector of a row.
 struct Place {
   int group, wpr, wig, lane, vec0, vecs, turn;
-  float* red;  // [2][kMaxWarps][R] of the group, used in turn
+  float* red;  // [2][R][kMaxWarps] of the group, used in turn
 };
 
 // Sums of R values over the lanes of a group, to every lane: in a warp the R rows' shuffles are merged (a lane passes on
@@ -104,19 +104,21 @@ __device__ __forceinline__ void group_sum(float (&v)[R], Place& p) {
   for (; o >= 1; o >>= 1) v[0] += __shfl_xor_sync(0xffffffffu, v[0], o);
   float* slot = p.red + p.turn * kMaxWarps * R;
   p.turn ^= 1;
-  if ((p.lane & (lanes - 1)) == 0) slot[p.wig * R + row] = v[0];
+  if ((p.lane & (lanes - 1)) == 0) slot[row * kMaxWarps + p.wig] = v[0];
   if (p.wpr == 1) __syncwarp();
   else asm volatile("bar.sync %0, %1;" ::"r"(p.group + 1), "r"(p.wpr * 32) : "memory");
   // (slots of warps that the group does not have are zero)
 #pragma unroll
-  for (int r = 0; r < R; ++r) v[r] = slot[r];
+  for (int r = 0; r < R; ++r) {
+    const float4 f = *reinterpret_cast<const float4*>(slot + r * kMaxWarps);
+    v[r] = (f.x + f.y) + (f.z + f.w);
+  }
+  for (int i = 4; i < p.wpr; i += 4)
 #pragma unroll
-  for (int i = 1; i < 4; ++i)
-#pragma unroll
-    for (int r = 0; r < R; ++r) v[r] += slot[i * R + r];
-  for (int i = 4; i < p.wpr; ++i)
-#pragma unroll
-    for (int r = 0; r < R; ++r) v[r] += slot[i * R + r];
+    for (int r = 0; r < R; ++r) {
+      const float4 f = *reinterpret_cast<const float4*>(slot + r * kMaxWarps + i);
+      v[r] += (f.x + f.y) + (f.z + f.w);
+    }
 }
 
 // v := norm(v) of R rows; elements past the row's end are zero before and behind.  kFull: no lane has such elements.
@@ -178,7 +180,7 @@ template <typename T, int V, int R, bool kFull>
 __global__ void __maxnreg__(max_registers(sizeof(T), V))
 gated_norm_kernel(const GatedNorm p, int wpr) {
   constexpr int E = VecTraits<T>::kElems, P = E / 2;
-  __shared__ float red[kCtaWarps][2 * kMaxWarps * R];
+  __shared__ __align__(16) float red[kCtaWarps][2 * kMaxWarps * R];
   pdl_trigger();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int groups = static_cast<int>(blockDim.x >> 5) / wpr;
