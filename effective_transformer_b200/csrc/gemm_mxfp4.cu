@@ -818,7 +818,7 @@ cudaError_t launch_pair(const MxArgs& g, const T* bias, cudaStream_t stream) {
 // once.  Its 16 epilogue warps first quantise the tile's rows into the operand layout, while the producer fetches the W
 // rows; there is no second kernel to launch and no 4-bit copy of the rows in memory.  Every CTA of a row tile
 // quantises the same rows again, which is little work for few of them.  One row of 1024 through a 1024 x 4096
-// projection with GELU: 4.1 us on the device against 6.0 us for quantisation and product, and one launch (3 us of host
+// projection with GELU: 3.7 us on the device against 5.4 us for quantisation and product, and one launch (3 us of host
 // time) less.
 struct RowsCfg {
   static constexpr int BN = 64;
@@ -1094,8 +1094,8 @@ MxRoute mxfp4_route(bool fp32_result, int rows, int n, int k) {
   return !fp32_result && k >= 2048 && tiles > sm_count() ? kMxPair : kMxSingle;
 }
 // The kernel that quantises the rows itself pays while its tiles are one round of CTAs, K fits its shared memory and the
-// rows, which every CTA quantises again, are few: 128 pieces of 256 values.  1024 x 1024, 1 / 16 / 32 / 64 rows: 3.6 /
-// 4.2 / 5.6 / 8.0 us on the device, quantisation and product 5.3 / 5.6 / 5.7 / 5.7 us, and 3 us more on the host.
+// rows, which every CTA quantises again, are few: 128 pieces of 256 values.  1024 x 1024, 1 / 16 / 32 rows: 3.6 / 4.7 /
+// 5.9 us on the device (64 would take 8.0), quantisation and product 5.2 / 5.5 / 5.4 us, and 3 us more on the host.
 bool mxfp4_rows_supported(int rows, int n, int k) {
   return rows <= BM && mx_k_tiles(k) <= RowsCfg::kMaxKTiles && rows * mx_k_tiles(k) <= 128 &&
          (n + RowsCfg::BN - 1) / RowsCfg::BN <= sm_count();
