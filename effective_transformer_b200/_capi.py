@@ -131,7 +131,7 @@ SIGNATURES = {
     "et_mxfp4_gemm": (i32, [i32, vp, vp, vp, vp, vp, vp, vp, i32, i32, i32, i32, vp, vp]),
     "et_mxfp4_linear": (i32, [i32, vp, i64, vp, vp, vp, vp, vp, vp, vp, i32, i32, i32, i32, vp, vp]),
     "et_mxfp4_route": (i32, [i32, i32, i32, i32, ip, ip, ip]),
-    "et_gated_residual_norm": (i32, [i32, C.POINTER(GatedNormParam), vp]),
+    "et_gated_residual_norm": (i32, [i32, vp, vp]),  # (a GatedNormParam or its bytes)
     "et_gemm_fp32_tensor": (i32, [vp, vp, vp, vp, vp, vp, vp, i32, i32, i32, i32, vp, vp]),
 }
 

@@ -8,17 +8,17 @@ p = post(x + bias);  h = residual_scale * residual + gate * p;  y = pre(h)   (in
 """
 from __future__ import annotations
 
-import ctypes as C
+import struct
 from typing import Optional, Tuple
 
 import torch
 
-from . import _capi
 from .mxfp4 import MxTensor, _call, _check, _check_mx, _count, _DTYPE, _require
 
 __all__ = ["gated_residual_norm"]
 
 _KIND = {"none": 0, "layer": 1, "rms": 2}
+_PARAM = struct.Struct("@13P5i2f4x")  # _capi.GatedNormParam, put together in a third of the time
 
 
 def gated_residual_norm(x: torch.Tensor, bias: Optional[torch.Tensor] = None, residual: Optional[torch.Tensor] = None,
@@ -46,7 +46,7 @@ def gated_residual_norm(x: torch.Tensor, bias: Optional[torch.Tensor] = None, re
     post, pre = _KIND.get(post_norm), _KIND.get(pre_norm)
     if post is None or pre is None:
         raise ValueError("post_norm and pre_norm must be 'none', 'layer' or 'rms'")
-    bias_p = res_p = gate_p = idx_p = post_g = post_b = pre_g = pre_b = y_p = mx_p = None
+    bias_p = res_p = gate_p = idx_p = post_g = post_b = pre_g = pre_b = y_p = mx_p = 0
     if h_out is None:
         h_out = torch.empty_like(x)
     else:
@@ -94,8 +94,11 @@ def gated_residual_norm(x: torch.Tensor, bias: Optional[torch.Tensor] = None, re
     if mx_out is not None:
         _check_mx(mx_out, "mx_out", rows, n, device)
         mx_p = mx_out.ptr
-    p = _capi.GatedNormParam(x.data_ptr(), bias_p, res_p, gate_p, idx_p, post_g, post_b, pre_g, pre_b, h_p, y_p, mx_p,
-                             None if valid_rows is None else _count(valid_rows, device), rows, n, gate_rows, post, pre,
-                             residual_scale, eps)
-    _call(device, "et_gated_residual_norm", _DTYPE[dtype], C.byref(p))
+    try:
+        p = _PARAM.pack(x.data_ptr(), bias_p, res_p, gate_p, idx_p, post_g, post_b, pre_g, pre_b, h_p, y_p, mx_p,
+                        0 if valid_rows is None else _count(valid_rows, device), rows, n, gate_rows, post, pre,
+                        residual_scale, eps)
+    except (struct.error, OverflowError) as e:
+        raise ValueError("residual_scale and eps must be numbers that fp32 has, and sizes fit 32 bits") from e
+    _call(device, "et_gated_residual_norm", _DTYPE[dtype], p)
     return h_out, y_out

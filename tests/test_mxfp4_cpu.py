@@ -119,6 +119,13 @@ def test_norm_refusals(change, text):
     refused(LIB.et_gated_residual_norm(1, C.byref(p), None), text)
 
 
+def test_norm_parameters_as_bytes():
+    values = list(range(1, 14)) + [-3, 5, 7, 1, 2, 0.5, 1e-5]
+    p = _capi.GatedNormParam(*values)
+    assert norms._PARAM.pack(*values) == bytes(p) and norms._PARAM.size == C.sizeof(p)
+    refused(LIB.et_gated_residual_norm(1, norms._PARAM.pack(*([P] * 13 + [-1, 64, 0, 0, 0, 1.0, 0.0])), None), "negative")
+
+
 def test_norm_refuses_types_and_null():
     p = _capi.GatedNormParam()
     refused(LIB.et_gated_residual_norm(9, C.byref(p), None), "dtype")
