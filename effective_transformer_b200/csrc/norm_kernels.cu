@@ -13,12 +13,13 @@
 // side.  Means and variances are taken in two passes over the registers.  y can leave as MXFP4 too (mxfp4.cuh): four
 // (fp16) or eight (fp32) neighbouring lanes hold a scale block.
 //
-// 39778 rows of 1024 fp16 values with both norms and a gate: 70 us, 4.6 TB/s (328 MB; 50 us at the rate of a copy), 60 %
+// 39778 rows of 1024 fp16 values with both norms and a gate: 68 us, 4.8 TB/s (328 MB; 50 us at the rate of a copy), 60 %
 // of the issue slots at 16 warps an SM: the sums' shuffles and the conversions are what is left.  4099 rows of 2080 fp32
 // values with RMS norms: 32 us, 4.2 TB/s.  One row of 768: 2.1 us.  The first of these by layout, while it took 81 us:
 // one row to a warp with the parameters read from L1 for every row 118 us, from shared memory in fp32 88 us (128
 // registers, and what is fetched ahead spills), four warps to one row 154 us, to four rows 82 us without and 96 us with
-// fetching ahead.  Registers capped for more warps: spills, slower at every cap.
+// fetching ahead.  Registers capped for more warps: spills, slower at every cap.  Rows counted in 32 bits: 78 us instead of
+// 68 (and 34 of 32 in fp32), in the compiler's other order of the loads.
 #include "common.cuh"
 #include "mxfp4.cuh"
 #include "packed_f32.cuh"
@@ -87,8 +88,8 @@ struct Place {
 };
 
 // Sums of R values over the lanes of a group, to every lane: in a warp the R rows' shuffles are merged (a lane passes on
-// what its half of the warp is not to keep), between warps through shared memory.
-template <int R>
+// what its half of the warp is not to keep), between warps through shared memory.  kFew: at most four warps.
+template <int R, bool kFew>
 __device__ __forceinline__ void group_sum(float (&v)[R], Place& p) {
   int o = 16, row = 0;
 #pragma unroll
@@ -108,15 +109,14 @@ __device__ __forceinline__ void group_sum(float (&v)[R], Place& p) {
   float* slot = p.red + p.turn * kMaxWarps * R;
   p.turn ^= 1;
   if ((p.lane & (lanes - 1)) == 0) slot[row * kMaxWarps + p.wig] = v[0];
-  if (p.wpr == 1) __syncwarp();
-  else asm volatile("bar.sync %0, %1;" ::"r"(p.group + 1), "r"(p.wpr * 32) : "memory");
+  asm volatile("bar.sync %0, %1;" ::"r"(p.group + 1), "r"(p.wpr * 32) : "memory");
   // (slots of warps that the group does not have are zero)
 #pragma unroll
   for (int r = 0; r < R; ++r) {
     const float4 f = *reinterpret_cast<const float4*>(slot + r * kMaxWarps);
     v[r] = (f.x + f.y) + (f.z + f.w);
   }
-  for (int i = 4; i < p.wpr; i += 4)
+  for (int i = 4; !kFew && i < p.wpr; i += 4)
 #pragma unroll
     for (int r = 0; r < R; ++r) {
       const float4 f = *reinterpret_cast<const float4*>(slot + r * kMaxWarps + i);
@@ -125,7 +125,7 @@ __device__ __forceinline__ void group_sum(float (&v)[R], Place& p) {
 }
 
 // v := norm(v) of R rows; elements past the row's end are zero before and behind.  kFull: no lane has such elements.
-template <typename T, int V, int R, bool kFull>
+template <typename T, int V, int R, bool kFull, bool kFew>
 __device__ __forceinline__ void normalise(Pair (&v)[R][V][Pairs<T>::kCount], int kind, const Vec16 (&gamma)[V],
                                           const Vec16 (&beta)[V], float inv_n, float eps, Place& p) {
   constexpr int P = Pairs<T>::kCount;
@@ -141,7 +141,7 @@ __device__ __forceinline__ void normalise(Pair (&v)[R][V][Pairs<T>::kCount], int
           if (i + j > 0) a = add2(a, v[r][j][i]);
       s[r] = a.x + a.y;
     }
-    group_sum<R>(s, p);
+    group_sum<R, kFew>(s, p);
 #pragma unroll
     for (int j = 0; j < V; ++j) {
       const float inside = kFull || p.vec0 + j * 32 * p.wpr < p.vecs ? -inv_n : 0.f;
@@ -161,7 +161,7 @@ __device__ __forceinline__ void normalise(Pair (&v)[R][V][Pairs<T>::kCount], int
         if (i + j > 0) a = fma2(v[r][j][i], v[r][j][i], a);
     s[r] = a.x + a.y;
   }
-  group_sum<R>(s, p);
+  group_sum<R, kFew>(s, p);
 #pragma unroll
   for (int r = 0; r < R; ++r) s[r] = rsqrtf(fmaf(s[r], inv_n, eps));
 #pragma unroll
@@ -179,7 +179,7 @@ __device__ __forceinline__ void normalise(Pair (&v)[R][V][Pairs<T>::kCount], int
 // 128 for a CTA of 512 threads; fewer where that brings a second CTA of a wide fp32 row's nine warps to the SM.
 __host__ __device__ constexpr int max_registers(size_t elem, int v) { return elem == 4 && v == 2 ? 96 : 128; }
 
-template <typename T, int V, int R, bool kFull>
+template <typename T, int V, int R, bool kFull, bool kFew>
 __global__ void __maxnreg__(max_registers(sizeof(T), V))
 gated_norm_kernel(const GatedNorm p, int wpr) {
   constexpr int E = VecTraits<T>::kElems, P = E / 2;
@@ -282,7 +282,7 @@ gated_norm_kernel(const GatedNorm p, int wpr) {
       }
     }
     fetch(p.x, off + advance, row0 + stride, vx);
-    if (post_kind != kNormNone) normalise<T, V, R, kFull>(v, post_kind, pog, pob, inv_n, eps, at);
+    if (post_kind != kNormNone) normalise<T, V, R, kFull, kFew>(v, post_kind, pog, pob, inv_n, eps, at);
     if (gate != nullptr) {
 #pragma unroll
       for (int r = 0; r < R; ++r) {
@@ -324,7 +324,7 @@ gated_norm_kernel(const GatedNorm p, int wpr) {
           if (inside(j) && row0 + r < rows) st_global_v4(to + r * pitch + j * vec_bytes, Pairs<T>::pack(v[r][j]));
     };
     if (p.h != nullptr) store(p.h);
-    if (pre_kind != kNormNone) normalise<T, V, R, kFull>(v, pre_kind, prg, prb, inv_n, eps, at);
+    if (pre_kind != kNormNone) normalise<T, V, R, kFull, kFew>(v, pre_kind, prg, prb, inv_n, eps, at);
     if (p.y != nullptr) store(p.y);
     if (p.y_mx != nullptr) {
 #pragma unroll
@@ -337,9 +337,9 @@ gated_norm_kernel(const GatedNorm p, int wpr) {
   }
 }
 
-template <typename T, int V, int R, bool kFull>
+template <typename T, int V, int R, bool kFull, bool kFew>
 cudaError_t launch_full(const GatedNorm& p, int wpr, cudaStream_t stream) {
-  auto kernel = gated_norm_kernel<T, V, R, kFull>;
+  auto kernel = gated_norm_kernel<T, V, R, kFull, kFew>;
   const int groups = wpr >= kCtaWarps ? 1 : kCtaWarps / wpr, threads = groups * wpr * 32;
   static std::atomic<int> resident[kMaxDevices][kMaxWarps + 1] = {};
   const int dev = current_device();
@@ -356,10 +356,10 @@ cudaError_t launch_full(const GatedNorm& p, int wpr, cudaStream_t stream) {
   return launch_pdl(kernel, dim3(static_cast<int>(ctas)), dim3(threads), 0, stream, p, wpr);
 }
 
-template <typename T, int V, int R>
+template <typename T, int V, int R, bool kFew>
 cudaError_t launch_rows(const GatedNorm& p, int wpr, cudaStream_t stream) {
-  if (p.n == 32 * wpr * V * VecTraits<T>::kElems) return launch_full<T, V, R, true>(p, wpr, stream);
-  return launch_full<T, V, R, false>(p, wpr, stream);
+  if (p.n == 32 * wpr * V * VecTraits<T>::kElems) return launch_full<T, V, R, true, kFew>(p, wpr, stream);
+  return launch_full<T, V, R, false, kFew>(p, wpr, stream);
 }
 
 }  // namespace
@@ -385,8 +385,11 @@ cudaError_t launch_gated_norm(const GatedNorm& p, cudaStream_t stream) {
   if (wpr > kMaxWarps) return cudaErrorInvalidValue;
   // Few rows: one at a time, so that they spread over the SMs.  Two vectors a lane: one row, for the registers.
   const long long busy = static_cast<long long>(sm_count()) * (wpr >= kCtaWarps ? 1 : kCtaWarps / wpr);
-  if (v == 2) return launch_rows<T, 2, 1>(p, wpr, stream);
-  return p.max_m <= busy ? launch_rows<T, 1, 1>(p, wpr, stream) : launch_rows<T, 1, 2>(p, wpr, stream);
+  if (v == 2) return launch_rows<T, 2, 1, false>(p, wpr, stream);
+  // (up to four warps to a row: without the loop over the further slots, 67.8 us instead of 70.3 at 39778 x 1024 fp16)
+  if (wpr <= 4)
+    return p.max_m <= busy ? launch_rows<T, 1, 1, true>(p, wpr, stream) : launch_rows<T, 1, 2, true>(p, wpr, stream);
+  return p.max_m <= busy ? launch_rows<T, 1, 1, false>(p, wpr, stream) : launch_rows<T, 1, 2, false>(p, wpr, stream);
 }
 
 template cudaError_t launch_gated_norm<__half>(const GatedNorm&, cudaStream_t);
