@@ -360,6 +360,33 @@ def test_linear_in_place(dtype, rows):
         assert got is y and torch.equal(got, want)
 
 
+def test_calls_on_two_streams_at_once():
+    """Products of all three kernels, rows and norms on two streams, each with its own buffers: what one call alone gives.
+    (They share the weights, the status word and the SMs' tensor memory.)"""
+    rng = np.random.RandomState(8)
+    shapes = [(5000, 768, 2304), (300, 768, 768), (9, 256, 512), (2, 1024, 1024), (4200, 2048, 1088)]
+    jobs = []
+    for m, k, n in shapes:
+        x = cuda(rows_of(rng, m, k, torch.float16))
+        w = mxfp4.pack_weight(cuda(rows_of(rng, k, n, torch.float16)))
+        jobs.append((x, w, mxfp4.linear(x, w)))
+    side = [torch.cuda.Stream(), torch.cuda.Stream()]
+    got = [[], []]
+    torch.cuda.synchronize()
+    for turn in range(6):
+        for s, stream in enumerate(side):
+            with torch.cuda.stream(stream):
+                x, w, _ = jobs[(turn + 2 * s) % len(jobs)]
+                got[s].append(((turn + 2 * s) % len(jobs), mxfp4.linear(x, w), mxfp4.dequantize(mxfp4.quantize(x), x.dtype)))
+    torch.cuda.synchronize()
+    for results in got:
+        for i, y, back in results:
+            x, _, want = jobs[i]
+            assert torch.equal(y, want)
+            assert torch.equal(back, mxfp4.dequantize(mxfp4.quantize(x), x.dtype))
+    assert mxfp4.device_status() == 0
+
+
 def test_capture_needs_a_status_word_first():
     word = mxfp4._status.pop(torch.cuda.current_device(), None)
     try:
