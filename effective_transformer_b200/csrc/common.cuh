@@ -558,6 +558,7 @@ struct GatedNorm {
   void *h = nullptr, *y = nullptr, *y_mx = nullptr;
   const int* m_ptr = nullptr;
   int max_m = 0, n = 0;
+  int route_rows = 0;  // rows by which the kernel is chosen, 0 = max_m
 };
 template <typename T>
 cudaError_t launch_gated_norm(const GatedNorm& p, cudaStream_t stream);

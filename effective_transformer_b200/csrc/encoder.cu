@@ -593,6 +593,7 @@ int run_layer_mx(et_handle_t h, const LayerWeights& lw, const T* x_in, T* x_out,
     g.y = y;
     g.y_mx = mx ? ws.x_mx : nullptr;
     g.m_ptr = t_ptr, g.max_m = max_m, g.n = hid;
+    g.route_rows = h->route_rows;
     return launch_gated_norm<T>(g, s);
   };
   if (in_mx)

@@ -176,11 +176,9 @@ __device__ __forceinline__ void normalise(Pair (&v)[R][V][Pairs<T>::kCount], int
   }
 }
 
-// 128 for a CTA of 512 threads; fewer where that brings a second CTA of a wide fp32 row's nine warps to the SM.
-__host__ __device__ constexpr int max_registers(size_t elem, int v) { return elem == 4 && v == 2 ? 96 : 128; }
-
-template <typename T, int V, int R, bool kFull, bool kFew>
-__global__ void __maxnreg__(max_registers(sizeof(T), V))
+// kRegs: 128, which a CTA of 512 threads may have, or 96.
+template <typename T, int V, int R, bool kFull, bool kFew, int kRegs>
+__global__ void __maxnreg__(kRegs)
 gated_norm_kernel(const GatedNorm p, int wpr) {
   constexpr int E = VecTraits<T>::kElems, P = E / 2;
   __shared__ __align__(16) float red[kCtaWarps][2 * kMaxWarps * R];
@@ -337,9 +335,9 @@ gated_norm_kernel(const GatedNorm p, int wpr) {
   }
 }
 
-template <typename T, int V, int R, bool kFull, bool kFew>
+template <typename T, int V, int R, bool kFull, bool kFew, int kRegs>
 cudaError_t launch_full(const GatedNorm& p, int wpr, cudaStream_t stream) {
-  auto kernel = gated_norm_kernel<T, V, R, kFull, kFew>;
+  auto kernel = gated_norm_kernel<T, V, R, kFull, kFew, kRegs>;
   const int groups = wpr >= kCtaWarps ? 1 : kCtaWarps / wpr, threads = groups * wpr * 32;
   static std::atomic<int> resident[kMaxDevices][kMaxWarps + 1] = {};
   const int dev = current_device();
@@ -356,10 +354,10 @@ cudaError_t launch_full(const GatedNorm& p, int wpr, cudaStream_t stream) {
   return launch_pdl(kernel, dim3(static_cast<int>(ctas)), dim3(threads), 0, stream, p, wpr);
 }
 
-template <typename T, int V, int R, bool kFew>
+template <typename T, int V, int R, bool kFew, int kRegs = 128>
 cudaError_t launch_rows(const GatedNorm& p, int wpr, cudaStream_t stream) {
-  if (p.n == 32 * wpr * V * VecTraits<T>::kElems) return launch_full<T, V, R, true, kFew>(p, wpr, stream);
-  return launch_full<T, V, R, false, kFew>(p, wpr, stream);
+  if (p.n == 32 * wpr * V * VecTraits<T>::kElems) return launch_full<T, V, R, true, kFew, kRegs>(p, wpr, stream);
+  return launch_full<T, V, R, false, kFew, kRegs>(p, wpr, stream);
 }
 
 }  // namespace
@@ -381,15 +379,27 @@ cudaError_t launch_gated_norm(const GatedNorm& p, cudaStream_t stream) {
     if (reinterpret_cast<uintptr_t>(q) & 15u) return cudaErrorMisalignedAddress;
   if (reinterpret_cast<uintptr_t>(p.y_mx) & 127u) return cudaErrorMisalignedAddress;
   const int vecs = p.n / E;
-  const int v = vecs <= 32 * kMaxWarps ? 1 : 2, wpr = (vecs + 32 * v - 1) / (32 * v);
+  int wpr = (vecs + 31) / 32;
+  // Few rows: one at a time, so that they spread over the SMs.
+  const int route = p.route_rows > 0 ? p.route_rows : p.max_m;
+  const bool few_rows = route <= static_cast<long long>(sm_count()) * (wpr >= kCtaWarps ? 1 : kCtaWarps / wpr);
+  // One vector a lane and two rows at a time, where 16 warps hold the row; but fp32 rows of eight warps and more leave
+  // too few registers for two rows: 13000 rows of 1024 / 1536 / 2048, 47.9 / 61.1 / 107.6 us, and with two vectors a
+  // lane 41.9 / 53.6 / 86.3.  (640, where they do not come out even, 27.4 and 32.1; fp16, 4096: 126 and 152.)
+  if (wpr <= kMaxWarps && (sizeof(T) == 2 || wpr < 8 || few_rows)) {
+    // (up to four warps to a row: without the loop over the further slots, 67.8 us instead of 70.3 at 39778 x 1024 fp16)
+    if (wpr <= 4) return few_rows ? launch_rows<T, 1, 1, true>(p, wpr, stream) : launch_rows<T, 1, 2, true>(p, wpr, stream);
+    return few_rows ? launch_rows<T, 1, 1, false>(p, wpr, stream) : launch_rows<T, 1, 2, false>(p, wpr, stream);
+  }
+  wpr = (vecs + 63) / 64;
   if (wpr > kMaxWarps) return cudaErrorInvalidValue;
-  // Few rows: one at a time, so that they spread over the SMs.  Two vectors a lane: one row, for the registers.
-  const long long busy = static_cast<long long>(sm_count()) * (wpr >= kCtaWarps ? 1 : kCtaWarps / wpr);
-  if (v == 2) return launch_rows<T, 2, 1, false>(p, wpr, stream);
-  // (up to four warps to a row: without the loop over the further slots, 67.8 us instead of 70.3 at 39778 x 1024 fp16)
-  if (wpr <= 4)
-    return p.max_m <= busy ? launch_rows<T, 1, 1, true>(p, wpr, stream) : launch_rows<T, 1, 2, true>(p, wpr, stream);
-  return p.max_m <= busy ? launch_rows<T, 1, 1, false>(p, wpr, stream) : launch_rows<T, 1, 2, false>(p, wpr, stream);
+  if constexpr (sizeof(T) == 4)
+    if (wpr <= 4) return launch_rows<T, 2, 1, true>(p, wpr, stream);
+  // Two vectors a lane spill a little with 96 registers, which pays where it brings one more CTA to an SM: 6699 rows of
+  // 2080 (9 warps) 49 us instead of 70, but 4096 (16 warps) 116 us instead of 98, 13000 of 2048 (8 warps) 97 instead of 86.
+  constexpr int kFile = 65536 / 32;
+  if (kFile / (wpr * 96) > kFile / (wpr * 128)) return launch_rows<T, 2, 1, false, 96>(p, wpr, stream);
+  return launch_rows<T, 2, 1, false>(p, wpr, stream);
 }
 
 template cudaError_t launch_gated_norm<__half>(const GatedNorm&, cudaStream_t);

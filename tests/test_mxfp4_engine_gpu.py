@@ -163,3 +163,15 @@ def test_toggling_drops_recorded_graphs():
     with pytest.raises(et.EtError):
         eng.replay()
     eng.close()
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_chunks_of_a_host_call_run_the_whole_batchs_kernels(dtype):
+    """A chunk has few rows where the batch has many: neither a product nor a norm may take another order of sums."""
+    eng, _, x, mask = make(dtype, 16, 24, layers=1, heads=16, ffn=256, seed=11)
+    eng.set_mxfp4_projections(True)
+    want = eng.forward(x, mask).cpu().numpy()
+    for _ in range(3):
+        host, t = eng.forward_host(x.cpu().numpy(), mask.cpu().numpy())
+        assert t == int(mask.sum()) and np.array_equal(host, want)
+    eng.close()

@@ -54,6 +54,22 @@ def test_norms(dtype, rows, n, post, pre):
     close(y, wy, wh, dtype)
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rows,n", [(601, 96), (400, 512), (301, 760), (333, 1024), (299, 1000), (301, 1536), (310, 2048),
+                                    (170, 2600), (160, 4096)])
+def test_norms_of_many_rows(dtype, rows, n):
+    """More rows than one to a CTA: two rows at a time or two vectors a lane, rounds of the grid, rows past the count."""
+    a = make(rows + n, rows, n, dtype, seqs=7)
+    h, y = torch.full_like(a["x"], 3.0), torch.full_like(a["x"], 3.0)
+    valid = torch.full((1,), rows - 5, dtype=torch.int32, device="cuda")
+    norms.gated_residual_norm(**a, post_norm="layer", pre_norm="rms", residual_scale=0.75, valid_rows=valid, h_out=h,
+                              y_out=y)
+    wh, wy = want_of(a, "layer", "rms", 0.75)
+    close(h[:-5], wh[:-5], wh[:-5], dtype)
+    close(y[:-5], wy[:-5], wh[:-5], dtype)
+    assert (h[-5:] == 3.0).all() and (y[-5:] == 3.0).all()
+
+
 @pytest.mark.parametrize("n", [8192, 5000, 8184])
 def test_widest_fp16_rows(n):
     a = make(n, 6, n, torch.float16)
