@@ -8,10 +8,10 @@
 //
 // Everything between the loads of x and residual and the stores of h and y stays in fp32 registers, so x and residual
 // are read once and h and y written once: the kernel is bound by those bytes once it spends few enough instructions.  A
-// group of warps (at most 16) takes R rows at a time; a lane holds V vectors of 16 bytes of each, 1 where the row allows
-// it.  So bias, gamma and beta stay in registers for all rows, and the R rows' sums go through their shuffles side by
-// side.  Means and variances are taken in two passes over the registers.  y can leave as MXFP4 too (mxfp4.cuh): four
-// (fp16) or eight (fp32) neighbouring lanes hold a scale block.
+// group of warps (at most 16) takes R rows at a time; a lane holds V vectors of 16 bytes of each, 1 or 2
+// (launch_gated_norm has the rule).  So bias, gamma and beta stay in registers for all rows, and the R rows' sums go
+// through their shuffles side by side.  Means and variances are taken in two passes over the registers.  y can leave as
+// MXFP4 too (mxfp4.cuh): four (fp16) or eight (fp32) neighbouring lanes hold a scale block.
 //
 // 39778 rows of 1024 fp16 values with both norms and a gate: 68 us, 4.8 TB/s (328 MB; 50 us at the rate of a copy), 60 %
 // of the issue slots at 16 warps an SM: the sums' shuffles and the conversions are what is left.  4099 rows of 2080 fp32
