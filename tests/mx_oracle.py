@@ -81,3 +81,30 @@ def gated_norm(x, bias, residual, scale, gate, batch_idx, post, post_gamma, post
             p = p * g.reshape(-1)
     h = p if residual is None else p + scale * residual.double()
     return h, norm(h, pre, pre_gamma, pre_beta, eps)
+
+
+def code_values(v, scales):
+    """v [rows, k] rounded to codes on given scale bytes [rows, k / 32], as values."""
+    s = np.exp2(scales.astype(np.float64) - 127).repeat(32, axis=1)
+    q = np.abs(v) / s
+    c = np.zeros(q.shape, np.int8)
+    for i in range(7):
+        mid = (GRID[i] + GRID[i + 1]) / 2
+        c += (q > mid) if i % 2 == 0 else (q >= mid)
+    return np.copysign(GRID[c], v) * s
+
+
+def check_codes(mx, want, bound):
+    """The first rows of mx (an MxTensor on a GPU) hold the quantised form of values within `bound` of `want` (float64,
+    on the GPU): scales and codes agree with those of `want` but where a border lies in between."""
+    rows, k = want.shape
+    codes, scales = (part[:rows] for part in mx_unpack(mx.data.cpu().numpy(), mx.rows, k))
+    got = GRID[codes & 7] * np.where(codes & 8, -1.0, 1.0) * np.exp2(scales.astype(np.float64) - 127).repeat(32, axis=1)
+    want, bound = want.cpu().numpy(), bound.cpu().numpy()
+    lo, hi = want - bound, want + bound
+    size = np.abs(want)
+    top_lo = np.maximum(size - bound, 1e-30).reshape(rows, -1, 32).max(-1)
+    top_hi = (size + bound).reshape(rows, -1, 32).max(-1)
+    e = scales.astype(np.float64) - 127 + 2
+    assert (np.floor(np.log2(top_lo)) <= e).all() and (e <= np.floor(np.log2(top_hi))).all()
+    assert (got >= code_values(lo, scales)).all() and (got <= code_values(hi, scales)).all()

@@ -70,6 +70,112 @@ def test_norms_of_many_rows(dtype, rows, n):
     assert (h[-5:] == 3.0).all() and (y[-5:] == 3.0).all()
 
 
+# (dtype, rows, width, rows of one round of the grid at the most: SMs x CTAs that 64 K registers hold x rows of a CTA)
+F16, F32 = DTYPES
+ROUNDS = [(F16, 12003, 96, 148 * 4 * 8), (F16, 12003, 256, 148 * 4 * 8), (F16, 7001, 512, 148 * 4 * 4),
+          (F16, 4099, 760, 148 * 5 * 2), (F16, 5003, 1024, 148 * 4 * 2), (F16, 3001, 1536, 148 * 2 * 2),
+          (F16, 2999, 1000, 148 * 4 * 2), (F16, 1501, 4096, 148 * 1 * 2), (F16, 1203, 4608, 148 * 2), (F16, 1203, 5120, 148 * 2),
+          (F16, 701, 5768, 148), (F16, 701, 8192, 148),
+          (F32, 12003, 96, 148 * 4 * 8), (F32, 7001, 256, 148 * 4 * 4), (F32, 4099, 640, 148 * 3 * 2),
+          (F32, 4099, 896, 148 * 2 * 2), (F32, 5003, 1024, 148 * 4), (F32, 3001, 1280, 148 * 4), (F32, 3001, 1536, 148 * 3),
+          (F32, 3001, 1792, 148 * 3), (F32, 2001, 2048, 148 * 2), (F32, 2001, 2080, 148 * 2), (F32, 2001, 2560, 148 * 2),
+          (F32, 1003, 2688, 148), (F32, 1003, 4096, 148)]
+
+
+@pytest.mark.parametrize("dtype,rows,n,one_round", ROUNDS)
+def test_rounds_of_the_grid(dtype, rows, n, one_round):
+    """More rows than the grid holds at once, several times over: what a lane fetches ahead for its next rows, the last
+    round's rows of which one or none is there, and every number of warps to a row, with the gate found through
+    batch_idx two rounds ahead."""
+    assert rows > 2 * one_round and rows % 2 == 1
+    a = make(rows + n, rows, n, dtype, seqs=37)
+    a["batch_idx"] = a["batch_idx"][torch.randperm(rows, device="cuda")].contiguous()
+    valid_rows = rows - 6
+    valid = torch.full((1,), valid_rows, dtype=torch.int32, device="cuda")
+    wh, wy = want_of(a, "layer", "rms", 0.75)
+    h, y = torch.full_like(a["x"], 3.0), torch.full_like(a["x"], 3.0)
+    norms.gated_residual_norm(**a, post_norm="layer", pre_norm="rms", residual_scale=0.75, valid_rows=valid, h_out=h,
+                              y_out=y)
+    close(h[:valid_rows], wh[:valid_rows], wh[:valid_rows], dtype)
+    close(y[:valid_rows], wy[:valid_rows], wh[:valid_rows], dtype)
+    assert (h[valid_rows:] == 3.0).all() and (y[valid_rows:] == 3.0).all()
+    # over its own inputs: what is fetched ahead is not what has just been written
+    norms.gated_residual_norm(**a, post_norm="layer", pre_norm="rms", residual_scale=0.75, h_out=a["x"],
+                              y_out=a["residual"])
+    assert torch.equal(a["x"][:valid_rows], h[:valid_rows]) and torch.equal(a["residual"][:valid_rows], y[:valid_rows])
+    close(a["x"], wh, wh, dtype)
+    close(a["residual"], wy, wh, dtype)
+
+
+@pytest.mark.parametrize("dtype,rows,n", [
+    (F16, 700, 96), (F16, 333, 1024), (F16, 301, 1536), (F16, 12003, 96), (F16, 5003, 1024), (F16, 1501, 4096),
+    (F16, 1203, 5120), (F16, 701, 8192), (F32, 700, 96), (F32, 333, 1024), (F32, 301, 1536), (F32, 4099, 608),
+    (F32, 5003, 1024), (F32, 2001, 2080), (F32, 1003, 4096)])
+def test_quantized_rows_of_a_batch(dtype, rows, n):
+    """y in 4 bits of many rows against the codes of float64: they agree but where a value lies within the fp32 error
+    (1e-5 of the row's size, as above) of a border."""
+    a = make(rows + n, rows, n, dtype, seqs=5)
+    valid_rows = rows - 3
+    valid = torch.full((1,), valid_rows, dtype=torch.int32, device="cuda")
+    mx = mxfp4.empty(rows, n)
+    mx.data.fill_(0xEE)
+    y_out = torch.full_like(a["x"], 3.0)
+    h, _ = norms.gated_residual_norm(**a, post_norm="rms", pre_norm="layer", valid_rows=valid, y_out=y_out, mx_out=mx)
+    wh, wy = want_of(a, "rms", "layer")
+    close(h[:valid_rows], wh[:valid_rows], wh[:valid_rows], dtype)
+    close(y_out[:valid_rows], wy[:valid_rows], wh[:valid_rows], dtype)
+    size = torch.maximum(wy.abs(), wh.abs()).amax(-1, keepdim=True) + 1.0
+    X.check_codes(mx, wy[:valid_rows], (1e-5 * size).expand_as(wy)[:valid_rows])
+    codes, scales = X.mx_unpack(mx.data.cpu().numpy(), rows, n)
+    assert (scales[valid_rows:] == 0xEE).all() and (codes[valid_rows:] == 0xE).all() and (y_out[valid_rows:] == 3.0).all()
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_norm_and_product_repeat_bit_by_bit(dtype):
+    """The rows that a norm leaves in 4 bits and the product behind it, over and over on buffers full of other values."""
+    a = make(77, 5003, 1024, dtype)
+    w = mxfp4.pack_weight(torch.randn(1024, 1088, device="cuda").to(dtype))
+    mx, out = mxfp4.empty(5003, 1024), torch.empty(5003, 1088, dtype=dtype, device="cuda")
+    first = None
+    for turn in range(12):
+        mx.data.fill_(0x11 * turn)
+        out.fill_(float("nan"))
+        h, _ = norms.gated_residual_norm(**a, post_norm="none", pre_norm="layer", mx_out=mx)
+        mxfp4.gemm(mx, w, out=out)
+        got = (h, mxfp4.dequantize(mx, torch.float32), out.clone())
+        first = first or got
+        assert all(torch.equal(u, v) for u, v in zip(got, first))
+
+
+def test_norms_on_two_streams_at_once():
+    """Norms, their 4-bit rows and the products behind them on two streams, each with its own buffers: what one call
+    alone gives."""
+    shapes = [(5003, 1024), (40, 768), (1501, 4096), (2, 1024)]
+    jobs = []
+    for rows, n in shapes:
+        a = make(rows + n, rows, n, torch.float16, seqs=3)
+        w = mxfp4.pack_weight(torch.randn(n, 576, device="cuda").half())
+
+        def chain(a=a, w=w, rows=rows, n=n):
+            mx = mxfp4.empty(rows, n)
+            h, _ = norms.gated_residual_norm(**a, post_norm="layer", mx_out=mx)
+            return h, mxfp4.gemm(mx, w)
+
+        jobs.append((chain, chain()))
+    side = [torch.cuda.Stream(), torch.cuda.Stream()]
+    torch.cuda.synchronize()
+    got = []
+    for turn in range(8):
+        for s, stream in enumerate(side):
+            with torch.cuda.stream(stream):
+                i = (turn + s) % len(jobs)
+                got.append((i, jobs[i][0]()))
+    torch.cuda.synchronize()
+    for i, results in got:
+        assert all(torch.equal(u, v) for u, v in zip(results, jobs[i][1]))
+    assert mxfp4.device_status() == 0
+
+
 @pytest.mark.parametrize("n", [8192, 5000, 8184])
 def test_widest_fp16_rows(n):
     a = make(n, 6, n, torch.float16)
