@@ -56,23 +56,28 @@ struct MxArgs {
 // Rows as MXFP4 instead of T.
 struct MxOut {};
 
-// tanh-form GELU of a pair whose result is rounded to fp16 or to 4 bits: 0.5 x (1 + tanh u) with the hardware's
-// tanh (relative error 2^-11, so at most 0.5 |x| 2^-11 here, the size of the fp16 rounding behind it; in 4 bits a
-// sixteenth of half a step at the least).  One special-function operation an element where exp and a reciprocal
-// would be two: those alone take 36 us of a 39778 x 4096 result.
-__device__ __forceinline__ Pair gelu_rough(const Pair& x) {
-  const Pair c1 = pack2(0.7978845608028654f, 0.7978845608028654f);
-  const Pair c2 = pack2(0.7978845608028654f * 0.044715f, 0.7978845608028654f * 0.044715f);
-  Pair t = mul2(x, fma2(mul2(x, x), c2, c1));
-  asm("tanh.approx.f32 %0, %0;" : "+f"(t.x));
-  asm("tanh.approx.f32 %0, %0;" : "+f"(t.y));
-  const Pair h = mul2(x, pack2(0.5f, 0.5f));
-  return fma2(h, t, h);
+// tanh-form GELU of a pair, 0.5 x (1 + tanh u) as x / (1 + 2^z) with z = -2 u log2(e): nothing cancels for negative x, where
+// 1 + tanh u does (with the hardware's tanh, right to 2^-11, the result at x = -3 would be off by a fifth of itself).  z is
+// rounded four times, so the relative error is 4 |z| 2^-24 ln 2 at the most, 7e-6 at x = -6; 2^z overflows from x = -10 on
+// and leaves -0, the limit.  Two special-function operations an element instead of tanh's one: 39778 x 1024 by 4096 103 ->
+// 116 us in fp16, 98 -> 117 us in 4 bits (without activation 93 us).  One reciprocal for both elements, of the product of
+// their denominators, takes clamps that keep a NaN from its neighbour and comes to 114 and 119 us; a polynomial and a Newton
+// step in place of the reciprocal 122 and 133 us.
+__device__ __forceinline__ Pair gelu_pair(const Pair& x) {
+  const Pair c1 = pack2(-2.302208198144325f, -2.302208198144325f);
+  const Pair c2 = pack2(-2.302208198144325f * 0.044715f, -2.302208198144325f * 0.044715f);
+  Pair d = mul2(x, fma2(mul2(x, x), c2, c1));
+  asm("ex2.approx.ftz.f32 %0, %0;" : "+f"(d.x));
+  asm("ex2.approx.ftz.f32 %0, %0;" : "+f"(d.y));
+  d = add2(d, pack2(1.f, 1.f));
+  asm("rcp.approx.ftz.f32 %0, %0;" : "+f"(d.x));
+  asm("rcp.approx.ftz.f32 %0, %0;" : "+f"(d.y));
+  return mul2(x, d);
 }
 
-template <int ACT, bool kRough>
+template <int ACT>
 __device__ __forceinline__ Pair activate(const Pair& x) {
-  if (ACT == kEpiBiasGelu) return kRough ? gelu_rough(x) : pack2(gelu_tanh(x.x), gelu_tanh(x.y));
+  if (ACT == kEpiBiasGelu) return gelu_pair(x);
   if (ACT == kEpiBiasTanh) return pack2(tanhf(x.x), tanhf(x.y));
   return x;
 }
@@ -186,7 +191,7 @@ struct Group {
         for (int j = 0; j < 4; ++j) f[j] = add2(f[j], b[j]);
       }
 #pragma unroll
-      for (int j = 0; j < 4; ++j) f[j] = activate<ACT, sizeof(T) == 2>(f[j]);
+      for (int j = 0; j < 4; ++j) f[j] = activate<ACT>(f[j]);
       if (kRes) {
         Pair x[4];
         res[i].unpack(x);
@@ -236,7 +241,7 @@ struct Group<T, MxOut, ACT> {
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         Pair& v = f[4 * i + j];
-        v = activate<ACT, true>(v);
+        v = activate<ACT>(v);
         asm("max.NaN.f32 %0, %0, %1, %2;" : "+f"(top) : "f"(fabsf(v.x)), "f"(fabsf(v.y)));
       }
     }

@@ -283,6 +283,64 @@ def test_product_in_4_bits(m, k, n, act):
     assert (got >= code_values(lo)).all() and (got <= code_values(hi)).all()
 
 
+# From few rows to CTA pairs: one kernel, tiles of 128 x 128, tiles of 256 x 192 (k >= 768 and three rounds of tiles).
+GELU_SHAPES = [(3, 64, 1), (300, 64, 0), (8000, 768, 0)]
+
+
+def gelu_bias(n, dtype, low, high):
+    """Pre-activations: rows of zeros leave the bias alone."""
+    return torch.linspace(low, high, n, dtype=torch.float64, device="cuda").to(dtype)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("m,k,one", GELU_SHAPES)
+def test_gelu_holds_its_precision_in_the_negative_tail(dtype, m, k, one):
+    """Relative to the result, not to x: for negative x the two terms of 0.5 x (1 + tanh u) cancel.
+
+    The product is exactly zero, so the pre-activation is the bias.  x / (1 + exp(-2u)) in fp32: the argument of the
+    exponential is below 37 for |x| <= 6 (as a power of two) and rounded four times, each 2^-24 of it, times ln 2; the
+    exponential, the reciprocal and two products add less than eight steps of 2^-23 between them: 7.1e-6 in all."""
+    n = 1024
+    assert route(m, n, k, DT[dtype])[2] == one and (m != 8000 or route(m, n, k, DT[dtype])[0] == 256)
+    bias = gelu_bias(n, dtype, -6.0, 6.0)
+    x = torch.zeros(m, k, dtype=dtype, device="cuda")
+    got = mxfp4.linear(x, mxfp4.pack_weight(torch.ones(k, n, dtype=dtype, device="cuda")), bias=bias, activation="gelu")
+    want = X.gelu(bias.double()).expand(m, n)
+    half_step = (2.0 ** -11 if dtype == torch.float16 else 2.0 ** -24) * want.abs()
+    subnormal = 2.0 ** -25 if dtype == torch.float16 else 0.0
+    assert ((got.double() - want).abs() <= (half_step + 7.5e-6 * want.abs()).clamp(min=subnormal) * (1 + 1e-5)).all()
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("m,k,one", GELU_SHAPES)
+def test_gelu_in_4_bits_in_the_negative_tail(dtype, m, k, one):
+    """Whole scale blocks of negative pre-activations: codes and scales of the float64 values, but where a value is
+    within the fp32 error above of a border."""
+    n = 1024
+    bias = gelu_bias(n, dtype, -6.0, -0.05)
+    x = torch.zeros(m, k, dtype=dtype, device="cuda")
+    w = mxfp4.pack_weight(torch.ones(k, n, dtype=dtype, device="cuda"))
+    out = mxfp4.linear(x, w, bias=bias, activation="gelu", out=mxfp4.empty(m, n))
+    want = X.gelu(bias.double())[None, :].cpu().numpy()
+    lo, hi = (X.mx_values(want * (1 + s * 7.5e-6)) for s in (1, -1))     # (negative: the larger magnitude is lower)
+    got = mxfp4.dequantize(out, torch.float32).double().cpu().numpy()
+    assert (got >= lo).all() and (got <= hi).all()
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_gelu_far_out(dtype):
+    """Nothing is left of large negative values, all of large positive ones."""
+    far = torch.tensor([-65000.0, -1000.0, -40.0, -20.0, 20.0, 40.0, 1000.0, 65000.0], device="cuda")
+    if dtype == torch.float32:
+        far = torch.cat([far, torch.tensor([-3e38, -1e20, 1e20, 3e38], device="cuda")])
+    bias = torch.zeros(64, dtype=dtype, device="cuda")
+    bias[:len(far)] = far.to(dtype)
+    x = torch.zeros(5, 64, dtype=dtype, device="cuda")
+    w = mxfp4.pack_weight(torch.ones(64, 64, dtype=dtype, device="cuda"))
+    got = mxfp4.linear(x, w, bias=bias, activation="gelu")
+    assert torch.equal(got, torch.where(bias > 0, bias, torch.zeros_like(bias)).expand(5, 64))
+
+
 @pytest.mark.parametrize("dtype", DTYPES)
 def test_rows_past_the_count_are_left_alone(dtype):
     x, kernel, bias, _, (want, bound) = product_case(23, 400, 288, 224, dtype, None, True, False)
