@@ -341,6 +341,29 @@ def test_gelu_far_out(dtype):
     assert torch.equal(got, torch.where(bias > 0, bias, torch.zeros_like(bias)).expand(5, 64))
 
 
+@pytest.mark.parametrize("act", [None, "gelu"])
+@pytest.mark.parametrize("m,k,n", [(77, 768, 320), (300, 512, 1024), (5001, 2080, 1856), (9001, 1024, 1088)])
+def test_product_in_4_bits_of_an_fp32_program(m, k, n, act):
+    """test_product_in_4_bits with bias and rows in fp32: on the last two sizes the CTA-pair kernel that the first
+    feed-forward projection of an fp32 handle runs on a full batch."""
+    if m > 5000:
+        assert route(m, n, k) == (256, 192, 0)
+    x, kernel, bias, _, _ = product_case(6, m, k, n, torch.float32, None, True, False)
+    w = mxfp4.pack_weight(cuda(kernel))
+    out = mxfp4.gemm(mxfp4.quantize(cuda(x)), w, bias=bias, activation=act, out=mxfp4.empty(m, n))
+    want, bound = reference(x, kernel, bias, act, None, torch.float32, rough=True)
+    X.check_codes(out, want, bound)
+    same = mxfp4.linear(cuda(x), w, bias=bias, activation=act, out=mxfp4.empty(m, n))
+    assert torch.equal(mxfp4.dequantize(same, torch.float32), mxfp4.dequantize(out, torch.float32))
+    valid = m - 70
+    part = mxfp4.empty(m, n)
+    part.data.fill_(0xCD)
+    mxfp4.linear(cuda(x), w, bias=bias, activation=act, valid_rows=count(valid), out=part)
+    assert torch.equal(mxfp4.dequantize(part, torch.float32)[:valid], mxfp4.dequantize(out, torch.float32)[:valid])
+    codes, scales = X.mx_unpack(part.data.cpu().numpy(), m, n)
+    assert (scales[valid:] == 0xCD).all() and (codes[valid:, 0::2] == 0xD).all() and (codes[valid:, 1::2] == 0xC).all()
+
+
 @pytest.mark.parametrize("dtype", DTYPES)
 def test_rows_past_the_count_are_left_alone(dtype):
     x, kernel, bias, _, (want, bound) = product_case(23, 400, 288, 224, dtype, None, True, False)
