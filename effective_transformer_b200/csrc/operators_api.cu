@@ -45,12 +45,14 @@ int check_width(int k) {
   return ET_OK;
 }
 
+// (an empty batch passes here: its tensors may have no address)
 int check_gemm(int dtype, const void* a, const void* w_mx, const void* bias, const void* residual, const void* c,
                const void* c_mx, int max_m, int n, int k, int epilogue) {
   if (!known_dtype(dtype)) return refuse("dtype must be ET_FP16 or ET_FP32");
   if (int rc = check_width(k)) return rc;
   if (max_m < 0 || n <= 0 || n % 32 != 0) return refuse("max_m must not be negative, n a positive multiple of 32");
   if (epilogue < kEpiNone || epilogue > kEpiBiasTanh) return refuse("epilogue must be 0 to 3");
+  if (max_m == 0) return ET_OK;
   if ((c == nullptr) == (c_mx == nullptr)) return refuse("exactly one of c and c_mx must be given");
   if (c_mx != nullptr && (n % 64 != 0 || residual != nullptr))
     return refuse("MXFP4 output needs n a multiple of 64 and takes no residual");
@@ -169,8 +171,8 @@ int et_mxfp4_gemm(int dtype, const void* a_mx, const void* w_mx, const void* bia
                   void* c_mx, const int* m_ptr, int max_m, int n, int k, int epilogue, int* status_word, void* stream) {
   return guarded([&] {
     if (int rc = check_gemm(dtype, a_mx, w_mx, bias, residual, c, c_mx, max_m, n, k, epilogue)) return rc;
-    if (misaligned_mx(a_mx)) return refuse(kAlignment);
     if (max_m == 0) return static_cast<int>(ET_OK);
+    if (misaligned_mx(a_mx)) return refuse(kAlignment);
     if (int rc = check_result(dtype, w_mx, bias, residual, c, c_mx, a_mx, max_m, n, k)) return rc;
     const MxGemm g = gemm_of(a_mx, w_mx, c_mx, m_ptr, max_m, n, k, status_word);
     cudaStream_t s = static_cast<cudaStream_t>(stream);
@@ -229,11 +231,11 @@ int et_gated_residual_norm(int dtype, const et_gated_norm_param_t* p, void* stre
     if ((p->post_norm != ET_NORM_NONE && !p->post_gamma) || (p->post_norm == ET_NORM_LAYER && !p->post_beta) ||
         (p->pre_norm != ET_NORM_NONE && !p->pre_gamma) || (p->pre_norm == ET_NORM_LAYER && !p->pre_beta))
       return refuse("a norm needs its gamma, a LayerNorm its beta too");
+    if (p->max_m == 0) return static_cast<int>(ET_OK);  // (an empty batch's tensors may have no address)
     if (!p->h_out && !p->y_out && !p->y_mx) return refuse("at least one of h_out, y_out and y_mx must be given");
     if (p->y_mx != nullptr && p->n % kMxBlock != 0) return refuse("y_mx needs n a multiple of 32");
     if (p->gate != nullptr && (p->gate_rows < 1 || (p->gate_rows > 1 && !p->batch_idx)))
       return refuse("gate needs gate_rows >= 1, and batch_idx with more than one row");
-    if (p->max_m == 0) return static_cast<int>(ET_OK);
     if (p->x == nullptr) return refuse("null pointer");
     for (const void* q : {p->x, p->bias, p->residual, p->gate, p->post_gamma, p->post_beta, p->pre_gamma, p->pre_beta,
                           static_cast<const void*>(p->h_out), static_cast<const void*>(p->y_out)})

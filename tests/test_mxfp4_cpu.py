@@ -188,6 +188,21 @@ def test_empty_batches_are_fine():
     assert LIB.et_gated_residual_norm(1, C.byref(p), None) == 0
 
 
+def test_empty_tensors_have_no_address():
+    """A torch tensor without rows has a null pointer; sizes are checked all the same."""
+    for mx in (None, P):
+        assert LIB.et_mxfp4_gemm(1, None, P, P, None, None, mx, None, 0, 64, 64, 1, None, None) == 0
+        assert LIB.et_mxfp4_linear(0, None, 64, None, P, P, None, None, mx, None, 0, 64, 64, 2, None, None) == 0
+    refused(LIB.et_mxfp4_gemm(1, None, P, None, None, None, None, None, 0, 64, 40, 0, None, None), "multiple of 32")
+    refused(LIB.et_mxfp4_linear(1, None, 64, None, P, None, None, None, None, None, 0, 48, 64, 0, None, None), "n a")
+    refused(LIB.et_mxfp4_linear(1, None, 32, None, P, None, None, None, None, None, 0, 64, 64, 0, None, None), "row_stride")
+    p = _capi.GatedNormParam()
+    p.n, p.gate, p.gate_rows, p.pre_norm, p.pre_gamma, p.pre_beta = 64, P, 3, 1, P, P
+    assert LIB.et_gated_residual_norm(1, C.byref(p), None) == 0
+    p.pre_beta = None
+    refused(LIB.et_gated_residual_norm(1, C.byref(p), None), "beta")
+
+
 def test_python_refuses_before_any_launch():
     x = torch.zeros(4, 64, dtype=torch.float16)
     w = mxfp4.MxTensor(torch.zeros(17408, dtype=torch.uint8), 64, 64)

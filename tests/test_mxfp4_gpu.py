@@ -504,3 +504,16 @@ def test_python_refusals_on_the_gpu():
             call()
     with pytest.raises(_capi.EtError):                          # rows that start between two 16-byte boundaries
         mxfp4.quantize(torch.zeros(4 * 64 + 4, dtype=torch.float16, device="cuda")[4:].view(4, 64))
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_empty_batches(dtype):
+    x, b = torch.zeros(0, 64, dtype=dtype, device="cuda"), torch.zeros(128, dtype=dtype, device="cuda")
+    w = mxfp4.pack_weight(torch.zeros(64, 128, dtype=dtype, device="cuda"))
+    a = mxfp4.quantize(x)
+    assert (a.rows, a.cols) == (0, 64) and mxfp4.dequantize(a, dtype).shape == (0, 64)
+    for y in (mxfp4.gemm(a, w, dtype=dtype), mxfp4.gemm(a, w, bias=b, activation="gelu", residual=x.new_zeros(0, 128)),
+              mxfp4.linear(x, w), mxfp4.linear(x, w, bias=b, activation="tanh", valid_rows=count(0))):
+        assert y.shape == (0, 128) and y.dtype == dtype
+    out = mxfp4.empty(0, 128)
+    assert mxfp4.gemm(a, w, bias=b, out=out) is out and mxfp4.linear(x, w, out=out) is out

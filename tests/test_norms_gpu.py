@@ -317,3 +317,15 @@ def test_streams_and_capture():
         norms.gated_residual_norm(**a, post_norm="layer", h_out=h2, y_out=y2)
     graph.replay()
     assert torch.equal(h2, h) and torch.equal(y2, y)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_empty_batches(dtype):
+    a = make(10, 4, 64, dtype, seqs=3)
+    for k in ("x", "residual", "batch_idx"):
+        a[k] = a[k][:0]
+    h, y = norms.gated_residual_norm(**a, post_norm="rms")
+    assert h.shape == y.shape == (0, 64) and h.dtype == dtype
+    mx = mxfp4.empty(0, 64)
+    h, y = norms.gated_residual_norm(**a, post_norm="rms", mx_out=mx, valid_rows=torch.zeros(1, dtype=torch.int32, device="cuda"))
+    assert h.shape == (0, 64) and y is None
