@@ -9,6 +9,8 @@ using namespace etb;
 namespace {
 
 constexpr char kAlignment[] = "pointers must be 16-byte aligned, those of MXFP4 tensors 128-byte aligned";
+constexpr char kElementAlignment[] =
+    "m_ptr, batch_idx and status_word must be 4-byte aligned, w aligned to its elements";
 
 int refuse(const char* msg) {
   set_global_error(msg);
@@ -33,6 +35,8 @@ int guarded(F f) {
 
 bool misaligned(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) != 0; }
 bool misaligned_mx(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 127u) != 0; }
+// (an access through a pointer that its type does not allow is a fault on the GPU)
+bool misaligned_to(const void* p, size_t size) { return reinterpret_cast<uintptr_t>(p) % size != 0; }
 bool known_dtype(int dtype) { return dtype == ET_FP16 || dtype == ET_FP32; }
 size_t size_of(int dtype) { return dtype == ET_FP16 ? 2 : 4; }
 // Bytes from the first to behind the last value of `rows` rows (at least one).
@@ -47,7 +51,7 @@ int check_width(int k) {
 
 // (an empty batch passes here: its tensors may have no address)
 int check_gemm(int dtype, const void* a, const void* w_mx, const void* bias, const void* residual, const void* c,
-               const void* c_mx, int max_m, int n, int k, int epilogue) {
+               const void* c_mx, const int* m_ptr, const int* status_word, int max_m, int n, int k, int epilogue) {
   if (!known_dtype(dtype)) return refuse("dtype must be ET_FP16 or ET_FP32");
   if (int rc = check_width(k)) return rc;
   if (max_m < 0 || n <= 0 || n % 32 != 0) return refuse("max_m must not be negative, n a positive multiple of 32");
@@ -59,6 +63,7 @@ int check_gemm(int dtype, const void* a, const void* w_mx, const void* bias, con
   if (a == nullptr || w_mx == nullptr || (epilogue != kEpiNone && bias == nullptr)) return refuse("null pointer");
   if (misaligned(a) || misaligned(bias) || misaligned(residual) || misaligned(c) || misaligned_mx(w_mx) || misaligned_mx(c_mx))
     return refuse(kAlignment);
+  if (misaligned_to(m_ptr, sizeof(int)) || misaligned_to(status_word, sizeof(int))) return refuse(kElementAlignment);
   return ET_OK;
 }
 
@@ -126,6 +131,7 @@ int et_mxfp4_quantize(int dtype, const void* x, long long row_stride, const int*
     if (max_m == 0) return static_cast<int>(ET_OK);
     if (x == nullptr || mx == nullptr) return refuse("null pointer");
     if (misaligned(x) || misaligned_mx(mx)) return refuse(kAlignment);
+    if (misaligned_to(m_ptr, sizeof(int))) return refuse(kElementAlignment);
     if (overlap(x, rows_size(dtype, max_m, row_stride, k), mx, mx_bytes(max_m, k)))
       return refuse("x and mx must not overlap");
     return run_quantize(dtype, x, row_stride, m_ptr, max_m, k, mx, static_cast<cudaStream_t>(stream));
@@ -140,6 +146,7 @@ int et_mxfp4_dequantize(int dtype, const void* mx, const int* m_ptr, int max_m, 
     if (max_m == 0) return static_cast<int>(ET_OK);
     if (mx == nullptr || out == nullptr) return refuse("null pointer");
     if (misaligned_mx(mx) || misaligned(out)) return refuse(kAlignment);
+    if (misaligned_to(m_ptr, sizeof(int))) return refuse(kElementAlignment);
     if (overlap(mx, mx_bytes(max_m, k), out, rows_size(dtype, max_m, k, k)))
       return refuse("mx and out must not overlap");
     cudaStream_t s = static_cast<cudaStream_t>(stream);
@@ -158,6 +165,7 @@ int et_mxfp4_pack_weight(int dtype, const void* w, void* w_mx, int k, int n, voi
     if (n <= 0 || n % 32 != 0) return refuse("n must be a positive multiple of 32");
     if (w == nullptr || w_mx == nullptr) return refuse("null pointer");
     if (misaligned_mx(w_mx)) return refuse(kAlignment);
+    if (misaligned_to(w, size_of(dtype))) return refuse(kElementAlignment);
     if (overlap(w, rows_size(dtype, k, n, n), w_mx, mx_bytes(n, k))) return refuse("w and w_mx must not overlap");
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     if (dtype == ET_FP16)
@@ -170,7 +178,7 @@ int et_mxfp4_pack_weight(int dtype, const void* w, void* w_mx, int k, int n, voi
 int et_mxfp4_gemm(int dtype, const void* a_mx, const void* w_mx, const void* bias, const void* residual, void* c,
                   void* c_mx, const int* m_ptr, int max_m, int n, int k, int epilogue, int* status_word, void* stream) {
   return guarded([&] {
-    if (int rc = check_gemm(dtype, a_mx, w_mx, bias, residual, c, c_mx, max_m, n, k, epilogue)) return rc;
+    if (int rc = check_gemm(dtype, a_mx, w_mx, bias, residual, c, c_mx, m_ptr, status_word, max_m, n, k, epilogue)) return rc;
     if (max_m == 0) return static_cast<int>(ET_OK);
     if (misaligned_mx(a_mx)) return refuse(kAlignment);
     if (int rc = check_result(dtype, w_mx, bias, residual, c, c_mx, a_mx, max_m, n, k)) return rc;
@@ -185,7 +193,7 @@ int et_mxfp4_linear(int dtype, const void* x, long long row_stride, void* x_mx, 
                     const void* residual, void* c, void* c_mx, const int* m_ptr, int max_m, int n, int k, int epilogue,
                     int* status_word, void* stream) {
   return guarded([&] {
-    if (int rc = check_gemm(dtype, x, w_mx, bias, residual, c, c_mx, max_m, n, k, epilogue)) return rc;
+    if (int rc = check_gemm(dtype, x, w_mx, bias, residual, c, c_mx, m_ptr, status_word, max_m, n, k, epilogue)) return rc;
     if (row_stride < k || row_stride * size_of(dtype) % 16 != 0)
       return refuse("row_stride must be at least k and a multiple of 16 bytes");
     if (max_m == 0) return static_cast<int>(ET_OK);
@@ -241,6 +249,9 @@ int et_gated_residual_norm(int dtype, const et_gated_norm_param_t* p, void* stre
                           static_cast<const void*>(p->h_out), static_cast<const void*>(p->y_out)})
       if (misaligned(q)) return refuse(kAlignment);
     if (misaligned_mx(p->y_mx)) return refuse(kAlignment);
+    if (misaligned_to(p->m_ptr, sizeof(int)) ||
+        (p->gate != nullptr && p->gate_rows > 1 && misaligned_to(p->batch_idx, sizeof(int))))
+      return refuse(kElementAlignment);
     {
       // every element of x and residual is read where h and y are written, nothing else is
       const size_t row = p->n * size_of(dtype), all = p->max_m * row;

@@ -606,7 +606,8 @@ int et_gemm_fp32_tensor(const float* a_hi, const float* a_lo, const float* w_hi,
  *
  * dtype is the element type of what is not MXFP4 (x, w, bias, residual, c, out);
  * m_ptr is a DEVICE pointer to the number of valid rows, NULL = all max_m; rows
- * past it are neither read nor written.  All other pointers 16-byte aligned.  The text
+ * past it are neither read nor written.  Pointers are 16-byte aligned, w of
+ * et_mxfp4_pack_weight to its elements, m_ptr and status_word to 4 bytes.  The text
  * of a refusal is et_last_error(NULL).  Calls that overlap on the GPU may share
  * what they only read. */
 size_t et_mxfp4_bytes(int rows, int k);
@@ -654,7 +655,7 @@ typedef struct {
   const void* bias;       /* [n] or NULL */
   const void* residual;   /* [max_m, n] or NULL (then h = gate * p) */
   const void* gate;       /* [gate_rows, n] or NULL */
-  const int* batch_idx;   /* [max_m] gate row of every row (et_padding_offsets); unused with gate_rows <= 1.
+  const int* batch_idx;   /* [max_m] gate row of every row (et_padding_offsets), 4-byte aligned; unused with gate_rows <= 1.
                            * A row whose entry is outside [0, gate_rows) has gate 0. */
   const void* post_gamma; /* [n] each */
   const void* post_beta;

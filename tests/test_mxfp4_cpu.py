@@ -188,6 +188,25 @@ def test_empty_batches_are_fine():
     assert LIB.et_gated_residual_norm(1, C.byref(p), None) == 0
 
 
+def test_pointers_that_their_type_does_not_allow_are_refused():
+    """A row count, a status word or gate rows between two words, a weight between two elements: faults on the GPU."""
+    text = "4-byte aligned"
+    refused(LIB.et_mxfp4_quantize(1, P, 64, P + 2, 3, 64, FAR, None), text)
+    refused(LIB.et_mxfp4_dequantize(1, P, P + 1, 3, 64, FAR, None), text)
+    for dtype, off in ((1, 1), (0, 2)):
+        refused(LIB.et_mxfp4_pack_weight(dtype, FAR + off, P, 64, 64, None), text)
+    for m_ptr, status in ((P + 2, None), (None, P + 1)):
+        tail = (FAR, None, None, FAR + (1 << 20), None, m_ptr, 3, 64, 64, 0, status, None)
+        refused(LIB.et_mxfp4_gemm(1, P, *tail), text)
+        refused(LIB.et_mxfp4_linear(1, P + (1 << 20), 64, P, *tail), text)
+    for change in (dict(m_ptr=FAR + 2), dict(gate=FAR, gate_rows=3, batch_idx=FAR + 4098)):
+        p = _capi.GatedNormParam()
+        p.x, p.h_out, p.max_m, p.n, p.residual_scale = P, P, 4, 64, 1.0
+        for k, v in change.items():
+            setattr(p, k, v)
+        refused(LIB.et_gated_residual_norm(1, C.byref(p), None), text)
+
+
 def test_empty_tensors_have_no_address():
     """A torch tensor without rows has a null pointer; sizes are checked all the same."""
     for mx in (None, P):
