@@ -14,6 +14,7 @@ them.  Tensors must be contiguous (x of quantize and linear: contiguous rows) an
 """
 from __future__ import annotations
 
+import threading
 from typing import Dict, Optional, Union
 
 import torch
@@ -25,6 +26,7 @@ __all__ = ["MxTensor", "empty", "quantize", "dequantize", "pack_weight", "gemm",
 _DTYPE = {torch.float16: _capi.ET_FP16, torch.float32: _capi.ET_FP32}
 _EPILOGUE = {None: 1, "gelu": 2, "tanh": 3}
 _status: Dict[int, tuple] = {}
+_status_lock = threading.Lock()
 _lib = None
 
 
@@ -110,14 +112,17 @@ def _call(device: int, name: str, *args) -> None:
 
 
 def _status_word(device: int) -> int:
-    """Address of the device's status word."""
+    """Address of the device's status word, one for all threads: a kernel may write to it at any time."""
     word = _status.get(device)
     if word is None:
-        _require(not torch.cuda.is_current_stream_capturing(),
-                 "call mxfp4.device_status(device) once before a product is captured on this device")
-        data = torch.zeros(1, dtype=torch.int32, device=torch.device("cuda", device))
-        torch.cuda.current_stream(device).synchronize()  # (other streams may use it from now on)
-        word = _status[device] = (data.data_ptr(), data)
+        with _status_lock, torch.cuda.device(device):
+            word = _status.get(device)
+            if word is None:
+                _require(not torch.cuda.is_current_stream_capturing(),
+                         "call mxfp4.device_status(device) once before a product is captured on this device")
+                data = torch.zeros(1, dtype=torch.int32, device=torch.device("cuda", device))
+                torch.cuda.current_stream(device).synchronize()  # (other streams may use it from now on)
+                word = _status[device] = (data.data_ptr(), data)
     return word[0]
 
 

@@ -207,6 +207,42 @@ def test_pointers_that_their_type_does_not_allow_are_refused():
         refused(LIB.et_gated_residual_norm(1, C.byref(p), None), text)
 
 
+def test_threads_share_one_status_word(monkeypatch):
+    """Two threads whose first product on a device comes at the same time: a second word would take the first one's place
+    and free memory that a kernel may write to."""
+    import contextlib
+    import threading
+    import time
+    made, words, entered = [], [], []
+
+    def zeros(*_, **__):
+        made.append(torch.empty(1, dtype=torch.int32))
+        time.sleep(0.2)                                         # (the other thread comes in meanwhile)
+        return made[-1]
+
+    @contextlib.contextmanager
+    def on(device):
+        entered.append(device)
+        yield
+
+    class Stream:
+        def synchronize(self):
+            pass
+
+    monkeypatch.setattr(mxfp4, "_status", {})
+    monkeypatch.setattr(torch, "zeros", zeros)
+    monkeypatch.setattr(torch.cuda, "device", on)
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: False)
+    monkeypatch.setattr(torch.cuda, "current_stream", lambda *_: Stream())
+    threads = [threading.Thread(target=lambda: words.append(mxfp4._status_word(3))) for _ in range(4)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert len(made) == 1 and words == [made[0].data_ptr()] * 4
+    assert set(entered) == {3}                                  # (a capture on that device's stream is what is asked about)
+
+
 def test_empty_tensors_have_no_address():
     """A torch tensor without rows has a null pointer; sizes are checked all the same."""
     for mx in (None, P):
