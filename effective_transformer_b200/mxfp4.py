@@ -11,6 +11,10 @@
 Every call runs on the current stream of the tensors' device and returns without waiting.  `valid_rows` is a device
 int32 [1] (valid_word_num of the input op): rows past it are neither read nor written, an output passed as `out` keeps
 them.  Tensors must be contiguous (x of quantize and linear: contiguous rows) and on one device.
+
+There is no backward pass.  Where autograd records and a tensor requires a gradient, a new result raises in backward, as a
+custom op without a formula does; a call that writes into a given buffer or into 4 bits, which could not, is refused.
+pack_weight takes a copy, to which no gradient belongs.
 """
 from __future__ import annotations
 
@@ -96,6 +100,41 @@ def _check_mx(t: "MxTensor", name: str, rows: int, cols: int, device: int) -> No
         raise ValueError(f"{name} must be an MxTensor of at least {rows} rows of {cols} values on cuda:{device}")
 
 
+def _wants_gradient(*tensors: Optional[torch.Tensor]) -> bool:
+    if not torch.is_grad_enabled():
+        return False
+    for t in tensors:
+        if t is not None and t.requires_grad:
+            return True
+    return False
+
+
+_NO_BACKWARD = "4-bit operators and gated norms have no backward pass: "
+
+
+class _NoBackward(torch.autograd.Function):
+    """Results (the first `count` tensors) tied to the tensors that require a gradient."""
+
+    @staticmethod
+    def forward(ctx, count: int, *tensors):
+        ctx.mark_dirty(*tensors[:count])
+        return tensors[:count]
+
+    @staticmethod
+    def backward(ctx, *_):
+        raise NotImplementedError(_NO_BACKWARD + "call them under torch.no_grad(), or detach what goes in")
+
+
+def _tie(results, *tensors):
+    """New results of a call that was given tensors with a gradient."""
+    return _NoBackward.apply(len(results), *results, *(t for t in tensors if t is not None and t.requires_grad))
+
+
+def _refuse_gradients() -> None:
+    raise ValueError(_NO_BACKWARD + "with a given buffer or an MXFP4 tensor for the result, call them under "
+                     "torch.no_grad(), or detach what goes in")
+
+
 def _call(device: int, name: str, *args) -> None:
     """One entry point of the library on the current stream of `device` (it launches on the current device)."""
     global _lib
@@ -150,6 +189,8 @@ def empty(rows: int, cols: int, device: Union[str, torch.device] = "cuda") -> Mx
 def quantize(x: torch.Tensor, valid_rows: Optional[torch.Tensor] = None, out: Optional[MxTensor] = None) -> MxTensor:
     """Rows of x [rows, width] to MXFP4 (rows may be strided, the values of a row are contiguous)."""
     rows, k, stride, device = _check_rows(x, "x")
+    if _wants_gradient(x):
+        _refuse_gradients()
     count = _count(valid_rows, device)
     if out is None:
         out = empty(rows, k, x.device)
@@ -232,9 +273,13 @@ def gemm(a: MxTensor, weight: MxTensor, bias: Optional[torch.Tensor] = None, act
         given = out if plain else bias if bias is not None else residual
         dtype = torch.float16 if given is None else given.dtype
     _require(dtype in _DTYPE, "dtype must be torch.float16 or torch.float32")
+    given = out
     out, args = _result(rows, a.device, weight, bias, activation, residual, valid_rows, out, dtype)
+    gradient = _wants_gradient(bias, residual)
+    if gradient and given is not None:
+        _refuse_gradients()
     _call(a.device, "et_mxfp4_gemm", _DTYPE[dtype], a.ptr, weight.ptr, *args)
-    return out
+    return _tie((out,), bias, residual)[0] if gradient else out
 
 
 def linear(x: torch.Tensor, weight: MxTensor, bias: Optional[torch.Tensor] = None, activation: Optional[str] = None,
@@ -251,6 +296,10 @@ def linear(x: torch.Tensor, weight: MxTensor, bias: Optional[torch.Tensor] = Non
         workspace = empty(rows, k, x.device)
     _check_mx(workspace, "workspace", rows, k, device)
     dtype = x.dtype
+    given = out
     out, args = _result(rows, device, weight, bias, activation, residual, valid_rows, out, dtype)
+    gradient = _wants_gradient(x, bias, residual)
+    if gradient and given is not None:
+        _refuse_gradients()
     _call(device, "et_mxfp4_linear", _DTYPE[dtype], x.data_ptr(), stride, workspace.ptr, weight.ptr, *args)
-    return out
+    return _tie((out,), x, bias, residual)[0] if gradient else out

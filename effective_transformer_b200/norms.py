@@ -5,6 +5,8 @@
                                      pre_norm="layer", pre_gamma=g2, pre_beta=b2)
 
 p = post(x + bias);  h = residual_scale * residual + gate * p;  y = pre(h)   (include/et_b200.h, et_gated_residual_norm)
+
+There is no backward pass: tensors that require a gradient are taken as effective_transformer_b200.mxfp4 takes them.
 """
 from __future__ import annotations
 
@@ -13,7 +15,8 @@ from typing import Optional, Tuple
 
 import torch
 
-from .mxfp4 import MxTensor, _call, _check, _check_mx, _count, _DTYPE, _require
+from .mxfp4 import (MxTensor, _call, _check, _check_mx, _count, _DTYPE, _refuse_gradients, _require, _tie,
+                    _wants_gradient)
 
 __all__ = ["gated_residual_norm"]
 
@@ -46,6 +49,7 @@ def gated_residual_norm(x: torch.Tensor, bias: Optional[torch.Tensor] = None, re
     post, pre = _KIND.get(post_norm), _KIND.get(pre_norm)
     if post is None or pre is None:
         raise ValueError("post_norm and pre_norm must be 'none', 'layer' or 'rms'")
+    fresh = h_out is None and y_out is None and mx_out is None
     bias_p = res_p = gate_p = idx_p = post_g = post_b = pre_g = pre_b = y_p = mx_p = 0
     if h_out is None:
         h_out = torch.empty_like(x)
@@ -94,6 +98,12 @@ def gated_residual_norm(x: torch.Tensor, bias: Optional[torch.Tensor] = None, re
     if mx_out is not None:
         _check_mx(mx_out, "mx_out", rows, n, device)
         mx_p = mx_out.ptr
+    # (what a norm does not use has been ignored above and is here)
+    inputs = (x, bias, residual, gate, post_gamma if post_g else None, post_beta if post_b else None,
+              pre_gamma if pre_g else None, pre_beta if pre_b else None)
+    gradient = _wants_gradient(*inputs)
+    if gradient and not fresh:
+        _refuse_gradients()
     try:
         p = _PARAM.pack(x.data_ptr(), bias_p, res_p, gate_p, idx_p, post_g, post_b, pre_g, pre_b, h_p, y_p, mx_p,
                         0 if valid_rows is None else _count(valid_rows, device), rows, n, gate_rows, post, pre,
@@ -101,4 +111,6 @@ def gated_residual_norm(x: torch.Tensor, bias: Optional[torch.Tensor] = None, re
     except (struct.error, OverflowError) as e:
         raise ValueError("residual_scale and eps must be numbers that fp32 has, and sizes fit 32 bits") from e
     _call(device, "et_gated_residual_norm", _DTYPE[dtype], p)
+    if gradient:
+        return _tie((h_out, y_out), *inputs)
     return h_out, y_out

@@ -517,3 +517,29 @@ def test_empty_batches(dtype):
         assert y.shape == (0, 128) and y.dtype == dtype
     out = mxfp4.empty(0, 128)
     assert mxfp4.gemm(a, w, bias=b, out=out) is out and mxfp4.linear(x, w, out=out) is out
+
+
+def test_gradients_are_not_lost_silently():
+    x = torch.randn(4, 64, device="cuda").half()
+    w = mxfp4.pack_weight(torch.nn.Parameter(torch.randn(64, 64, device="cuda").half()))
+    b = torch.nn.Parameter(torch.zeros(64, device="cuda").half())
+    leaf = x.clone().requires_grad_()
+    want = mxfp4.linear(x, w, bias=b.detach(), residual=x)
+    a = mxfp4.quantize(x)
+    for call in (lambda: mxfp4.linear(x, w, bias=b, residual=x), lambda: mxfp4.gemm(a, w, bias=b, residual=x),
+                 lambda: mxfp4.linear(leaf, w, bias=b.detach(), residual=x),
+                 lambda: mxfp4.gemm(a, w, bias=b.detach(), residual=leaf)):
+        y = call()
+        assert torch.equal(y, want) and y.requires_grad
+        with pytest.raises(NotImplementedError, match="no backward"):
+            (y.float().sum() + leaf.float().sum()).backward()
+        with torch.no_grad():
+            assert torch.equal(call(), want) and not call().requires_grad
+    assert not want.requires_grad
+    out = torch.empty_like(x)
+    for call in (lambda: mxfp4.linear(leaf, w, out=out), lambda: mxfp4.gemm(a, w, bias=b, out=out),
+                 lambda: mxfp4.quantize(leaf), lambda: mxfp4.linear(x, w, bias=b, out=mxfp4.empty(4, 64))):
+        with pytest.raises(ValueError, match="no backward"):
+            call()
+        with torch.no_grad():
+            call()

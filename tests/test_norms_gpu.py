@@ -329,3 +329,20 @@ def test_empty_batches(dtype):
     mx = mxfp4.empty(0, 64)
     h, y = norms.gated_residual_norm(**a, post_norm="rms", mx_out=mx, valid_rows=torch.zeros(1, dtype=torch.int32, device="cuda"))
     assert h.shape == (0, 64) and y is None
+
+
+@pytest.mark.parametrize("name", ["x", "bias", "residual", "gate", "post_gamma", "post_beta", "pre_gamma", "pre_beta"])
+def test_gradients_are_not_lost_silently(name):
+    a = make(11, 4, 64, torch.float16, seqs=2)
+    want = norms.gated_residual_norm(**a, post_norm="layer")
+    a[name] = a[name].clone().requires_grad_()
+    got = norms.gated_residual_norm(**a, post_norm="layer")
+    assert all(torch.equal(u, v) and u.requires_grad for u, v in zip(got, want))
+    for u in got:
+        with pytest.raises(NotImplementedError, match="no backward"):
+            u.float().sum().backward(retain_graph=True)
+    for kw in (dict(h_out=torch.empty_like(a["x"])), dict(y_out=torch.empty_like(a["x"])), dict(mx_out=mxfp4.empty(4, 64))):
+        with pytest.raises(ValueError, match="no backward"):
+            norms.gated_residual_norm(**a, post_norm="layer", **kw)
+        with torch.no_grad():
+            norms.gated_residual_norm(**a, post_norm="layer", **kw)
