@@ -600,12 +600,14 @@ int run_layer_mx(et_handle_t h, const LayerWeights& lw, const T* x_in, T* x_out,
     ET_LAUNCH(h, ET_PROF_GEMM_QKV, 1, s, gemm(ws.x_mx, lw.wqkv_mx, lw.bqkv, qkv, nullptr, 3 * hid, hid, kEpiBias));
   else
     ET_LAUNCH(h, ET_PROF_GEMM_QKV, kernels(3 * hid), s, linear(x_in, lw.wqkv_mx, lw.bqkv, qkv, 3 * hid, kEpiBias));
+  h->prev_ascending = true;  // (the 4-bit products, rows and norms only run first-to-last)
   if (int rc = run_attention<T>(h, qkv, ctx, nullptr, max_m, cu_seqlens, batch, seq, s); rc != ET_OK) return rc;
   ET_LAUNCH(h, ET_PROF_GEMM_ATTN_OUT, kernels(hid), s, linear(ctx, lw.wo_mx, nullptr, att, hid, kEpiNone));
   ET_LAUNCH(h, ET_PROF_LAYERNORM, 1, s, norm(att, lw.bo, x_in, lw.ln1_gamma, lw.ln1_beta, att, true));
   ET_LAUNCH(h, ET_PROF_GEMM_FFN1, 1, s, gemm(ws.x_mx, lw.w1_mx, lw.b1, nullptr, ws.ffn_mx, f, hid, kEpiBiasGelu));
   ET_LAUNCH(h, ET_PROF_GEMM_FFN2, 1, s, gemm(ws.ffn_mx, lw.w2_mx, nullptr, x_out, nullptr, hid, f, kEpiNone));
   ET_LAUNCH(h, ET_PROF_LAYERNORM, 1, s, norm(x_out, lw.b2, att, lw.ln2_gamma, lw.ln2_beta, x_out, out_mx));
+  h->prev_ascending = true;
   return ET_OK;
 }
 

@@ -305,3 +305,16 @@ def test_routes():
         assert LIB.et_mxfp4_route(1, rows, n, k, C.byref(a), C.byref(a), C.byref(a)) == BAD
     assert LIB.et_mxfp4_route(2, 1, 32, 32, C.byref(a), C.byref(a), C.byref(a)) == BAD
     assert LIB.et_mxfp4_route(1, 1, 32, 32, None, C.byref(a), C.byref(a)) == BAD
+
+
+def test_the_attention_of_a_4_bit_layer_starts_with_the_rows_that_came_last():
+    """Products, rows and norms in 4 bits only run first-to-last, so the attention behind them always runs last-to-first;
+    left to the flag that the attention itself flips, its order would depend on the calls before."""
+    import os
+    import re
+    with open(os.path.join(os.path.dirname(_capi.__file__), "csrc", "encoder.cu")) as f:
+        body = re.search(r"\nint run_layer_mx\(.*?\n\}\n", f.read(), re.S).group(0)
+    steps = re.findall(r"ET_PROF_\w+|run_attention|prev_ascending = true", body)
+    assert steps == ["ET_PROF_GEMM_QKV"] * 2 + ["prev_ascending = true", "run_attention", "ET_PROF_GEMM_ATTN_OUT",
+                                                "ET_PROF_LAYERNORM", "ET_PROF_GEMM_FFN1", "ET_PROF_GEMM_FFN2",
+                                                "ET_PROF_LAYERNORM", "prev_ascending = true"]
