@@ -395,10 +395,16 @@ cudaError_t launch_gated_norm(const GatedNorm& p, cudaStream_t stream) {
   if (wpr > kMaxWarps) return cudaErrorInvalidValue;
   if constexpr (sizeof(T) == 4)
     if (wpr <= 4) return launch_rows<T, 2, 1, true>(p, wpr, stream);
-  // Two vectors a lane spill a little with 96 registers, which pays where it brings one more CTA to an SM: 6699 rows of
-  // 2080 (9 warps) 49 us instead of 70, but 4096 (16 warps) 116 us instead of 98, 13000 of 2048 (8 warps) 97 instead of 86.
+  // Two vectors a lane spill with 96 registers (fp32 40 to 96 bytes a thread, fp16 330).  That pays where it brings two CTAs
+  // to an SM instead of one, and in full rows, which spill least, of five and six warps (four instead of three, three instead
+  // of two); not at seven.  128 / 96 registers, both norms and a gate per sequence, us:
+  //   9 and 10 warps: 6699 rows fp32 2080 82 / 66, 2304 80 / 59, 2560 81 / 62; fp16 4608 141 / 91, 5120 147 / 96;
+  //   full rows: 13000 rows fp32 1280 57.1 / 55.9, 1536 76 / 70; but 1792 (7 warps) 83 / 94;
+  //   others: 1184 58 / 63, 1408 77 / 80, 1664 84 / 106.
   constexpr int kFile = 65536 / 32;
-  if (kFile / (wpr * 96) > kFile / (wpr * 128)) return launch_rows<T, 2, 1, false, 96>(p, wpr, stream);
+  const int more = kFile / (wpr * 96), few = kFile / (wpr * 128);
+  const bool full = p.n == 64 * wpr * E;
+  if (more >= 2 * few || (more > few && full && wpr <= 6)) return launch_rows<T, 2, 1, false, 96>(p, wpr, stream);
   return launch_rows<T, 2, 1, false>(p, wpr, stream);
 }
 

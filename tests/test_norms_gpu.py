@@ -78,7 +78,7 @@ ROUNDS = [(F16, 12003, 96, 148 * 4 * 8), (F16, 12003, 256, 148 * 4 * 8), (F16, 7
           (F16, 701, 5768, 148), (F16, 701, 8192, 148),
           (F32, 12003, 96, 148 * 4 * 8), (F32, 7001, 256, 148 * 4 * 4), (F32, 4099, 640, 148 * 3 * 2),
           (F32, 4099, 896, 148 * 2 * 2), (F32, 5003, 1024, 148 * 4), (F32, 3001, 1280, 148 * 4), (F32, 3001, 1536, 148 * 3),
-          (F32, 3001, 1792, 148 * 3), (F32, 2001, 2048, 148 * 2), (F32, 2001, 2080, 148 * 2), (F32, 2001, 2560, 148 * 2),
+          (F32, 3001, 1792, 148 * 3), (F32, 3001, 1184, 148 * 4), (F32, 3001, 1408, 148 * 3), (F32, 3001, 1664, 148 * 3), (F32, 2001, 2048, 148 * 2), (F32, 2001, 2080, 148 * 2), (F32, 2001, 2560, 148 * 2),
           (F32, 1003, 2688, 148), (F32, 1003, 4096, 148)]
 
 
