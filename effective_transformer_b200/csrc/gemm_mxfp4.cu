@@ -537,8 +537,9 @@ gemm_mxfp4_kernel(const MxArgs g, const T* bias) {
 // 104 / 83 us (and, with an earlier epilogue that took 104 / 76 us here: 256 x 256 in two column halves with three
 // half-width buffers 120 / 82 us, 256 x 256 with one buffer 118 / 71 us).
 //
-// What bounds it now is the way of the operands from L2 to the SMs: 7.4 KB per 64 values of K and CTA, 119 cycles at 64
-// bytes a cycle where the MMA needs 96; 47 to 57 bytes a cycle and SM are measured.
+// What bounds it now is the way of the operands from L2 to the SMs: 7.75 KB per 64 values of K and CTA, 124 cycles at 64
+// bytes a cycle where the MMA needs 96; 62 bytes a cycle and SM are measured at 4096 -> 1024, 41 at 1024 -> 4096, where the
+// results take 15 more.  With GELU it is the special functions (gelu_pair): their unit is 75 % busy, 70 % into 4 bits.
 //
 // Epilogue: all twelve warps on every tile, two column groups each that are in registers before the buffer goes back.
 // Two sets of eight warps in turn, three groups each one after the other, took the same time for plain results (which
@@ -1088,10 +1089,10 @@ cudaError_t launch_checked(const MxGemm& p, const T* x, long long row_stride, co
 // Tiles of 256 x 192 by CTA pairs need half the L2 traffic per product and 40 % fewer issue slots; tiles of 128 x 128
 // start sooner, waste less at the edges and have the shorter epilogue.  Measured, 128 x 128 / pairs, us:
 //   at least three rounds of 128 x 128 tiles, K = 4096: 8192 x 1024 23.2 / 17.0; K = 2048: 4096 x 2048 14.1 / 11.6;
-//     K = 1024: 40000 x 4096 108 / 92, with GELU 114 / 102; K = 768: 16000 x 2304 22.8 / 20.3, with a residual 48 / 38
-//     (fp32 31.8 / 31.2 and 93 / 58); but K = 256: 40000 x 1024 20.0 / 20.7, with GELU 22.5 / 24.4;
+//     K = 1024: 40000 x 4096 104 / 87, with GELU 115 / 115 to 123; K = 768: 16000 x 2304 22.8 / 19.1, with GELU 26.5 / 28,
+//     with a residual 49 / 33 (fp32 31.8 / 30.2 and 93 / 56); but K = 256: 40000 x 1024 16.6 / 17.2, with GELU 26.7 / 31.4;
 //   one to three rounds, K = 4096: 4096 x 1024 13.7 / 12.6; K = 2048: 2048 x 2048 9.1 / 8.7 (fp32 9.1 / 10.0);
-//     K = 1024: 4096 x 1024 with GELU 6.8 / 7.2;
+//     K = 1024: 4096 x 1024 with GELU 6.7 / 7.9;
 //   one round, K = 2048: 1024 x 2048 6.4 / 6.6.
 MxRoute mxfp4_route(bool fp32_result, int rows, int n, int k) {
   const long long tiles = static_cast<long long>((rows + BM - 1) / BM) * ((n + 127) / 128);

@@ -35,8 +35,9 @@ def gated_residual_norm(x: torch.Tensor, bias: Optional[torch.Tensor] = None, re
                         ) -> Tuple[torch.Tensor, Optional[torch.Tensor]]:
     """(h, y) of packed rows x [rows, width], fp16 or fp32.
 
-    gate [width], or [sequences, width] with batch_idx int32 [rows] (of the input op; any shape with at least that many
-    entries).  A row whose batch_idx is outside the gate's rows has gate 0.  post_norm / pre_norm: "none", "layer" or
+    gate [width] or [1, width], for every row; or [sequences, width] with batch_idx int32 [rows] (of the input op; any shape
+    with at least that many entries), where a row whose batch_idx is outside the gate's rows has gate 0.  eps <= 0 selects
+    1e-6.  post_norm / pre_norm: "none", "layer" or
     "rms"; parameters of a norm that is not used are ignored.  valid_rows: device int32 [1], rows past it are left as
     they are.  h_out / y_out: buffers for the results, either may be x or residual.  mx_out takes y in MXFP4 for the
     projection behind it; y itself is then written only where y_out is given (None is returned otherwise).  The width
