@@ -13,6 +13,10 @@
 // gemm_mxfp4_kernel works on tiles of 128 x 128, gemm_mxfp4_pair_kernel on tiles of 256 x 192 by CTA pairs.  The third,
 // gemm_mxfp4_rows_kernel, takes few rows in fp16 or fp32 and quantises them itself.
 // Scales have a TMEM region per stage, so a stage's are replaced only after the MMAs that read them have retired.
+//
+// Tensor memory is taken behind the wait for the kernels in front and before dependents are released.  A CTA of a dependent
+// that held it while it waits could leave none for a CTA of the kernel that it waits for: a pair kernel's CTA (159 KB of
+// shared memory, all 512 columns) fits an SM beside one of the attention, which releases its dependents before it allocates.
 #include "common.cuh"
 #include "mxfp4.cuh"
 #include "packed_f32.cuh"
@@ -39,6 +43,7 @@ enum Site : int {
   kSiteMmaDrain = 5,
   kSiteEpilogueFull = 6,
   kSiteSmemAlign = 7,
+  kSiteMmaPeerTmem = 8,
 };
 
 struct MxArgs {
@@ -330,6 +335,25 @@ __device__ __forceinline__ void issue_stage(int steps, uint32_t d_tmem, uint32_t
   }
 }
 
+// The kernels' tensor memory, behind their wait (see the top of the file).  Warp 1 allocates and then releases the
+// dependents, since a CTA of theirs must not take what this one is about to; it waits for nobody, and the epilogue's warps
+// (the other `threads`) ask for the address when they need it.
+template <typename Alloc>
+__device__ __forceinline__ uint32_t take_tmem(const uint32_t* slot, int threads, Alloc alloc) {
+  alloc();
+  __syncwarp();
+  tc_fence_before();
+  asm volatile("bar.arrive 1, %0;" ::"r"(threads + 32) : "memory");
+  tc_fence_after();
+  pdl_trigger();
+  return __shfl_sync(0xffffffffu, *static_cast<const volatile uint32_t*>(slot), 0);
+}
+__device__ __forceinline__ uint32_t tmem_address(const uint32_t* slot, int threads) {
+  asm volatile("bar.sync 1, %0;" ::"r"(threads + 32) : "memory");
+  tc_fence_after();
+  return __shfl_sync(0xffffffffu, *static_cast<const volatile uint32_t*>(slot), 0);
+}
+
 template <int BN>
 struct Cfg {
   static constexpr int kStages = 6;
@@ -382,19 +406,17 @@ gemm_mxfp4_kernel(const MxArgs g, const T* bias) {
     fence_mbar_init();
     fence_proxy_async_smem();
   }
-  if (warp == 1) {
-    tmem_alloc(smem_u32(tmem_slot), cfg::kTmemCols);
-    tmem_relinquish();
-  }
-  tc_fence_before();
   __syncthreads();
-  tc_fence_after();
-  pdl_trigger();  // (not before: a dependent's CTA must not take the tensor memory that this one waits for)
-  const uint32_t tmem_base = __shfl_sync(0xffffffffu, *tmem_slot, 0);
-
   int M = g.max_m;
   if (g.m_ptr != nullptr) M = pdl_wait_row_count(g.m_ptr, g.max_m, 0);
   else pdl_wait();
+  uint32_t tmem_base = 0;  // (the producer needs none)
+  if (warp == 1)
+    tmem_base = take_tmem(tmem_slot, kNumThreads - 64, [&] {
+      tmem_alloc(smem_u32(tmem_slot), cfg::kTmemCols);
+      tmem_relinquish();
+    });
+
   const int N = g.n;
   const int n_tiles = (N + BN - 1) / BN;
   const int num_tiles = (M + BM - 1) / BM * n_tiles;
@@ -498,6 +520,7 @@ gemm_mxfp4_kernel(const MxArgs g, const T* bias) {
     }
     __syncwarp();
   } else {
+    tmem_base = tmem_address(tmem_slot, kNumThreads - 64);
     const int quad = warp & 3, half = ((warp - 2) >> 2) & 1, acc = (warp - 2) / kEpilogueSet;
     const uint32_t t_row = tmem_base + (static_cast<uint32_t>(quad * 32) << 16) + acc * BN + half * (BN / 2);
     uint32_t phase = 0;
@@ -559,7 +582,7 @@ struct PairCfg {
   static constexpr int kStageBytes = kMxTileBytes + kBCodes + 2 * kMxScaleBytes;
   static constexpr int kScaleCols = 24;  // per stage: 2 pieces of A, 2 of each block of W, 4 columns each
   static constexpr int kTmemCols = 512;
-  static constexpr int kNumBars = 2 * kStages + 5;
+  static constexpr int kNumBars = 2 * kStages + 6;
   static constexpr int kSmemBytes = kStages * kStageBytes + 256;
   static_assert(2 * BN + kStages * kScaleCols <= kTmemCols, "tensor memory");
   static_assert(kStageBytes % 1024 == 0 && kSmemBytes <= 232448 && kNumBars * 8 + 8 <= 256, "shared memory");
@@ -587,7 +610,7 @@ gemm_mxfp4_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_
   auto free_bar = [&](int s) { return bar0 + 8u * (S + s); };
   auto tmem_full_bar = [&](int a) { return bar0 + 8u * (2 * S + a); };
   auto tmem_empty_bar = [&](int a) { return bar0 + 8u * (2 * S + 2 + a); };
-  const uint32_t drain_bar = bar0 + 8u * (2 * S + 4);
+  const uint32_t drain_bar = bar0 + 8u * (2 * S + 4), peer_tmem_bar = drain_bar + 8u;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + cfg::kNumBars);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   const int warp = __shfl_sync(0xffffffffu, static_cast<int>(threadIdx.x) >> 5, 0), lane = threadIdx.x & 31;
@@ -602,24 +625,27 @@ gemm_mxfp4_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_
       mbar_init(tmem_empty_bar(a), 2 * cfg::kEpilogueWarps);
     }
     mbar_init(drain_bar, 1);
+    mbar_init(peer_tmem_bar, 1);
     *abort_flag = 0;
     fence_mbar_init();
     fence_proxy_async_smem();
   }
-  if (warp == 1) {
-    tmem_alloc_pair(smem_u32(tmem_slot), cfg::kTmemCols);
-    tmem_relinquish_pair();
-  }
-  tc_fence_before();
   __syncthreads();
   cluster_sync_all();  // the peer's barriers are initialised before anything signals them
-  tc_fence_after();
-  pdl_trigger();  // (not before: a dependent's CTA must not take the tensor memory that this one waits for)
-  const uint32_t tmem_base = __shfl_sync(0xffffffffu, *tmem_slot, 0);
-
   int M = g.max_m;
   if (g.m_ptr != nullptr) M = pdl_wait_row_count(g.m_ptr, g.max_m, 0);
   else pdl_wait();
+  uint32_t tmem_base = 0;  // (the producer needs none)
+  if (warp == 1)
+    tmem_base = take_tmem(tmem_slot, cfg::kThreads - 64, [&] {
+      tmem_alloc_pair(smem_u32(tmem_slot), cfg::kTmemCols);
+      tmem_relinquish_pair();
+      __syncwarp();
+      tc_fence_before();
+      // (CTA 0 issues into both CTAs' tensor memory; a second cluster barrier instead: 0.7 us a launch)
+      if (rank == 1 && lane == 0) mbar_arrive_cluster(mapa_shared(peer_tmem_bar, 0));
+    });
+
   const int N = g.n;
   const int n_tiles = (N + cfg::BN - 1) / cfg::BN;
   const int num_tiles = (M + 255) / 256 * n_tiles;
@@ -713,7 +739,9 @@ gemm_mxfp4_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_
       const bool issuer = elect_one();
       uint32_t stage = 0, phase = 0;
       int it = 0;
-      bool ok = true;
+      bool ok = __all_sync(0xffffffffu, mbar_wait(peer_tmem_bar, 0u, abort_flag)) != 0;
+      if (!ok && lane == 0) fail(kSiteMmaPeerTmem);
+      tc_fence_after();
       for (int tile = pair_id; tile < num_tiles && ok; tile += num_pairs, ++it) {
         const int n_tile = tile % n_tiles, cols = columns(n_tile), acc = it & 1;
         if (!__all_sync(0xffffffffu, mbar_wait(tmem_empty_bar(acc), ((it >> 1) & 1) ^ 1u, abort_flag))) {
@@ -756,6 +784,7 @@ gemm_mxfp4_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_
     }
   } else {
     // ------------------------- epilogue (both CTAs) -------------------------
+    tmem_base = tmem_address(tmem_slot, cfg::kThreads - 64);
     const int quad = warp & 3, part = (warp - 2) >> 2;
     const uint32_t t_row = tmem_base + (static_cast<uint32_t>(quad * 32) << 16) + part * 64;
     int it = 0;
@@ -869,33 +898,29 @@ gemm_mxfp4_rows_kernel(const MxArgs g, const T* x, long long row_stride, const T
     fence_mbar_init();
     fence_proxy_async_smem();
   }
-  if (warp == 1) {
-    tmem_alloc(smem_u32(tmem_slot), cfg::kTmemCols);
-    tmem_relinquish();
-  }
-  tc_fence_before();
   __syncthreads();
-  tc_fence_after();
-  pdl_trigger();  // (not before: a dependent's CTA must not take the tensor memory that this one waits for)
-  const uint32_t tmem_base = __shfl_sync(0xffffffffu, *tmem_slot, 0);
-
   int M = g.max_m;
   if (g.m_ptr != nullptr) M = pdl_wait_row_count(g.m_ptr, g.max_m, 0);
   else pdl_wait();
+
   const int N = g.n;
   const int n_tiles = (N + BN - 1) / BN;
   const int m_tile = blockIdx.x / n_tiles, n_tile = blockIdx.x - m_tile * n_tiles;
   const int row_tile = m_tile * BM;
-  const bool work = row_tile < M;  // (uniform for the CTA)
+  if (row_tile >= M) return;  // (the whole CTA, with nothing in flight)
+  uint32_t tmem_base = 0;  // (the producer needs none)
+  if (warp == 1)
+    tmem_base = take_tmem(tmem_slot, kNumThreads - 64, [&] {
+      tmem_alloc(smem_u32(tmem_slot), cfg::kTmemCols);
+      tmem_relinquish();
+    });
 
   auto fail = [&](int site) {
     *abort_flag = 1;
     report_timeout(g.status_word, kKernelGemmMx, site);
   };
 
-  if (!work) {
-    // nothing in flight, straight to the end
-  } else if (warp == 0) {
+  if (warp == 0) {
     const bool issuer = elect_one();
     if (issuer) {
       const uint8_t* w_src =
@@ -978,6 +1003,7 @@ gemm_mxfp4_rows_kernel(const MxArgs g, const T* x, long long row_stride, const T
     fence_proxy_async_smem();  // these stores are read by the tensor core
     __syncwarp();
     if (lane == 0) mbar_arrive(rows_bar);
+    tmem_base = tmem_address(tmem_slot, kNumThreads - 64);
     // ---- epilogue: eight of the warps, a lane quadrant and 32 columns each ----
     if (warp < 2 + kEpilogueSet) {
       const int quad = warp & 3, half = (warp - 2) >> 2;

@@ -318,3 +318,20 @@ def test_the_attention_of_a_4_bit_layer_starts_with_the_rows_that_came_last():
     assert steps == ["ET_PROF_GEMM_QKV"] * 2 + ["prev_ascending = true", "run_attention", "ET_PROF_GEMM_ATTN_OUT",
                                                 "ET_PROF_LAYERNORM", "ET_PROF_GEMM_FFN1", "ET_PROF_GEMM_FFN2",
                                                 "ET_PROF_LAYERNORM", "prev_ascending = true"]
+
+
+def test_products_take_tensor_memory_behind_their_wait():
+    """A CTA that holds tensor memory while it waits for the kernel in front can leave none for a CTA of that kernel which
+    has yet to allocate: both would wait for good.  (The attention's CTAs release their dependents before they allocate, and
+    one of them fits an SM beside a CTA of the pair kernel, which takes all 512 columns.)  And dependents are released
+    behind the allocation, for the same reason the other way round."""
+    import re
+    from test_kernel_sources_cpu import kernels, read
+    text = read("gemm_mxfp4.cu")
+    take = re.search(r"uint32_t take_tmem\(.*?\n\}", text, re.S).group(0)
+    assert take.index("alloc();") < take.index("pdl_trigger();")
+    for name, _, body in kernels(text):
+        wait = body.index("else pdl_wait();")
+        alloc = [m.start() for m in re.finditer(r"tmem_alloc(_pair)?\(", body)]
+        assert len(alloc) == 1 and wait < body.index("take_tmem(") < alloc[0], name
+        assert "pdl_trigger" not in body, name
